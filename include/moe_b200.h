@@ -487,6 +487,94 @@ MOE_API int moe_ep_combine(void* const* peers, int64_t ld_peer, const int32_t* o
                            const void* weights, int64_t hidden, void* out, int64_t ld_out,
                            int dtype, void* stream);
 
+/*
+ * Few tokens (decode).  No counterpart in the reference, whose layer pads every
+ * expert's rows to a tile; the result is triton_moe/moe.py:148-249's for up to 64
+ * tokens, in two launches: router logits (fp32), sigmoid, the top_k largest
+ * logits (equal ones: lower index; NaN above all, as torch.topk), weights
+ * p / (sum p + 1e-20) or p, up product, activation, down product, weighted sum.
+ * Sums are fp32 and nothing is rounded before the output, so near-equal logits
+ * that the storage type would merge are told apart.
+ *   x [num_tokens, hidden], router [num_experts, hidden], w1 [hidden,
+ *   total_width], w2 [total_width, hidden] (SwiGLU: [total_width / 2, hidden]),
+ *   out [num_tokens, hidden]: one dtype, 16-byte aligned, contiguous but for ld_x
+ *   (a multiple of 16 bytes) and ld_out.
+ *   group = 0: w1, w2 as above; scales NULL.  group = 32, 64 or 128: w1 and w2
+ *   packed by moe_int4_quantize / _pack with that group (w1 as one segment, w2
+ *   with one segment an expert), scales in dtype (bf16 or fp16); w2_blocks and
+ *   w2_groups are moe_int4_rows' of w2.
+ *   expert_weight_offsets [E+1], num_experts <= 256, top_k <= 32, hidden and
+ *   max_expert_width multiples of 16 up to 32768.  An expert whose offsets leave
+ *   the matrices, are no multiples of 16, or exceed max_expert_width adds
+ *   nothing and sets MOE_ERR_BAD_ARG in status.
+ *   workspace: moe_few_tokens_workspace_bytes(...) bytes, 16-byte aligned, any
+ *   contents; one per call that may run at the same time.
+ * num_tokens = 0 launches nothing.  moe_few_tokens_workspace_bytes returns -1
+ * for sizes out of range.
+ */
+MOE_API int64_t moe_few_tokens_workspace_bytes(int64_t num_tokens, int64_t hidden,
+                                               int num_experts, int top_k,
+                                               int64_t max_expert_width, int activation);
+MOE_API int moe_few_tokens(const void* x, int64_t num_tokens, int64_t ld_x, int64_t hidden,
+                           const void* router, int num_experts, const void* w1,
+                           const void* w1_scales, const void* w2, const void* w2_scales,
+                           int group, int64_t w2_blocks, int64_t w2_groups, int64_t total_width,
+                           const int32_t* expert_weight_offsets, int64_t max_expert_width,
+                           int top_k, int normalize, int activation, void* out, int64_t ld_out,
+                           void* workspace, int64_t workspace_bytes, int dtype, int* status,
+                           void* stream);
+
+/*
+ * 4-bit weights with group scales (no counterpart in the reference).  A weight
+ * [rows, cols] (multiples of 16) is (q - 8) * scale with q in 0..15 and one scale
+ * for `group` (32, 64 or 128) rows of a column.  row_offsets (HOST, ascending
+ * multiples of 16 from 0 to rows, num_segments + 1 of them, or NULL for one
+ * segment): groups start anew in each of up to 256 segments, e.g. each expert's
+ * rows of w2.  moe_int4_rows gives the block rows B and groups S: packed takes
+ * B * (cols / 16) * 512 bytes, scales [S, cols] in scale_dtype.
+ *   quantize: scale = amax / 7 rounded to scale_dtype, q = rint(w / scale) + 8
+ *   (ties to even) within 0..15; scale_dtype is the weight's, bf16 or fp16 for
+ *   fp32 weights.  A group holding a NaN or infinity reads back as NaN.
+ *   pack: the same layout from codes [rows, cols] of one byte (low 4 bits).
+ *   dequantize: (q - 8) * scale in dtype (the scales').
+ */
+MOE_API int moe_int4_rows(int64_t rows, int group, const int32_t* row_offsets, int num_segments,
+                          int64_t* blocks, int64_t* groups);
+MOE_API int moe_int4_quantize(const void* w, int64_t rows, int64_t cols, int64_t ld,
+                              int w_dtype, int group, const int32_t* row_offsets,
+                              int num_segments, void* packed, void* scales, int scale_dtype,
+                              void* stream);
+MOE_API int moe_int4_pack(const uint8_t* codes, int64_t rows, int64_t cols, int64_t ld,
+                          int group, const int32_t* row_offsets, int num_segments, void* packed,
+                          void* stream);
+MOE_API int moe_int4_dequantize(const void* packed, const void* scales, int64_t rows,
+                                int64_t cols, int group, const int32_t* row_offsets,
+                                int num_segments, void* out, int64_t ld, int dtype,
+                                void* stream);
+
+/*
+ * moe_grouped_gemm_up / _down with 4-bit weights, for a few rows an expert (the
+ * weights are read once for every 16 rows): down = 0: out [rows, max_expert_width]
+ * = act(x @ w1_e) over x [rows, hidden], total_width columns; down = 1: out [rows,
+ * hidden] = x[:, :w_e] @ w2_e over x [rows, max_expert_width], total_width rows,
+ * activation NONE.  Every element of out is written; rows of no expert (or beyond
+ * tokens_per_expert, when given) and columns >= w_e are zero.  rows <= 65536,
+ * dtype bf16 or fp16 (the scales').  For SwiGLU expert_weight_offsets step by
+ * 2 w_e.  blocks and groups: moe_int4_rows' of the weight.  workspace:
+ * moe_grouped_gemv_int4_workspace_bytes(rows, columns of the product) bytes
+ * (hidden, or max_expert_width, doubled for SwiGLU), as moe_few_tokens'.
+ */
+MOE_API int64_t moe_grouped_gemv_int4_workspace_bytes(int64_t rows, int64_t cols);
+MOE_API int moe_grouped_gemv_int4(const void* x, int64_t rows, int64_t ld_x, const void* w,
+                                  const void* scales, int group, int64_t blocks, int64_t groups,
+                                  int64_t hidden, int64_t total_width,
+                                  const int32_t* expert_token_offsets,
+                                  const int32_t* expert_weight_offsets,
+                                  const int32_t* tokens_per_expert, int num_experts,
+                                  int64_t max_expert_width, int activation, int down, void* out,
+                                  int64_t ld_out, void* workspace, int64_t workspace_bytes,
+                                  int dtype, int* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

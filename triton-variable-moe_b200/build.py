@@ -23,7 +23,8 @@ INCLUDE = HERE.parent / "include"
 OBJ_DIR = HERE / "_build"
 OUT = HERE / "moe_b200" / "libmoe_b200.so"
 
-SOURCES = ["route.cu", "router.cu", "permute.cu", "grouped_gemm.cu", "capi.cu", "ep.cu"]
+SOURCES = ["route.cu", "router.cu", "permute.cu", "grouped_gemm.cu", "capi.cu", "ep.cu",
+           "few_tokens.cu", "int4.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
     "-O3",

@@ -46,6 +46,29 @@ int build_row_map(const int32_t* indices, const int32_t* bin_ids, const int32_t*
                   cudaStream_t st);
 int gather_map_from_rows(const int32_t* row_asg, long long rows, int k, int32_t* gmap,
                          cudaStream_t st);
+long long few_tokens_workspace(long long T, long long H, int E, int k, long long max_width,
+                               int act);
+int few_tokens(const void* x, long long T, long long ldx, long long H, const void* router, int E,
+               const void* w1, const void* s1, const void* w2, const void* s2, int group,
+               long long blocks2, long long groups2, long long total, const int* off,
+               long long max_width, int k, int norm, int act, void* out, long long ldo, void* ws,
+               long long ws_bytes, int dtype, int* status, cudaStream_t st);
+long long grouped_int4_workspace(long long rows, long long cols);
+int grouped_int4(const void* x, long long rows, long long ldx, const void* w, const void* s,
+                 int group, long long blocks, long long groups, long long H, long long total,
+                 const int* tok_off, const int* off, const int* tok_cnt, int E,
+                 long long max_width, int act, int down, void* out, long long ldo, void* ws,
+                 long long ws_bytes, int dtype, int* status, cudaStream_t st);
+int int4_rows(long long K, int group, const int32_t* off, int n, long long* blocks,
+              long long* groups);
+int int4_quantize(const void* w, long long K, long long N, long long ld, int w_dtype, int group,
+                  const int32_t* off, int n, void* packed, void* scales, int s_dtype,
+                  cudaStream_t st);
+int int4_pack(const uint8_t* codes, long long K, long long N, long long ld, int group,
+              const int32_t* off, int n, void* packed, cudaStream_t st);
+int int4_dequantize(const void* packed, const void* scales, long long K, long long N, int group,
+                    const int32_t* off, int n, void* out, long long ld, int dtype,
+                    cudaStream_t st);
 }  // namespace moe
 
 namespace {
@@ -231,6 +254,73 @@ int moe_relu_squared_grad(const void* grad_out, const void* pre_act, int64_t row
                           int64_t ld, void* grad_act, int dtype, void* stream) {
   if (rows < 0 || cols < 0 || ld < cols) return MOE_ERR_BAD_ARG;
   return moe::relu2_grad(grad_out, pre_act, rows, cols, ld, grad_act, dtype, S(stream));
+}
+
+int64_t moe_few_tokens_workspace_bytes(int64_t num_tokens, int64_t hidden, int num_experts,
+                                       int top_k, int64_t max_expert_width, int activation) {
+  return moe::few_tokens_workspace(num_tokens, hidden, num_experts, top_k, max_expert_width,
+                                   activation);
+}
+
+int moe_few_tokens(const void* x, int64_t num_tokens, int64_t ld_x, int64_t hidden,
+                   const void* router, int num_experts, const void* w1, const void* w1_scales,
+                   const void* w2, const void* w2_scales, int group, int64_t w2_blocks,
+                   int64_t w2_groups, int64_t total_width, const int32_t* expert_weight_offsets,
+                   int64_t max_expert_width, int top_k, int normalize, int activation, void* out,
+                   int64_t ld_out, void* workspace, int64_t workspace_bytes, int dtype,
+                   int* status, void* stream) {
+  return moe::few_tokens(x, num_tokens, ld_x, hidden, router, num_experts, w1, w1_scales, w2,
+                         w2_scales, group, w2_blocks, w2_groups, total_width,
+                         expert_weight_offsets, max_expert_width, top_k, normalize, activation,
+                         out, ld_out, workspace, workspace_bytes, dtype, status, S(stream));
+}
+
+int moe_int4_rows(int64_t rows, int group, const int32_t* row_offsets, int num_segments,
+                  int64_t* blocks, int64_t* groups) {
+  if (!blocks || !groups) return MOE_ERR_BAD_ARG;
+  long long b = 0, g = 0;
+  const int rc = moe::int4_rows(rows, group, row_offsets, num_segments, &b, &g);
+  *blocks = b;
+  *groups = g;
+  return rc;
+}
+
+int moe_int4_quantize(const void* w, int64_t rows, int64_t cols, int64_t ld, int w_dtype,
+                      int group, const int32_t* row_offsets, int num_segments, void* packed,
+                      void* scales, int scale_dtype, void* stream) {
+  return moe::int4_quantize(w, rows, cols, ld, w_dtype, group, row_offsets, num_segments, packed,
+                            scales, scale_dtype, S(stream));
+}
+
+int moe_int4_pack(const uint8_t* codes, int64_t rows, int64_t cols, int64_t ld, int group,
+                  const int32_t* row_offsets, int num_segments, void* packed, void* stream) {
+  return moe::int4_pack(codes, rows, cols, ld, group, row_offsets, num_segments, packed,
+                        S(stream));
+}
+
+int moe_int4_dequantize(const void* packed, const void* scales, int64_t rows, int64_t cols,
+                        int group, const int32_t* row_offsets, int num_segments, void* out,
+                        int64_t ld, int dtype, void* stream) {
+  return moe::int4_dequantize(packed, scales, rows, cols, group, row_offsets, num_segments, out,
+                              ld, dtype, S(stream));
+}
+
+int64_t moe_grouped_gemv_int4_workspace_bytes(int64_t rows, int64_t cols) {
+  return moe::grouped_int4_workspace(rows, cols);
+}
+
+int moe_grouped_gemv_int4(const void* x, int64_t rows, int64_t ld_x, const void* w,
+                          const void* scales, int group, int64_t blocks, int64_t groups,
+                          int64_t hidden, int64_t total_width,
+                          const int32_t* expert_token_offsets,
+                          const int32_t* expert_weight_offsets, const int32_t* tokens_per_expert,
+                          int num_experts, int64_t max_expert_width, int activation, int down,
+                          void* out, int64_t ld_out, void* workspace, int64_t workspace_bytes,
+                          int dtype, int* status, void* stream) {
+  return moe::grouped_int4(x, rows, ld_x, w, scales, group, blocks, groups, hidden, total_width,
+                           expert_token_offsets, expert_weight_offsets, tokens_per_expert,
+                           num_experts, max_expert_width, activation, down, out, ld_out,
+                           workspace, workspace_bytes, dtype, status, S(stream));
 }
 
 }  // extern "C"

@@ -93,6 +93,16 @@ _SIGS = {
     "moe_ep_plan": [_I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P],
     "moe_ep_dispatch": [_P, _L, _L, _P, _I, _P, _P, _L, _P, _P, _P, _L, _I, _P],
     "moe_ep_combine": [_P, _L, _P, _P, _P, _P, _L, _I, _P, _L, _P, _L, _I, _P],
+    "moe_few_tokens_workspace_bytes": [_L, _L, _I, _I, _L, _I],
+    "moe_few_tokens": [_P, _L, _L, _L, _P, _I, _P, _P, _P, _P, _I, _L, _L, _L, _P, _L, _I, _I, _I,
+                       _P, _L, _P, _L, _I, _P, _P],
+    "moe_int4_rows": [_L, _I, _P, _I, _P, _P],
+    "moe_int4_quantize": [_P, _L, _L, _L, _I, _I, _P, _I, _P, _P, _I, _P],
+    "moe_int4_pack": [_P, _L, _L, _L, _I, _P, _I, _P, _P],
+    "moe_int4_dequantize": [_P, _P, _L, _L, _I, _P, _I, _P, _L, _I, _P],
+    "moe_grouped_gemv_int4_workspace_bytes": [_L, _L],
+    "moe_grouped_gemv_int4": [_P, _L, _L, _P, _P, _I, _L, _L, _L, _L, _P, _P, _P, _I, _L, _I, _I, _P,
+                              _L, _P, _L, _I, _P, _P],
 }
 _RESTYPE = {
     "moe_version": c_char_p,
@@ -101,6 +111,8 @@ _RESTYPE = {
     "moe_route_workspace_bytes": c_int64,
     "moe_router_head_workspace_floats": c_int64,
     "moe_up_down_dep_words": c_int64,
+    "moe_few_tokens_workspace_bytes": c_int64,
+    "moe_grouped_gemv_int4_workspace_bytes": c_int64,
 }
 
 EXPORTED = tuple(_SIGS)

@@ -35,12 +35,15 @@ import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
 from .kernels import (
+    Int4Weight,
     _ops,
     fused_route,
     grouped_gemm_down,
     grouped_gemm_up,
+    moe_few_tokens,
     padded_gather,
     padded_scatter,
+    quantize_int4,
 )
 
 
@@ -371,6 +374,31 @@ class TritonMoEMLP(nn.Module):
         self._join_aux(x.device)
         aux, f_i = self._aux_losses(router_logits, lse, head_losses, router_probs)
         return output, aux, f_i
+
+    # ------------------------------------------------------------------- decode
+    def decode(self, x: torch.Tensor,
+               experts: tuple[Int4Weight, Int4Weight] | None = None) -> torch.Tensor:
+        """The layer's output for a few tokens, for serving: x [..., n_embd] with at
+        most kernels.FEW_TOKENS_MAX (64) tokens in all -> output of x's shape, in two
+        launches (`forward` takes any number of tokens, and gradients and the
+        auxiliary losses, which this does not).  experts: `quantize_experts()`, to
+        run on 4-bit expert weights.  Logits, routing weights and the intermediate
+        stay fp32, so the result differs from `forward` by that rounding.  Call it
+        under torch.no_grad()."""
+        w1, w2 = (self.w1, self.w2) if experts is None else experts
+        out = moe_few_tokens(x.reshape(-1, x.shape[-1]), self.router.weight, w1, w2,
+                             self.expert_weight_offsets_t, self.max_expert_width,
+                             self.num_active_experts, self.norm_topk_prob)
+        return out.reshape(x.shape)
+
+    def quantize_experts(self, group_size: int = 64,
+                         dtype: torch.dtype | None = None) -> tuple[Int4Weight, Int4Weight]:
+        """w1 and w2 in 4 bits with group scales, for `decode` (and the kernels'
+        grouped_gemv_*_int4); a snapshot: quantise again after the weights change.
+        dtype: of the scales and of decode's x (default: the weights'; bf16 for
+        fp32 weights)."""
+        return (quantize_int4(self.w1, group_size, dtype=dtype),
+                quantize_int4(self.w2, group_size, row_offsets=self.expert_offsets, dtype=dtype))
 
     def _offsets(self, padded_bins, device):
         expert_token_offsets = torch.cat(
