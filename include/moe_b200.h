@@ -561,10 +561,12 @@ MOE_API int moe_int4_dequantize(const void* packed, const void* scales, int64_t 
  * tokens_per_expert, when given) and columns >= w_e are zero.  rows <= 65536,
  * dtype bf16 or fp16 (the scales').  For SwiGLU expert_weight_offsets step by
  * 2 w_e.  blocks and groups: moe_int4_rows' of the weight.  workspace:
- * moe_grouped_gemv_int4_workspace_bytes(rows, columns of the product) bytes
- * (hidden, or max_expert_width, doubled for SwiGLU), as moe_few_tokens'.
+ * moe_grouped_gemv_int4_workspace_bytes(...) bytes, as moe_few_tokens' (-1 for
+ * sizes out of range).
  */
-MOE_API int64_t moe_grouped_gemv_int4_workspace_bytes(int64_t rows, int64_t cols);
+MOE_API int64_t moe_grouped_gemv_int4_workspace_bytes(int64_t rows, int64_t hidden,
+                                                      int64_t max_expert_width, int activation,
+                                                      int down);
 MOE_API int moe_grouped_gemv_int4(const void* x, int64_t rows, int64_t ld_x, const void* w,
                                   const void* scales, int group, int64_t blocks, int64_t groups,
                                   int64_t hidden, int64_t total_width,

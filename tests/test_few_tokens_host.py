@@ -42,8 +42,9 @@ def test_workspace_sizes():
                 (1, 32784, 4, 2, 32, 0), (1, 64, 4, 2, 32784, 0)]:
         assert f(*bad) == -1, bad
     g = lib.moe_grouped_gemv_int4_workspace_bytes
-    assert g(1, 16) > 0 and g(0, 16) > 0
-    for bad in [(-1, 16), (65537, 16), (1, 8), (1, 65552)]:
+    assert g(1, 16, 16, 0, 1) > 0 and g(0, 16, 16, 2, 0) > 0
+    for bad in [(-1, 16, 16, 0, 0), (65537, 16, 16, 0, 0), (1, 8, 16, 0, 0), (1, 16, 40, 0, 0),
+                (1, 32784, 16, 0, 0), (1, 16, 32784, 0, 0), (1, 16, 16, 3, 0), (1, 16, 16, 1, 1)]:
         assert g(*bad) == -1, bad
 
 

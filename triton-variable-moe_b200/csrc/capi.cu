@@ -53,7 +53,8 @@ int few_tokens(const void* x, long long T, long long ldx, long long H, const voi
                long long blocks2, long long groups2, long long total, const int* off,
                long long max_width, int k, int norm, int act, void* out, long long ldo, void* ws,
                long long ws_bytes, int dtype, int* status, cudaStream_t st);
-long long grouped_int4_workspace(long long rows, long long cols);
+long long grouped_int4_workspace(long long rows, long long H, long long max_width, int act,
+                                 int down);
 int grouped_int4(const void* x, long long rows, long long ldx, const void* w, const void* s,
                  int group, long long blocks, long long groups, long long H, long long total,
                  const int* tok_off, const int* off, const int* tok_cnt, int E,
@@ -305,8 +306,10 @@ int moe_int4_dequantize(const void* packed, const void* scales, int64_t rows, in
                               ld, dtype, S(stream));
 }
 
-int64_t moe_grouped_gemv_int4_workspace_bytes(int64_t rows, int64_t cols) {
-  return moe::grouped_int4_workspace(rows, cols);
+int64_t moe_grouped_gemv_int4_workspace_bytes(int64_t rows, int64_t hidden,
+                                              int64_t max_expert_width, int activation,
+                                              int down) {
+  return moe::grouped_int4_workspace(rows, hidden, max_expert_width, activation, down);
 }
 
 int moe_grouped_gemv_int4(const void* x, int64_t rows, int64_t ld_x, const void* w,

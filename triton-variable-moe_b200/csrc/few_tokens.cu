@@ -16,25 +16,30 @@
 //                an eighth of the hidden size, the sums exchanged over
 //                distributed shared memory): it costs one or two microseconds of
 //                L2 reads and needs no launch and no grid-wide wait of its own.
-//                Then the grid's teams of four warps share the units (expert,
-//                64-column tile, slice of the reduction) and write fp32 partial
-//                sums of u.
-//   down kernel  The units (expert, slice of its width, 64-column tile of the
-//                hidden size); the partial sums of u are added and activated as
-//                they are loaded.  The team that finishes a column tile's last
-//                unit (a counter per tile, zeroed by the up kernel) adds the
-//                tile's partial sums in a fixed order, weights them and writes
-//                the output: results do not depend on timing.
-// Nothing waits in a loop: the only waits are hardware barriers and the grid
-// dependency between the two launches.
+//                Then the grid's teams of four warps share the items (expert,
+//                64-column tile, up to 8 NG of its tokens).  With few items each
+//                is cut into slices of the reduction, all in one cluster; the
+//                team that finishes an item's last slice (a counter in shared
+//                memory) adds them in order, applies the activation and writes h.
+//   down kernel  The units (slice of an expert's width, 64-column tile of the
+//                hidden size).  The team that finishes a column tile's last unit
+//                (a counter per tile, zeroed by the up kernel) adds the tile's
+//                partial sums in a fixed order, weights them and writes the
+//                output: results do not depend on timing.
+// No block waits for another but at hardware barriers and the grid dependency
+// between the two launches; a warp's wait for its own copies is bounded.
 #include <cooperative_groups.h>
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 
 #include <atomic>
 #include <cstdint>
+#include <mutex>
 
 #include "few_tokens.cuh"
 #include "moe_internal.h"
+#include "sm100_ptx.cuh"
 
 namespace moe {
 namespace {
@@ -50,24 +55,39 @@ constexpr int kThreads = 512;     // 16 warps: at 128 registers a thread the SM 
 constexpr int kWarps = kThreads / 32;
 constexpr int kTeam = 4;          // warps that share a unit (they split its reduction)
 constexpr int kTeams = kWarps / kTeam;
+constexpr int kTeamThreads = kTeam * 32;
 constexpr int kTile = 64;         // columns of a unit
 constexpr int kRedLd = kTile + 4;
 constexpr int kMaxSlices = 16;
+constexpr int kMaxLocal = 256;    // sliced items of a cluster
+constexpr int kMaxDepth = 4;
+constexpr int kAddTokens = 8;     // up to this many, the down kernel writes the output
 constexpr int kMaxWidth = 32768;  // hidden size and expert width: item counts stay 32-bit
 
-template <typename L, int NG>
-struct Shape {
-  static constexpr int kTok = 8 * NG;
-};
-template <int NG>
-struct Shape<Dense32, NG> {
-  static constexpr int kTok = 4 * NG;
-};
-
 __host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+// Outputs of a 64-column tile: a gated activation's tile is 32 gate and 32 up columns.
+__host__ __device__ inline int tile_outputs(int act) { return act == ACT_SWIGLU ? 32 : 64; }
+__host__ __device__ inline int group_count(int rows, int shift) {
+  return (rows + (1 << shift) - 1) >> shift;
+}
 
 // ---- what both kernels of the layer know -----------------------------------
+// The experts that have rows, in order (built by the up kernel).
+struct Active {
+  int n[kMaxExperts];      // rows
+  int base[kMaxExperts];   // first row in expert-sorted order
+  int first[kMaxExperts];  // first column of w1 (grouped: of the offsets)
+  int width[kMaxExperts];  // intermediate width
+  int kb[kMaxExperts];     // packed w2: first block row, first group
+  int sg[kMaxExperts];
+  int item[kMaxExperts];   // first work item
+};
+constexpr int kActiveArrays = 7;
+// The same numbers for the down kernel, in the workspace.
+enum PlanWord : int { PLAN_ACTIVE = 0, PLAN_LENGTH = 1, PLAN_ITEMS = 2, PLAN_WORDS = 32 };
+
 struct LayerParams {
+  CUtensorMap map1, map2;    // dense w1, w2
   const void* x;
   long long ldx;
   const void* router;
@@ -79,59 +99,50 @@ struct LayerParams {
   int T, H, E, k, norm, act, total, max_width;
   int shift;                 // log2 of the group
   int blocks2, groups2;      // block rows and groups of the packed w2
+  int down_teams;            // teams of the down kernel's grid
+  int smem_work;             // up kernel: bytes before its UpSmem
   void* out;
   long long ldo;
   // workspace
-  unsigned long long* mask;  // [E] tokens of each expert
-  int* sel;                  // [T * k]
+  int* plan;                 // [PLAN_WORDS], then kActiveArrays x [E]
+  int* slot;                 // [T * k] active expert of an assignment (-1: none)
+  int* row;                  // [T * k] its expert-sorted row
   float* wgt;                // [T * k]
-  int* info;                 // [0]: slices of u
   int* ticket;               // [tiles of the hidden size]
-  float* u;                  // [slices][T * k][ldu]
+  float* u;                  // [slices][T * k][ldu]: partial sums of sliced items
   long long ldu;
+  void* h;                   // [T * k][ldh]: see HiddenSource
+  long long ldh;
   float* y;                  // [slices][T * k][H]
   int max_slices;
   int* status;
 };
 
-// Per-expert numbers, in shared memory (16-byte vectors of floats follow them).
-struct alignas(16) Meta {
-  int n[kMaxExperts];      // rows (0 when the expert's offsets are refused)
-  int base[kMaxExperts];   // first row in expert-sorted order
-  int first[kMaxExperts];  // first column of w1 (layer: the offsets' own units)
-  int width[kMaxExperts];  // intermediate width
-  int item[kMaxExperts + 1];  // prefix of the work items
-  int kb[kMaxExperts];     // packed w2: first block row, first group
-  int sg[kMaxExperts];
-  int scan[kWarps + 1];
+// What every kernel here keeps in shared memory (16-byte vectors follow it).
+struct alignas(16) Common {
+  Active act;
+  unsigned long long bar[kWarps][kMaxDepth];
+  int plan[4];  // number of active experts, items, rounds of a slice
+  int last[kTeams];
+  int abort;
 };
 
-// Exclusive prefix sum over the block's threads; every thread also gets the total.
-__device__ __forceinline__ int block_scan(int v, int* buf, int* total) {
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+// Exclusive prefix sum over a warp; `total` gets the sum.
+__device__ __forceinline__ int warp_scan(int v, int* total) {
+  const int lane = threadIdx.x & 31;
   int s = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int q = __shfl_up_sync(0xffffffffu, s, o);
     if (lane >= o) s += q;
   }
-  __syncthreads();  // buf may still be read from a call before
-  if (lane == 31) buf[w] = s;
-  __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int i = 0; i < kWarps; ++i) {
-    const int q = buf[i];
-    before += i < w ? q : 0;
-    all += q;
-  }
-  *total = all;
-  return before + s - v;
+  *total = __shfl_sync(0xffffffffu, s, 31);
+  return s - v;
 }
 
-// The expert whose items hold index i (item is an exclusive prefix, E + 1 long).
-__device__ __forceinline__ int find_item(const int* item, int E, int i) {
-  int lo = 0, hi = E - 1;
+// The active expert whose items hold index i.
+__device__ __forceinline__ int find_item(const int* item, int n, int i) {
+  int lo = 0, hi = n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (item[mid] <= i) lo = mid; else hi = mid - 1;
@@ -140,69 +151,262 @@ __device__ __forceinline__ int find_item(const int* item, int E, int i) {
 }
 
 __device__ __forceinline__ void team_sync(int team) {
-  asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(kTeam * 32) : "memory");
+  asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(kTeamThreads) : "memory");
 }
 
-// Rounds (a step by each warp of a team) of a slice: enough slices that every
-// team of the grid has a few units, and no more (a slice costs its partial
-// sums); never more than the workspace holds.
-__device__ __forceinline__ int slice_rounds(long long all_rounds, int most, int teams,
-                                            int max_slices) {
-  const int want = static_cast<int>(min(all_rounds / (4ll * teams), 1ll << 20));
-  return max(max(want, 1), ceil_div(most, max_slices));
+// Where unit i lies.  Finding it takes a search and a few divisions, so a warp's
+// lanes do it for 32 units of their team at once and hand them out by shuffle.
+struct Place {
+  unsigned a, b;  // e | tile << 8 | slice << 20; pass
+  __device__ __forceinline__ Place() {}
+  __device__ __forceinline__ Place(int e, int tile, int slice, int pass)
+      : a(static_cast<unsigned>(e) | static_cast<unsigned>(tile) << 8 |
+          static_cast<unsigned>(slice) << 20),
+        b(static_cast<unsigned>(pass)) {}
+};
+static_assert(kMaxExperts <= 256 && kMaxWidth / 32 <= 4096, "bits of a place");
+
+// One unit of a team.
+struct Unit {
+  Strip strip;
+  int begin;           // first reduction row
+  int count;           // vectors
+  int row;             // first of them in expert-sorted order
+  int e, tile, slice;  // active expert, column tile, slice of the reduction
+  int pass;            // first vector within the expert
+  __device__ __forceinline__ void set(const Place& w, int vectors) {
+    e = static_cast<int>(w.a & 255);
+    tile = static_cast<int>(w.a >> 8 & 4095);
+    slice = static_cast<int>(w.a >> 20);
+    pass = static_cast<int>(w.b) * vectors;
+  }
+};
+
+// The strip of an up product's tile: 64 columns, or 32 gate and their 32 up columns.
+__device__ __forceinline__ void up_strip(Strip& s, int first, int width, int act, int tile, int H,
+                                         int shift) {
+  s.row = 0;
+  s.kb = s.sg = 0;
+  s.groups = group_count(H, shift);
+  if (act == ACT_SWIGLU) {
+    s.col = first + tile * 32;
+    s.lo = s.hi = min(32, width - tile * 32);
+    s.jump = width;
+  } else {
+    s.col = first + tile * 64;
+    s.lo = min(32, width - tile * 64);
+    s.hi = min(32, max(0, width - tile * 64 - 32));
+    s.jump = 32;
+  }
+}
+__device__ __forceinline__ void down_strip(Strip& s, const Active& a, int e, int row, int tile,
+                                           int H, int shift) {
+  s.row = row;
+  s.col = tile * kTile;
+  s.lo = min(32, H - s.col);
+  s.hi = min(32, max(0, H - s.col - 32));
+  s.jump = 32;
+  s.kb = a.kb[e];
+  s.sg = a.sg[e];
+  s.groups = group_count(a.width[e], shift);
 }
 
-// Adds the team's partial sums and writes rows [0, count) x cols of the unit.
-template <int TOK>
-__device__ __forceinline__ void team_store(const float* red, int count, int cols, float* dst,
-                                           long long ldd) {
-  const int i0 = threadIdx.x % (kTeam * 32);
-  for (int i = i0; i < TOK * (kTile / 4); i += kTeam * 32) {
-    const int tok = i / (kTile / 4), c = 4 * (i % (kTile / 4));
-    if (tok < count && c < cols) {
-      const float* p = red + tok * kRedLd + c;
-      float4 v = *reinterpret_cast<const float4*>(p);
-#pragma unroll
-      for (int w = 1; w < kTeam; ++w) {
-        const float4 q = *reinterpret_cast<const float4*>(p + w * TOK * kRedLd);
-        v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
+// Bounded wait for a phase of a copy barrier.  false: it ran out, here or in
+// another warp (abort).
+__device__ __forceinline__ bool ring_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*abort) return false;
+    if (global_timer_ns() - t0 > MOE_WAIT_NS) {
+      *abort = 1;
+      return false;
+    }
+  }
+  return true;
+}
+
+// Runs units i, i + stride, ... < total of a team.  Every warp copies its steps
+// (begin + (wr + 4 j) kStep) into its ring as far ahead as it is deep, on into its
+// next units, so the loads go on during the reduction and the output of a unit.
+// place(i) finds a unit, unit(place) describes it, source(unit) gives its vectors, and
+// finish(i, unit) finds the unit's sums in red (see unit_sum) between team barriers.
+template <typename L, int NG, typename Find, typename MakeUnit, typename MakeSource,
+          typename Finish>
+__device__ __forceinline__ void run_units(int i, int stride, int total, const Matrix& m,
+                                          unsigned char* work, float* red, Common& c, Find place,
+                                          MakeUnit unit, MakeSource source, Finish finish) {
+  constexpr int kRows = kTeam * L::kStep, TOK = L::template kTokens<NG>;
+  constexpr int D = L::template kDepth<NG>;
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const int team = wid / kTeam, wr = wid % kTeam;
+  const uint32_t ring = smem_u32(work) + wid * (D * L::kStage);
+  const uint32_t bars = smem_u32(&c.bar[wid][0]);
+  const typename L::Lane at(lane, m.gated);
+  using Src = decltype(source(unit(Place())));
+  const int start = i;
+  // the n-th unit of the team
+  auto nth = [&](int n, Place& mine) {
+    if (n % 32 == 0) {
+      const int first = start + (n + lane) * stride;
+      if (first < total) mine = place(first);
+    }
+    Place q;
+    q.a = __shfl_sync(0xffffffffu, mine.a, n % 32);
+    q.b = __shfl_sync(0xffffffffu, mine.b, n % 32);
+    return unit(q);
+  };
+
+  int copied = 0, used = 0;  // steps
+  // the copying side: strip of the team's cn-th unit, next step at row ck
+  int cn = -1, ck = 0;
+  bool more = true;
+  Place ahead(0, 0, 0, 0), here(0, 0, 0, 0);
+  Unit cu;
+  cu.strip.end = 0;
+  // the multiplying side
+  int k = 0, n = -1;
+  Unit u;
+  u.strip.end = 0;
+  float acc[4][NG][4];
+  typename L::template Vectors<NG, Src> v;
+  Src src;
+  while (true) {
+    while (more && copied - used < D) {
+      if (ck >= cu.strip.end) {
+        ++cn;
+        more = start + cn * stride < total && !c.abort;
+        if (more) {
+          cu = nth(cn, ahead);
+          ck = cu.begin + wr * L::kStep;
+        }
+      } else {
+        const int slot = copied % D;
+        if (lane == 0) L::issue(m, cu.strip, ck, ring + slot * L::kStage, bars + 8 * slot);
+        ++copied;
+        ck += kRows;
       }
-      *reinterpret_cast<float4*>(dst + static_cast<long long>(tok) * ldd + c) = v;
+    }
+    if (k < u.strip.end) {
+      const int slot = used % D;
+      v.load(src, u.strip, k, lane);
+      if (used < copied) ring_wait(bars + 8 * slot, (used / D) & 1, &c.abort);
+      L::template step<NG, Src>(acc, at, m, u.strip, k, ring + slot * L::kStage, lane, v);
+      __syncwarp();  // the step has been read by every lane: its place is free
+      ++used;
+      k += kRows;
+    } else {
+      if (n >= 0) {
+        // warps 2 and 3 leave their sums, 0 and 1 add theirs to them
+        float* mine = red + (wr & 1) * TOK * kRedLd;
+        if (wr >= 2) L::template store<NG, kRedLd, false>(acc, lane, mine);
+        team_sync(team);
+        if (wr < 2) L::template store<NG, kRedLd, true>(acc, lane, mine);
+        team_sync(team);
+        finish(i, u);
+        team_sync(team);
+        i += stride;
+      }
+      if (i >= total) break;
+      u = nth(++n, here);
+      k = u.begin + wr * L::kStep;
+      src = source(u);
+      v.rows(src, u.count, lane);
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[a][g][j] = 0.f;
+    }
+  }
+  // after an abort: copies still in flight land before the block ends
+  for (; used < copied; ++used) {
+    const uint64_t t0 = global_timer_ns();
+    while (!mbar_try_wait(bars + 8 * (used % D), (used / D) & 1) &&
+           global_timer_ns() - t0 <= MOE_WAIT_NS) {
     }
   }
 }
 
-// Expert e's strip of 64 columns from `col` of a matrix whose reduction rows of
-// this expert start at `row`, up to reduction row `end`.
-template <typename L>
-struct Strips;
+// Before a kernel's first copies: the warp's barriers, each for one arrival (its
+// own lane's) a phase.
+template <int D>
+__device__ __forceinline__ void ring_init(Common& c) {
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  if (lane < D) {
+    mbar_init(reinterpret_cast<uint64_t*>(&c.bar[wid][lane]), 1);
+    fence_barrier_init();
+  }
+  __syncwarp();
+  if (threadIdx.x == 0) c.abort = 0;  // (seen by all after the next block barrier)
+}
+
+// The unit's sums of vector `tok`, columns c .. c + 3.
+template <int TOK>
+__device__ __forceinline__ float4 unit_sum(const float* red, int tok, int c) {
+  const float4 a = *reinterpret_cast<const float4*>(red + tok * kRedLd + c);
+  const float4 b = *reinterpret_cast<const float4*>(red + (TOK + tok) * kRedLd + c);
+  return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
+}
+__device__ __forceinline__ void add4(float4& a, const float4& b) {
+  a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+}
 template <typename T>
-struct Strips<Dense16<T>> {
-  static __device__ __forceinline__ typename Dense16<T>::Strip make(
-      const void* w, const void*, long long ld, long long row, int, int, int, int col, int end,
-      int cols, int) {
-    return {static_cast<const T*>(w) + row * ld + col, ld, end, cols};
+__device__ __forceinline__ void store4(T* d, float4 v, bool vec) {
+  if (vec) {
+    if constexpr (sizeof(T) == 2)
+      *reinterpret_cast<uint2*>(d) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+    else
+      *reinterpret_cast<float4*>(d) = v;
+  } else {
+    d[0] = from_f<T>(v.x);
+    d[1] = from_f<T>(v.y);
+    d[2] = from_f<T>(v.z);
+    d[3] = from_f<T>(v.w);
   }
-};
-template <>
-struct Strips<Dense32> {
-  static __device__ __forceinline__ Dense32::Strip make(const void* w, const void*, long long ld,
-                                                        long long row, int, int, int, int col,
-                                                        int end, int cols, int) {
-    return {static_cast<const float*>(w) + row * ld + col, ld, end, cols};
+}
+
+// Shared memory of the teams: rings (1 KB aligned for the swizzle), then two sum
+// buffers a team.
+template <typename L, int NG>
+constexpr int kRingBytes = kWarps * L::template kDepth<NG> * L::kStage;
+template <typename L, int NG>
+constexpr int kRedFloats = 2 * L::template kTokens<NG> * kRedLd;  // a team
+template <typename L, int NG>
+constexpr int kWorkBytes = kRingBytes<L, NG> + 4 * kTeams * kRedFloats<L, NG>;
+
+// Length of a slice, in rounds (a step by each warp of a team), that finishes
+// first for items of `rounds` rounds each and `passes` each: whole waves of units
+// over the teams, a unit's own cost being `own` and a round's four quarter rounds;
+// what a slice adds to the final sum counts a quarter.  One warp; lane 0's result
+// is everyone's.
+__device__ __forceinline__ int slice_length(int i) {  // 1 2 3 4 6 8 12 16 .. 512
+  return i == 0 ? 1 : i % 2 ? 2 << (i - 1) / 2 : 3 << (i - 2) / 2;
+}
+constexpr int kLengths = 18;
+static_assert(kMaxWidth <= 512 * 64, "the last length is the rounds of the longest reduction");
+template <typename Units>
+__device__ __forceinline__ int plan_length(int most, int teams, int max_slices, int own,
+                                           Units units) {
+  long long best = 0x7fffffffffffffffll;
+  int best_len = 0;
+#pragma unroll 1
+  for (int i = 0; i < kLengths; ++i) {
+    const int len = slice_length(i);
+    const int parts = ceil_div(most, len);
+    if (parts <= max_slices) {
+      const long long waves = (units(len) + teams - 1) / teams;
+      const long long cost = waves * (4 * min(len, most) + own) + parts;
+      if (cost < best) {
+        best = cost;
+        best_len = len;
+      }
+    }
+    if (len >= most) break;
   }
-};
-template <typename T>
-struct Strips<Int4<T>> {
-  static __device__ __forceinline__ typename Int4<T>::Strip make(
-      const void* w, const void* sc, long long ld, long long, int kb, int sg, int groups, int col,
-      int end, int cols, int shift) {
-    const long long nb = ld / 16;
-    return {static_cast<const uint4*>(w) + (kb * nb + col / 16) * 32, nb,
-            static_cast<const T*>(sc) + static_cast<long long>(sg) * ld + col, ld, end, cols,
-            shift, groups};
-  }
-};
+  return best_len;
+}
 
 // ---- routing --------------------------------------------------------------
 // This CTA's partial logits over reduction range [k_lo, k_hi): log[t][E16].
@@ -367,66 +571,125 @@ __device__ __forceinline__ void choose(const float (&v)[kMaxExperts / 32], int E
   *wgt = w;
 }
 
-// ---- the layer's per-expert numbers ----------------------------------------
-// From the token masks (shared) and the offsets (global): rows, first rows,
-// widths.  Offsets that leave the matrices, or are not in steps of 16, empty the
-// expert and set the status word.
-__device__ __forceinline__ void layer_meta(const LayerParams& p, const unsigned long long* mask,
-                                           Meta& m) {
-  const int e = threadIdx.x;
+// ---- the layer's active experts ----------------------------------------------
+struct alignas(16) UpSmem {
+  Common c;
+  unsigned long long mask[kMaxExperts];      // tokens of each expert
+  unsigned long long act_mask[kMaxExperts];  // of each active expert
+  int off[kMaxExperts + 1];
+  int slot[kMaxExperts];  // active expert of an expert (-1: none)
+  int base[kMaxExperts];  // first expert-sorted row of an expert
+  int ticket[kMaxLocal];  // slices done of the cluster's items (rank 0's is used)
+};
+static_assert(sizeof(UpSmem) % 16 == 0, "16-byte vectors follow");
+
+// One warp: from the token masks and the offsets, the experts that have rows and
+// columns, and their (pass, tile) items.  Offsets that leave the matrices, or are
+// not in steps of 16, empty the expert and set the status word.
+template <int TOK>
+__device__ __forceinline__ void find_active(const LayerParams& p, UpSmem& s) {
+  const int lane = threadIdx.x & 31;
   const int gated = p.act == ACT_SWIGLU ? 2 : 1;
-  int n = 0, a = 0, w = 0;
-  bool ok = true;
-  if (e < p.E) {
-    n = __popcll(mask[e]);
-    a = p.off[e];
-    const int b = p.off[e + 1];
-    ok = a >= 0 && b >= a && b <= p.total && a % (16 * gated) == 0 &&
-         (b - a) % (16 * gated) == 0 && (b - a) / gated <= p.max_width;
-    w = ok ? (b - a) / gated : 0;
-  }
-  int all;
-  const int base = block_scan(n, m.scan, &all);
-  int kb = 0, sg = 0;
-  if (p.shift) {
-    kb = block_scan(ceil_div(w, 64), m.scan, &all);
-    sg = block_scan((w + (1 << p.shift) - 1) >> p.shift, m.scan, &all);
-  }
-  if (e < p.E) {
-    // a packed w2 quantised for other offsets
-    if (p.shift && (kb + ceil_div(w, 64) > p.blocks2 ||
-                    sg + ((w + (1 << p.shift) - 1) >> p.shift) > p.groups2))
-      ok = false;
+  int active = 0, base = 0, item = 0, kb = 0, sg = 0;
+#pragma unroll 1
+  for (int e0 = 0; e0 < p.E; e0 += 32) {
+    const int e = e0 + lane;
+    int n = 0, a = 0, w = 0;
+    bool ok = true;
+    if (e < p.E) {
+      n = __popcll(s.mask[e]);
+      a = s.off[e];
+      const int b = s.off[e + 1];
+      ok = a >= 0 && b >= a && b <= p.total && a % (16 * gated) == 0 &&
+           (b - a) % (16 * gated) == 0 && (b - a) / gated <= p.max_width;
+      w = ok ? (b - a) / gated : 0;
+    }
+    int total;
+    const int my_base = base + warp_scan(n, &total);
+    base += total;
+    int my_kb = 0, my_sg = 0;
+    if (p.shift) {
+      const int blocks = ceil_div(w, 64), groups = group_count(w, p.shift);
+      my_kb = kb + warp_scan(blocks, &total);
+      kb += total;
+      my_sg = sg + warp_scan(groups, &total);
+      sg += total;
+      // a packed w2 quantised for other offsets
+      if (my_kb + blocks > p.blocks2 || my_sg + groups > p.groups2) ok = false;
+    }
     if (!ok && p.status && blockIdx.x == 0) *p.status = kStatusBadArg;
-    m.n[e] = ok ? n : 0;
-    m.base[e] = base;
-    m.first[e] = a;
-    m.width[e] = ok ? w : 0;
-    m.kb[e] = kb;
-    m.sg[e] = sg;
+    const bool here = ok && n > 0 && w > 0;
+    const int my_items = here ? ceil_div(n, TOK) * ceil_div(w, tile_outputs(p.act)) : 0;
+    const int my_item = item + warp_scan(my_items, &total);
+    item += total;
+    const unsigned who = __ballot_sync(0xffffffffu, here);
+    const int at = active + __popc(who & ((1u << lane) - 1));
+    active += __popc(who);
+    if (e < p.E) {
+      s.slot[e] = here ? at : -1;
+      s.base[e] = my_base;
+    }
+    if (here) {
+      s.c.act.n[at] = n;
+      s.c.act.base[at] = my_base;
+      s.c.act.first[at] = a;
+      s.c.act.width[at] = w;
+      s.c.act.kb[at] = my_kb;
+      s.c.act.sg[at] = my_sg;
+      s.c.act.item[at] = my_item;
+      s.act_mask[at] = s.mask[e];
+    }
+  }
+  if (lane == 0) {
+    s.c.plan[0] = active;
+    s.c.plan[1] = item;
+  }
+}
+
+// One warp: the down kernel's slice length and items, into the workspace.
+template <int TOK, int ROUND>
+__device__ __forceinline__ void plan_down(const LayerParams& p, const Active& act, int active) {
+  const int lane = threadIdx.x & 31, tiles = ceil_div(p.H, kTile);
+  int widest = 0;
+  for (int j = lane; j < active; j += 32) widest = max(widest, act.width[j]);
+  widest = __reduce_max_sync(0xffffffffu, widest);
+  const int len = plan_length(max(1, ceil_div(widest, ROUND)), p.down_teams, p.max_slices, 4,
+                              [&](int length) {
+    int n = 0;
+    for (int j = lane; j < active; j += 32)
+      n += ceil_div(act.n[j], TOK) * ceil_div(ceil_div(act.width[j], ROUND), length);
+    return static_cast<long long>(__reduce_add_sync(0xffffffffu, n)) * tiles;
+  });
+  int items = 0;
+  for (int j0 = 0; j0 < active; j0 += 32) {
+    const int j = j0 + lane;
+    int n = 0, total;
+    if (j < active) n = ceil_div(act.n[j], TOK) * ceil_div(ceil_div(act.width[j], ROUND), len);
+    const int before = items + warp_scan(n, &total);
+    items += total;
+    if (j < active) p.plan[PLAN_WORDS + 6 * p.E + j] = before;
+  }
+  if (lane == 0) {
+    p.plan[PLAN_ACTIVE] = active;
+    p.plan[PLAN_LENGTH] = len;
+    p.plan[PLAN_ITEMS] = items;
   }
 }
 
 // ---- up kernel ---------------------------------------------------------------
-struct alignas(16) UpSmem {
-  Meta m;
-  unsigned long long mask[kMaxExperts];
-  int sel[kMaxTokens * kMaxTopK];
-  float wgt[kMaxTokens * kMaxTopK];
-  int list[kMaxTokens * kMaxTopK];  // token of each expert-sorted row
-};
-
-static_assert(sizeof(Meta) % 16 == 0 && sizeof(UpSmem) % 16 == 0, "16-byte vectors follow");
-
 template <typename L, int NG>
-__global__ void __launch_bounds__(kThreads, 1) few_up_kernel(const LayerParams p) {
+__global__ void __launch_bounds__(kThreads, 1)
+    few_up_kernel(const __grid_constant__ LayerParams p) {
   using T = typename L::Elem;
-  constexpr int TOK = Shape<L, NG>::kTok;
-  extern __shared__ __align__(16) unsigned char raw[];
-  UpSmem& s = *reinterpret_cast<UpSmem*>(raw);
-  const int lde = ceil_div(p.E, 16) * 16;
-  float* log = reinterpret_cast<float*>(raw + sizeof(UpSmem));
-  float* part = log + p.T * lde;  // the routing's partial sums, then the teams'
+  constexpr int TOK = L::template kTokens<NG>, kRound = kTeam * L::kStep;
+  extern __shared__ __align__(1024) unsigned char raw[];
+  unsigned char* work = raw;  // rings first: 1 KB aligned
+  const int lde = ceil_div(p.E, 16) * 16, A = p.T * p.k;
+  float* log = reinterpret_cast<float*>(work);  // the routing's sums, before the rings
+  float* part = log + p.T * lde;
+  UpSmem& s = *reinterpret_cast<UpSmem*>(raw + p.smem_work);
+  int* sel_s = reinterpret_cast<int*>(raw + p.smem_work + sizeof(UpSmem));
+  float* wgt_s = reinterpret_cast<float*>(sel_s + A);
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = static_cast<int>(cluster.block_rank());
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
@@ -434,22 +697,27 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(const LayerParams p
   asm volatile("griddepcontrol.wait;" ::: "memory");
   // every block of this grid runs by the time the last one gets here
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  for (int e = tid; e <= p.E; e += kThreads) s.off[e] = p.off[e];
+  for (int e = tid; e < p.E; e += kThreads) s.mask[e] = 0;
+  for (int i = tid; i < kMaxLocal; i += kThreads) s.ticket[i] = 0;
+  ring_init<L::template kDepth<NG>>(s.c);
 
   // routing: an eighth of the hidden size, then tokens rank, rank + 8, ...
   const int per = ceil_div(ceil_div(p.H, 32), kCluster) * 32;
   partial_logits<T>(p, min(rank * per, p.H), min((rank + 1) * per, p.H), part, log, lde);
-  for (int e = tid; e < p.E; e += kThreads) s.mask[e] = 0;
   cluster.sync();
   for (int t = rank + kCluster * wid; t < p.T; t += kCluster * kWarps) {
     float v[kMaxExperts / 32];
 #pragma unroll
     for (int j = 0; j < kMaxExperts / 32; ++j) {
-      const int e = 32 * j + lane;
       v[j] = 0.f;
-      if (e < p.E) {
+      if (32 * j < p.E) {
+        const int e = min(32 * j + lane, p.E - 1);
+        float q[kCluster];
 #pragma unroll
-        for (int c = 0; c < kCluster; ++c)
-          v[j] += cluster.map_shared_rank(log, c)[t * lde + e];
+        for (int c = 0; c < kCluster; ++c) q[c] = cluster.map_shared_rank(log, c)[t * lde + e];
+#pragma unroll
+        for (int c = 0; c < kCluster; ++c) v[j] += q[c];
       }
     }
     int sel;
@@ -458,181 +726,350 @@ __global__ void __launch_bounds__(kThreads, 1) few_up_kernel(const LayerParams p
     if (lane < p.k) {
 #pragma unroll
       for (int c = 0; c < kCluster; ++c) {
-        cluster.map_shared_rank(s.sel, c)[t * p.k + lane] = sel;
-        cluster.map_shared_rank(s.wgt, c)[t * p.k + lane] = wgt;
+        cluster.map_shared_rank(sel_s, c)[t * p.k + lane] = sel;
+        cluster.map_shared_rank(wgt_s, c)[t * p.k + lane] = wgt;
+        // (32-bit words: 64-bit atomics of several CTAs on one shared word lose bits)
+        atomicOr(reinterpret_cast<unsigned*>(cluster.map_shared_rank(s.mask, c) + sel) + (t >> 5),
+                 1u << (t & 31));
       }
     }
   }
   cluster.sync();
 
-  const int A = p.T * p.k;
-  for (int a = tid; a < A; a += kThreads) atomicOr(&s.mask[s.sel[a]], 1ull << (a / p.k));
-  __syncthreads();
-  layer_meta(p, s.mask, s.m);
-  const int gated = p.act == ACT_SWIGLU ? 2 : 1;
-  int items = 0;  // (pass, tile) pairs of this thread's expert
-  if (tid < p.E)
-    items = ceil_div(s.m.n[tid], TOK) * ceil_div(gated * s.m.width[tid], kTile);
-  int U;
-  const int before = block_scan(items, s.m.scan, &U);
-  if (tid < p.E) s.m.item[tid] = before;
-  for (int a = tid; a < A; a += kThreads) {
-    const int e = s.sel[a], t = a / p.k;
-    s.list[s.m.base[e] + __popcll(s.mask[e] & ((1ull << t) - 1))] = t;
-  }
-  const int teams = gridDim.x * kTeams;
-  constexpr int kRound = kTeam * L::kStep;
+  const int clusters = gridDim.x / kCluster, teams = gridDim.x * kTeams;
   const int rounds = ceil_div(p.H, kRound);
-  const int q = slice_rounds(static_cast<long long>(U) * rounds, rounds, teams, p.max_slices);
+  if (wid == 0) {
+    find_active<TOK>(p, s);
+    __syncwarp();
+    // whole items over all teams, or slices of a cluster's items over its teams
+    const int U = s.c.plan[1], local = ceil_div(U, clusters);
+    const long long whole = static_cast<long long>(ceil_div(U, teams)) * (4 * rounds + 2);
+    int len = rounds;
+    if (local <= kMaxLocal && rounds > 1) {
+      const int sliced = min(p.max_slices, rounds);
+      const int cut = lane + 2;  // slices
+      long long cost = 0x7fffffffll;
+      if (cut <= sliced)
+        cost = static_cast<long long>(ceil_div(local * cut, kCluster * kTeams)) *
+                   (4 * ceil_div(rounds, cut) + 5) + 3;
+      const unsigned best = __reduce_min_sync(0xffffffffu, static_cast<unsigned>(cost));
+      const int at = __ffs(__ballot_sync(0xffffffffu, static_cast<unsigned>(cost) == best)) - 1;
+      if (static_cast<long long>(best) < whole) len = ceil_div(rounds, at + 2);
+    }
+    if (lane == 0) s.c.plan[2] = len;
+  }
+  fence_proxy_async_smem();  // the routing's use of the rings, before copies into them
+  __syncthreads();
+  const int active = s.c.plan[0], U = s.c.plan[1], q = s.c.plan[2];
   const int slices = ceil_div(rounds, q);
-  if (blockIdx.x == 0) {
-    for (int e = tid; e < p.E; e += kThreads) p.mask[e] = s.mask[e];
+
+  if (blockIdx.x == gridDim.x - 1) {  // (the block that units come to last)
     for (int a = tid; a < A; a += kThreads) {
-      p.sel[a] = s.sel[a];
-      p.wgt[a] = s.wgt[a];
+      const int e = sel_s[a], t = a / p.k;
+      p.slot[a] = s.slot[e];
+      p.row[a] = s.base[e] + __popcll(s.mask[e] & ((1ull << t) - 1));
+      p.wgt[a] = wgt_s[a];
     }
     for (int i = tid; i < ceil_div(p.H, kTile); i += kThreads) p.ticket[i] = 0;
-    if (tid == 0) p.info[0] = slices;
+    for (int j = tid; j < active; j += kThreads) {
+      int* d = p.plan + PLAN_WORDS + j;
+      d[0 * p.E] = s.c.act.n[j];
+      d[1 * p.E] = s.c.act.base[j];
+      d[2 * p.E] = s.c.act.first[j];
+      d[3 * p.E] = s.c.act.width[j];
+      d[4 * p.E] = s.c.act.kb[j];
+      d[5 * p.E] = s.c.act.sg[j];
+    }
+    if (wid == kWarps - 1) plan_down<TOK, kRound>(p, s.c.act, active);
   }
-  __syncthreads();
 
-  const int team = wid / kTeam, wr = wid % kTeam;
-  float* red = part + team * (kTeam * TOK * kRedLd);
-  for (int i = blockIdx.x * kTeams + team; i < U * slices; i += teams) {
-    const int sl = i / U, r = i % U;
-    const int e = find_item(s.m.item, p.E, r);
-    const int cols = gated * s.m.width[e], tiles = ceil_div(cols, kTile);
-    const int pass = (r - s.m.item[e]) / tiles, tile = (r - s.m.item[e]) % tiles;
-    const int begin = sl * q * kRound, end = min(p.H, begin + q * kRound);
-    const int count = min(s.m.n[e] - pass * TOK, TOK);
-    const int row = s.m.base[e] + pass * TOK;
-    const auto strip =
-        Strips<L>::make(p.w1, p.s1, p.total, 0, 0, 0, (p.H + (1 << p.shift) - 1) >> p.shift,
-                        s.m.first[e] + tile * kTile, end, cols - tile * kTile, p.shift);
-    const RowSource<T> src{static_cast<const T*>(p.x), p.ldx, s.list, row};
-    product<L, NG, kRound, kRedLd>(strip, src, count, begin + wr * L::kStep, lane,
-                                   red + wr * TOK * kRedLd);
-    team_sync(team);
-    team_store<TOK>(red, count, cols - tile * kTile,
-                    p.u + (static_cast<long long>(sl) * A + row) * p.ldu + tile * kTile, p.ldu);
-    team_sync(team);
+  // item of unit i: the whole grid's, or (sliced) every `clusters`-th item for this
+  // cluster, slices of one item on different CTAs
+  const int team = wid / kTeam, tt = tid % kTeamThreads;
+  const int mine = blockIdx.x / kCluster;
+  int start, stride, total;
+  if (slices == 1) {
+    start = blockIdx.x * kTeams + team;
+    stride = teams;
+    total = U;
+  } else {
+    start = team * kCluster + rank;
+    stride = kCluster * kTeams;
+    total = U > mine ? ceil_div(U - mine, clusters) * slices : 0;
   }
+  const Active& act = s.c.act;
+  auto place = [&](int i) {
+    const int item = slices == 1 ? i : mine + clusters * (i / slices);
+    const int e = find_item(act.item, active, item), r = item - act.item[e];
+    const int tiles = ceil_div(act.width[e], tile_outputs(p.act));
+    return Place(e, r % tiles, slices == 1 ? 0 : i % slices, r / tiles);
+  };
+  auto unit = [&](const Place& w) {
+    Unit u;
+    u.set(w, TOK);
+    const int width = act.width[u.e];
+    u.count = min(act.n[u.e] - u.pass, TOK);
+    u.row = act.base[u.e] + u.pass;
+    u.begin = u.slice * q * kRound;
+    u.strip.end = min(p.H, u.begin + q * kRound);
+    up_strip(u.strip, act.first[u.e], width, p.act, u.tile, p.H, p.shift);
+    return u;
+  };
+  auto source = [&](const Unit& u) {
+    return RowSource<T>{static_cast<const T*>(p.x), p.ldx, s.act_mask[u.e], u.pass};
+  };
+  float* red = reinterpret_cast<float*>(work + kRingBytes<L, NG>) + team * kRedFloats<L, NG>;
+  // activated sums of vector tok, from get(tok, column)
+  auto emit = [&](const Unit& u, int tok, int c, auto get) {
+    const float4 a = get(tok, c);
+    float v[4];
+    int col = u.tile * 64 + c;
+    if (p.act == ACT_SWIGLU) {
+      const float4 b = get(tok, c + 32);
+      col = u.tile * 32 + c;
+      v[0] = act_gated(a.x, b.x); v[1] = act_gated(a.y, b.y);
+      v[2] = act_gated(a.z, b.z); v[3] = act_gated(a.w, b.w);
+    } else {
+      v[0] = act_plain(a.x, p.act); v[1] = act_plain(a.y, p.act);
+      v[2] = act_plain(a.z, p.act); v[3] = act_plain(a.w, p.act);
+    }
+    if (col < act.width[u.e])
+      hidden_store4<T>(static_cast<T*>(p.h) + (u.row + tok) * p.ldh, p.max_width, col, v);
+  };
+  const int vecs = tile_outputs(p.act) / 4;
+  const Matrix m{&p.map1, p.w1, p.s1, p.total, p.shift, p.act == ACT_SWIGLU};
+  run_units<L, NG>(start, stride, total, m, work, red, s.c, place, unit, source, [&](int i, const Unit& u) {
+    if (slices == 1) {
+      for (int j = tt; j < u.count * vecs; j += kTeamThreads)
+        emit(u, j / vecs, 4 * (j % vecs),
+             [&](int tok, int c) { return unit_sum<TOK>(red, tok, c); });
+      return;
+    }
+    float* dst = p.u + u.row * p.ldu + u.tile * kTile;
+    const long long slice = static_cast<long long>(A) * p.ldu;
+    for (int j = tt; j < u.count * (kTile / 4); j += kTeamThreads) {
+      const int tok = j / (kTile / 4), c = 4 * (j % (kTile / 4));
+      *reinterpret_cast<float4*>(dst + u.slice * slice + tok * p.ldu + c) =
+          unit_sum<TOK>(red, tok, c);
+    }
+    team_sync(team);
+    if (tt == 0) {
+      __threadfence();  // the team's sums, before the count
+      s.c.last[team] =
+          atomicAdd(cluster.map_shared_rank(s.ticket, 0) + i / slices, 1) == slices - 1;
+      __threadfence();  // and the other teams' sums, after it
+    }
+    team_sync(team);
+    if (s.c.last[team]) {
+      for (int j = tt; j < u.count * vecs; j += kTeamThreads)
+        emit(u, j / vecs, 4 * (j % vecs), [&](int tok, int c) {
+          const float* src = dst + tok * p.ldu + c;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+          for (int z = 0; z < slices; ++z)
+            add4(v, __ldcg(reinterpret_cast<const float4*>(src + z * slice)));
+          return v;
+        });
+    }
+  });
+  if (s.c.abort && lane == 0 && p.status) *p.status = kStatusTimeout;
+  if (slices > 1) cluster.sync();  // rank 0's counters stay until the last team is done
 }
 
 // ---- down kernel -------------------------------------------------------------
-struct alignas(16) DownSmem {
-  Meta m;
-  unsigned long long mask[kMaxExperts];
-  int sel[kMaxTokens * kMaxTopK];
-  float wgt[kMaxTokens * kMaxTopK];
-  int last[kTeams];
-};
-
-static_assert(sizeof(DownSmem) % 16 == 0, "16-byte vectors follow");
-
 template <typename L, int NG>
-__global__ void __launch_bounds__(kThreads, 1) few_down_kernel(const LayerParams p) {
+__global__ void __launch_bounds__(kThreads, 1)
+    few_down_kernel(const __grid_constant__ LayerParams p) {
   using T = typename L::Elem;
-  constexpr int TOK = Shape<L, NG>::kTok;
-  extern __shared__ __align__(16) unsigned char raw[];
-  DownSmem& s = *reinterpret_cast<DownSmem*>(raw);
-  float* part = reinterpret_cast<float*>(raw + sizeof(DownSmem));
-  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+  constexpr int TOK = L::template kTokens<NG>, kRound = kTeam * L::kStep;
+  extern __shared__ __align__(1024) unsigned char raw[];
+  unsigned char* work = raw;
+  Common& s = *reinterpret_cast<Common*>(raw + kWorkBytes<L, NG>);
   const int A = p.T * p.k, gated = p.act == ACT_SWIGLU ? 2 : 1;
+  int* slot_s = reinterpret_cast<int*>(raw + kWorkBytes<L, NG> + sizeof(Common));
+  int* row_s = slot_s + A;
+  float* wgt_s = reinterpret_cast<float*>(row_s + A);
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+  ring_init<L::template kDepth<NG>>(s);
+  if (tid == 0 && p.shift == 0) tma_prefetch_desc(&p.map2);
 
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  for (int e = tid; e < p.E; e += kThreads) s.mask[e] = p.mask[e];
+  if (tid < 3) s.plan[tid] = p.plan[tid];
+  for (int i = tid; i < kActiveArrays * p.E; i += kThreads) {
+    const int j = i / p.E;
+    (&s.act.n[0])[j * kMaxExperts + i - j * p.E] = p.plan[PLAN_WORDS + i];
+  }
   for (int a = tid; a < A; a += kThreads) {
-    s.sel[a] = p.sel[a];
-    s.wgt[a] = p.wgt[a];
+    slot_s[a] = p.slot[a];
+    row_s[a] = p.row[a];
+    wgt_s[a] = p.wgt[a];
   }
-  const int u_slices = p.info[0];
   __syncthreads();
-  layer_meta(p, s.mask, s.m);
-  constexpr int kRound = kTeam * L::kStep;
-  int mine = 0, passes = 0, all_rounds, most;
-  if (tid < p.E) {
-    passes = ceil_div(s.m.n[tid], TOK);
-    mine = ceil_div(s.m.width[tid], kRound);
-  }
-  block_scan(passes * mine, s.m.scan, &all_rounds);
-  most = ceil_div(p.max_width, kRound);
-  const int tiles = ceil_div(p.H, kTile), teams = gridDim.x * kTeams;
-  const int q = slice_rounds(static_cast<long long>(all_rounds) * tiles, most, teams, p.max_slices);
-  int items;
-  const int before = block_scan(passes * ceil_div(mine, q), s.m.scan, &items);
-  if (tid < p.E) s.m.item[tid] = before;
-  __syncthreads();
+  const int active = s.plan[PLAN_ACTIVE], q = s.plan[PLAN_LENGTH], items = s.plan[PLAN_ITEMS];
+  const int tiles = ceil_div(p.H, kTile);
+  const Active& act = s.act;
 
   T* out = static_cast<T*>(p.out);
+  const bool add = p.T <= kAddTokens;  // this kernel also adds the parts up
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (items == 0) {  // no expert has a column (or all were refused): the sum is empty
+    if (!add) return;
     for (long long i = blockIdx.x * static_cast<long long>(kThreads) + tid;
          i < static_cast<long long>(p.T) * p.H; i += static_cast<long long>(gridDim.x) * kThreads)
       out[i / p.H * p.ldo + i % p.H] = from_f<T>(0.f);
     return;
   }
 
-  const int team = wid / kTeam, wr = wid % kTeam;
-  float* red = part + team * (kTeam * TOK * kRedLd);
-  for (int i = blockIdx.x * kTeams + team; i < items * tiles; i += teams) {
-    const int it = i / tiles, tile = i % tiles;
-    const int e = find_item(s.m.item, p.E, it);
-    const int width = s.m.width[e], ns = ceil_div(ceil_div(width, kRound), q);
-    const int pass = (it - s.m.item[e]) / ns, sl = (it - s.m.item[e]) % ns;
-    const int begin = sl * q * kRound, end = min(width, begin + q * kRound);
-    const int count = min(s.m.n[e] - pass * TOK, TOK);
-    const int row = s.m.base[e] + pass * TOK, cols = p.H - tile * kTile;
-    const auto strip =
-        Strips<L>::make(p.w2, p.s2, p.H, s.m.first[e] / gated, s.m.kb[e], s.m.sg[e],
-                        (width + (1 << p.shift) - 1) >> p.shift, tile * kTile, end, cols, p.shift);
-    const PartialSource<T> src{p.u, p.ldu, static_cast<long long>(A) * p.ldu, u_slices, row,
-                               p.act, width};
-    product<L, NG, kRound, kRedLd>(strip, src, count, begin + wr * L::kStep, lane,
-                                   red + wr * TOK * kRedLd);
-    team_sync(team);
-    team_store<TOK>(red, count, cols,
-                    p.y + (static_cast<long long>(sl) * A + row) * p.H + tile * kTile, p.H);
-    team_sync(team);
-    if (tid % (kTeam * 32) == 0) {
-      __threadfence();  // the team's stores, before the count
-      s.last[team] = atomicAdd(&p.ticket[tile], 1) == items - 1;
-      __threadfence();  // and the other teams' stores, after it
-    }
-    team_sync(team);
-    if (s.last[team]) {
-      // token by token: slots in order, slices in order
-      for (int j = tid % (kTeam * 32); j < p.T * (kTile / 4); j += kTeam * 32) {
-        const int t = j / (kTile / 4), c = 4 * (j % (kTile / 4));
-        if (c >= cols) continue;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int a = t * p.k; a < (t + 1) * p.k; ++a) {
-          const int ex = s.sel[a];
-          if (s.m.n[ex] == 0) continue;
-          const int parts = ceil_div(ceil_div(s.m.width[ex], kRound), q);
-          const int r = s.m.base[ex] + __popcll(s.mask[ex] & ((1ull << t) - 1));
-          const float* y = p.y + static_cast<long long>(r) * p.H + tile * kTile + c;
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-          for (int z = 0; z < parts; ++z) {
-            const float4 d = __ldcg(
-                reinterpret_cast<const float4*>(y + static_cast<long long>(z) * A * p.H));
-            v.x += d.x; v.y += d.y; v.z += d.z; v.w += d.w;
-          }
-          const float w = s.wgt[a];
-          o.x = fmaf(w, v.x, o.x);
-          o.y = fmaf(w, v.y, o.y);
-          o.z = fmaf(w, v.z, o.z);
-          o.w = fmaf(w, v.w, o.w);
+  const int team = wid / kTeam, tt = tid % kTeamThreads;
+  // Eight column tiles (1 KB of a row) at a time: neighbouring teams read
+  // neighbouring pieces, and the tiles finish one block after another, so that
+  // only the last block's final sums have nothing to overlap.
+  auto place = [&](int i) {
+    const int block = i / (8 * items), r = i - block * 8 * items;
+    const int nb = min(8, tiles - 8 * block), it = r / nb;
+    const int e = find_item(act.item, active, it), j = it - act.item[e];
+    const int ns = ceil_div(ceil_div(act.width[e], kRound), q);
+    return Place(e, 8 * block + r % nb, j % ns, j / ns);
+  };
+  auto unit = [&](const Place& w) {
+    Unit u;
+    u.set(w, TOK);
+    const int width = act.width[u.e];
+    u.count = min(act.n[u.e] - u.pass, TOK);
+    u.row = act.base[u.e] + u.pass;
+    u.begin = u.slice * q * kRound;
+    u.strip.end = min(width, u.begin + q * kRound);
+    down_strip(u.strip, act, u.e, act.first[u.e] / gated, u.tile, p.H, p.shift);
+    return u;
+  };
+  auto source = [&](const Unit& u) {
+    return HiddenSource<T>{static_cast<const T*>(p.h), p.ldh, p.max_width, u.row};
+  };
+  float* red = reinterpret_cast<float*>(work + kRingBytes<L, NG>) + team * kRedFloats<L, NG>;
+  const long long slice = static_cast<long long>(A) * p.H;
+  const bool vec = (p.ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  // threads that share a (token, column vector) of the final sum
+  const int share = p.T == 1 ? 8 : p.T == 2 ? 4 : p.T <= 4 ? 2 : 1;
+  const Matrix m{&p.map2, p.w2, p.s2, p.H, p.shift, 0};
+  run_units<L, NG>(
+      blockIdx.x * kTeams + team, gridDim.x * kTeams, items * tiles, m, work, red, s, place, unit,
+      source,
+      [&](int, const Unit& u) {
+        const int cols = p.H - u.tile * kTile;
+        float* y = p.y + u.tile * kTile;
+        for (int j = tt; j < u.count * (kTile / 4); j += kTeamThreads) {
+          const int tok = j / (kTile / 4), c = 4 * (j % (kTile / 4));
+          if (c < cols)
+            *reinterpret_cast<float4*>(y + u.slice * slice +
+                                       static_cast<long long>(u.row + tok) * p.H + c) =
+                unit_sum<TOK>(red, tok, c);
         }
-        T* d = out + t * p.ldo + tile * kTile + c;
-        d[0] = from_f<T>(o.x);
-        d[1] = from_f<T>(o.y);
-        d[2] = from_f<T>(o.z);
-        d[3] = from_f<T>(o.w);
-      }
-    }
-    team_sync(team);  // s.last and the partial sums are free again
+        if (!add) return;
+        team_sync(team);
+        if (tt == 0) {
+          __threadfence();  // the team's sums, before the count
+          s.last[team] = atomicAdd(&p.ticket[u.tile], 1) == items - 1;
+          __threadfence();  // and the other teams' sums, after it
+        }
+        team_sync(team);
+        if (!s.last[team]) return;
+        // each thread's slots in order, four at a time, their parts in order
+        const int lanes = kTeamThreads / share, part = tt / lanes;
+        for (int j0 = 0; j0 < p.T * (kTile / 4); j0 += lanes) {  // (barriers inside)
+          const int j = j0 + tt % lanes, t = j / (kTile / 4), c = 4 * (j % (kTile / 4));
+          const bool in = t < p.T && c < cols;
+          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (in) {
+            for (int a0 = part; a0 < p.k; a0 += 4 * share) {
+              const float* src[4];
+              int parts[4];
+              float4 v[4];
+              int longest = 0;
+#pragma unroll
+              for (int n = 0; n < 4; ++n) {
+                const int a = t * p.k + a0 + n * share;
+                v[n] = make_float4(0.f, 0.f, 0.f, 0.f);
+                parts[n] = 0;
+                src[n] = y;
+                if (a0 + n * share < p.k && slot_s[a] >= 0) {
+                  parts[n] = ceil_div(ceil_div(act.width[slot_s[a]], kRound), q);
+                  src[n] = y + static_cast<long long>(row_s[a]) * p.H + c;
+                }
+                longest = max(longest, parts[n]);
+              }
+#pragma unroll 2
+              for (int z = 0; z < longest; ++z)
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+                  if (z < parts[n])
+                    add4(v[n], __ldcg(reinterpret_cast<const float4*>(src[n] + z * slice)));
+#pragma unroll
+              for (int n = 0; n < 4; ++n) {
+                // (an expert without columns adds nothing, whatever its weight)
+                const float g = parts[n] ? wgt_s[t * p.k + a0 + n * share] : 0.f;
+                o.x = fmaf(g, v[n].x, o.x);
+                o.y = fmaf(g, v[n].y, o.y);
+                o.z = fmaf(g, v[n].z, o.z);
+                o.w = fmaf(g, v[n].w, o.w);
+              }
+            }
+          }
+          if (share > 1) {
+            float4* sums = reinterpret_cast<float4*>(red);  // read above, before a barrier
+            sums[tt] = o;
+            team_sync(team);
+            if (part == 0)
+              for (int g = 1; g < share; ++g) add4(o, sums[tt + g * lanes]);
+          }
+          if (part == 0 && in) store4<T>(out + t * p.ldo + u.tile * kTile + c, o, vec);
+        }
+      });
+  if (s.abort && lane == 0 && p.status) *p.status = kStatusTimeout;
+}
+
+// More than 8 tokens: the final sum as a kernel of its own.  (In the down kernel a
+// team adds the tile that it finishes; at 64 tokens that is 40,000 cycles of it at
+// the end, with the other teams idle.)  A block is a token's 1024 columns; slots in
+// order, their parts in order.
+constexpr int kSumThreads = 256;
+template <typename L>
+__global__ void __launch_bounds__(kSumThreads) few_sum_kernel(const __grid_constant__ LayerParams p) {
+  using T = typename L::Elem;
+  constexpr int kRound = kTeam * L::kStep;
+  __shared__ int row_s[kMaxTopK], parts_s[kMaxTopK];
+  __shared__ float wgt_s[kMaxTopK];
+  const int t = blockIdx.y, tid = threadIdx.x;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (tid < p.k) {
+    const int a = t * p.k + tid, slot = p.slot[a];
+    row_s[tid] = p.row[a];
+    wgt_s[tid] = p.wgt[a];
+    parts_s[tid] = 0;
+    if (slot >= 0)
+      parts_s[tid] = ceil_div(ceil_div(p.plan[PLAN_WORDS + 3 * p.E + slot], kRound),
+                              p.plan[PLAN_LENGTH]);
   }
+  __syncthreads();
+  const int c = 4 * (blockIdx.x * kSumThreads + tid);
+  if (c >= p.H) return;
+  T* out = static_cast<T*>(p.out);
+  const bool vec = (p.ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  const long long slice = static_cast<long long>(p.T) * p.k * p.H;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int a = 0; a < p.k; ++a) {
+    const float* y = p.y + static_cast<long long>(row_s[a]) * p.H + c;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int z = 0; z < parts_s[a]; ++z)
+      add4(v, __ldcg(reinterpret_cast<const float4*>(y + z * slice)));
+    // (an expert without columns adds nothing, whatever its weight)
+    const float g = parts_s[a] ? wgt_s[a] : 0.f;
+    o.x = fmaf(g, v.x, o.x);
+    o.y = fmaf(g, v.y, o.y);
+    o.z = fmaf(g, v.z, o.z);
+    o.w = fmaf(g, v.w, o.w);
+  }
+  store4<T>(out + t * p.ldo + c, o, vec);
 }
 
 // ---- 4-bit products of rows grouped by expert --------------------------------
@@ -647,8 +1084,8 @@ struct GroupParams {
   const int* off;      // [E + 1]: columns of w (up) or rows of w (down)
   int E, H, total, max_width, act, down;
   int shift, blocks, groups;
-  int* info;           // [0]: rounds of a slice
-  float* part;         // [slices][rows][ldp]
+  int* plan;           // [PLAN_WORDS], then n, base, width [E] of the active experts
+  float* part;         // [slices][rows][ldp]: 64 columns a tile
   long long ldp;
   int max_slices;
   void* out;
@@ -656,145 +1093,206 @@ struct GroupParams {
   int* status;
 };
 
-// Rows, widths and work items; the same numbers in both kernels.
-__device__ __forceinline__ void group_meta(const GroupParams& p, Meta& m) {
-  const int e = threadIdx.x;
-  const int gated = p.act == ACT_SWIGLU ? 2 : 1;
-  int n = 0, a = 0, w = 0, lo = 0;
-  bool ok = true;
-  if (e < p.E) {
-    a = p.off[e];
-    const int b = p.off[e + 1];
-    lo = p.tok_off[e];
-    const int hi = p.tok_off[e + 1];
-    n = hi - lo;
-    if (p.tok_cnt) n = min(n, p.tok_cnt[e]);
-    ok = a >= 0 && b >= a && b <= p.total && a % (16 * gated) == 0 &&
-         (b - a) % (16 * gated) == 0 && (b - a) / gated <= p.max_width && lo >= 0 && hi >= lo &&
-         hi <= p.rows && n >= 0;
-    w = ok ? (b - a) / gated : 0;
-  }
-  int kb = 0, sg = 0, all;
-  if (p.down) {
-    kb = block_scan(ceil_div(w, 64), m.scan, &all);
-    sg = block_scan((w + (1 << p.shift) - 1) >> p.shift, m.scan, &all);
-  }
-  if (e < p.E) {
-    if (p.down && (kb + ceil_div(w, 64) > p.blocks ||
-                   sg + ((w + (1 << p.shift) - 1) >> p.shift) > p.groups))
-      ok = false;
-    if (!ok && p.status && blockIdx.x == 0) *p.status = kStatusBadArg;
-    m.n[e] = ok ? n : 0;
-    m.base[e] = lo;
-    m.first[e] = a;
-    m.width[e] = ok ? w : 0;
-    m.kb[e] = kb;
-    m.sg[e] = sg;
-  }
-  __syncthreads();
-}
+struct alignas(16) GroupSmem {
+  Common c;
+  int off[kMaxExperts + 1];
+  int tok[kMaxExperts + 1];
+  int cnt[kMaxExperts];
+};
+static_assert(sizeof(GroupSmem) % 16 == 0, "16-byte vectors follow");
 
 template <typename L, int NG>
-__global__ void __launch_bounds__(kThreads, 1) few_group_kernel(const GroupParams p) {
+__global__ void __launch_bounds__(kThreads, 1)
+    few_group_kernel(const __grid_constant__ GroupParams p) {
   using T = typename L::Elem;
-  constexpr int TOK = Shape<L, NG>::kTok;
-  constexpr int kRound = kTeam * L::kStep;
-  extern __shared__ __align__(16) unsigned char raw[];
-  Meta& m = *reinterpret_cast<Meta*>(raw);
-  float* part = reinterpret_cast<float*>(raw + sizeof(Meta));
+  constexpr int TOK = L::template kTokens<NG>, kRound = kTeam * L::kStep;
+  extern __shared__ __align__(1024) unsigned char raw[];
+  unsigned char* work = raw;
+  GroupSmem& s = *reinterpret_cast<GroupSmem*>(raw + kWorkBytes<L, NG>);
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  group_meta(p, m);
-  const int gated = p.act == ACT_SWIGLU ? 2 : 1;
-  int passes = 0, mine = 0, tiles_e = 0, all;
-  if (tid < p.E) {
-    passes = ceil_div(m.n[tid], TOK);
-    tiles_e = ceil_div(p.down ? p.H : gated * m.width[tid], kTile);
-    mine = ceil_div(p.down ? m.width[tid] : p.H, kRound);
+  for (int e = tid; e <= p.E; e += kThreads) {
+    s.off[e] = p.off[e];
+    s.tok[e] = p.tok_off[e];
+    if (e < p.E) s.cnt[e] = p.tok_cnt ? p.tok_cnt[e] : 0x7fffffff;
   }
-  block_scan(passes * tiles_e * mine, m.scan, &all);
-  const int teams = gridDim.x * kTeams;
-  const int q = slice_rounds(all, ceil_div(p.down ? p.max_width : p.H, kRound), teams, p.max_slices);
-  int U;
-  const int before = block_scan(passes * tiles_e * ceil_div(mine, q), m.scan, &U);
-  if (tid < p.E) m.item[tid] = before;
-  if (blockIdx.x == 0 && tid == 0) p.info[0] = q;
+  ring_init<L::template kDepth<NG>>(s.c);
   __syncthreads();
-
-  const int team = wid / kTeam, wr = wid % kTeam;
-  float* red = part + team * (kTeam * TOK * kRedLd);
-  for (int i = blockIdx.x * kTeams + team; i < U; i += teams) {
-    const int e = find_item(m.item, p.E, i);
-    const int width = m.width[e];
-    const int n_cols = p.down ? p.H : gated * width, k_rows = p.down ? width : p.H;
-    const int tiles = ceil_div(n_cols, kTile), ns = ceil_div(ceil_div(k_rows, kRound), q);
-    const int r = i - m.item[e];
-    const int tile = r % tiles, pass = r / tiles / ns, sl = r / tiles % ns;
-    const int begin = sl * q * kRound, end = min(k_rows, begin + q * kRound);
-    const int count = min(m.n[e] - pass * TOK, TOK);
-    const int row = m.base[e] + pass * TOK, cols = n_cols - tile * kTile;
-    const auto strip = p.down
-        ? Strips<L>::make(p.w, p.s, p.H, m.first[e], m.kb[e], m.sg[e],
-                          (width + (1 << p.shift) - 1) >> p.shift, tile * kTile, end, cols, p.shift)
-        : Strips<L>::make(p.w, p.s, p.total, 0, 0, 0, (p.H + (1 << p.shift) - 1) >> p.shift,
-                          m.first[e] + tile * kTile, end, cols, p.shift);
-    const RowSource<T> src{static_cast<const T*>(p.x), p.ldx, nullptr, row};
-    product<L, NG, kRound, kRedLd>(strip, src, count, begin + wr * L::kStep, lane,
-                                   red + wr * TOK * kRedLd);
-    team_sync(team);
-    team_store<TOK>(red, count, cols,
-                    p.part + (static_cast<long long>(sl) * p.rows + row) * p.ldp + tile * kTile,
-                    p.ldp);
-    team_sync(team);
+  const int outputs = tile_outputs(p.act), teams = gridDim.x * kTeams;
+  if (wid == 0) {  // as find_active
+    const int gated = p.act == ACT_SWIGLU ? 2 : 1;
+    int active = 0, kb = 0, sg = 0;
+#pragma unroll 1
+    for (int e0 = 0; e0 < p.E; e0 += 32) {
+      const int e = e0 + lane;
+      int n = 0, a = 0, w = 0, lo = 0, total;
+      bool ok = true;
+      if (e < p.E) {
+        a = s.off[e];
+        const int b = s.off[e + 1], hi = s.tok[e + 1];
+        lo = s.tok[e];
+        ok = a >= 0 && b >= a && b <= p.total && a % (16 * gated) == 0 &&
+             (b - a) % (16 * gated) == 0 && (b - a) / gated <= p.max_width && lo >= 0 &&
+             hi >= lo && hi <= p.rows && s.cnt[e] >= 0;
+        w = ok ? (b - a) / gated : 0;
+        n = ok ? min(hi - lo, s.cnt[e]) : 0;
+      }
+      int my_kb = 0, my_sg = 0;
+      if (p.down) {
+        const int blocks = ceil_div(w, 64), groups = group_count(w, p.shift);
+        my_kb = kb + warp_scan(blocks, &total);
+        kb += total;
+        my_sg = sg + warp_scan(groups, &total);
+        sg += total;
+        if (my_kb + blocks > p.blocks || my_sg + groups > p.groups) ok = false;
+      }
+      if (!ok && p.status && blockIdx.x == 0) *p.status = kStatusBadArg;
+      const bool here = ok && n > 0 && w > 0;
+      const unsigned who = __ballot_sync(0xffffffffu, here);
+      const int at = active + __popc(who & ((1u << lane) - 1));
+      active += __popc(who);
+      if (here) {
+        s.c.act.n[at] = n;
+        s.c.act.base[at] = lo;
+        s.c.act.first[at] = a;
+        s.c.act.width[at] = w;
+        s.c.act.kb[at] = my_kb;
+        s.c.act.sg[at] = my_sg;
+      }
+    }
+    __syncwarp();
+    auto units = [&](int j, int len) {
+      return ceil_div(s.c.act.n[j], TOK) *
+             (p.down ? ceil_div(p.H, kTile) * ceil_div(ceil_div(s.c.act.width[j], kRound), len)
+                     : ceil_div(s.c.act.width[j], outputs) * ceil_div(ceil_div(p.H, kRound), len));
+    };
+    int widest = 0;
+    for (int j = lane; j < active; j += 32) widest = max(widest, s.c.act.width[j]);
+    widest = __reduce_max_sync(0xffffffffu, widest);
+    const int most = max(1, ceil_div(p.down ? widest : p.H, kRound));
+    const int len = plan_length(most, teams, p.max_slices, 2, [&](int length) {
+      int n = 0;
+      for (int j = lane; j < active; j += 32) n += units(j, length);
+      return static_cast<long long>(__reduce_add_sync(0xffffffffu, n));
+    });
+    int items = 0;
+    for (int j0 = 0; j0 < active; j0 += 32) {
+      const int j = j0 + lane;
+      int total;
+      const int before = items + warp_scan(j < active ? units(j, len) : 0, &total);
+      items += total;
+      if (j < active) s.c.act.item[j] = before;
+    }
+    if (lane == 0) {
+      s.c.plan[0] = active;
+      s.c.plan[1] = items;
+      s.c.plan[2] = len;
+    }
   }
+  __syncthreads();
+  const int active = s.c.plan[0], q = s.c.plan[2];
+  const Active& act = s.c.act;
+  if (blockIdx.x == gridDim.x - 1) {
+    for (int j = tid; j < active; j += kThreads) {
+      int* d = p.plan + PLAN_WORDS + j;
+      d[0 * p.E] = act.n[j];
+      d[1 * p.E] = act.base[j];
+      d[2 * p.E] = act.width[j];
+    }
+    if (tid == 0) {
+      p.plan[PLAN_ACTIVE] = active;
+      p.plan[PLAN_LENGTH] = q;
+    }
+  }
+
+  const int team = wid / kTeam, tt = tid % kTeamThreads;
+  auto place = [&](int i) {
+    const int e = find_item(act.item, active, i), r = i - act.item[e], width = act.width[e];
+    const int tiles = p.down ? ceil_div(p.H, kTile) : ceil_div(width, outputs);
+    const int ns = ceil_div(ceil_div(p.down ? width : p.H, kRound), q);
+    return Place(e, r % tiles, r / tiles % ns, r / tiles / ns);
+  };
+  auto unit = [&](const Place& w) {
+    Unit u;
+    u.set(w, TOK);
+    const int width = act.width[u.e], k_rows = p.down ? width : p.H;
+    u.count = min(act.n[u.e] - u.pass, TOK);
+    u.row = act.base[u.e] + u.pass;
+    u.begin = u.slice * q * kRound;
+    u.strip.end = min(k_rows, u.begin + q * kRound);
+    if (p.down)
+      down_strip(u.strip, act, u.e, act.first[u.e], u.tile, p.H, p.shift);
+    else
+      up_strip(u.strip, act.first[u.e], width, p.act, u.tile, p.H, p.shift);
+    return u;
+  };
+  auto source = [&](const Unit& u) {
+    return RowSource<T>{static_cast<const T*>(p.x), p.ldx, 0ull, u.row};
+  };
+  float* red = reinterpret_cast<float*>(work + kRingBytes<L, NG>) + team * kRedFloats<L, NG>;
+  const Matrix m{nullptr, p.w, p.s, p.down ? p.H : p.total, p.shift, p.act == ACT_SWIGLU};
+  run_units<L, NG>(blockIdx.x * kTeams + team, teams, s.c.plan[1], m, work, red, s.c, place, unit, source,
+                   [&](int, const Unit& u) {
+                     float* dst = p.part +
+                                  (static_cast<long long>(u.slice) * p.rows + u.row) * p.ldp +
+                                  u.tile * kTile;
+                     const int cols = p.act == ACT_SWIGLU ? kTile : static_cast<int>(p.ldp) - u.tile * kTile;
+                     for (int j = tt; j < u.count * (kTile / 4); j += kTeamThreads) {
+                       const int tok = j / (kTile / 4), c = 4 * (j % (kTile / 4));
+                       if (c < cols)
+                         *reinterpret_cast<float4*>(dst + tok * p.ldp + c) =
+                             unit_sum<TOK>(red, tok, c);
+                     }
+                   });
+  if (s.c.abort && lane == 0 && p.status) *p.status = kStatusTimeout;
 }
 
 // Adds the slices, applies the activation, writes every element of the output:
 // zero in rows and columns that belong to no expert.
 template <typename L>
-__global__ void __launch_bounds__(kThreads) few_group_sum_kernel(const GroupParams p) {
+__global__ void __launch_bounds__(kThreads)
+    few_group_sum_kernel(const __grid_constant__ GroupParams p) {
   using T = typename L::Elem;
   constexpr int kRound = kTeam * L::kStep;
-  __shared__ Meta m;
+  __shared__ int n_s[kMaxExperts], base_s[kMaxExperts], width_s[kMaxExperts], head[2];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  group_meta(p, m);
-  const int q = p.info[0];
-  const int out_cols = p.down ? p.H : p.max_width, vec = out_cols / 4;
-  const long long stride = static_cast<long long>(p.rows) * p.ldp;
-  for (long long i = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x; i < p.rows * vec;
+  for (int j = threadIdx.x; j < p.E; j += kThreads) {
+    n_s[j] = p.plan[PLAN_WORDS + j];
+    base_s[j] = p.plan[PLAN_WORDS + p.E + j];
+    width_s[j] = p.plan[PLAN_WORDS + 2 * p.E + j];
+  }
+  if (threadIdx.x < 2) head[threadIdx.x] = p.plan[threadIdx.x];
+  __syncthreads();
+  const int active = head[PLAN_ACTIVE], q = head[PLAN_LENGTH];
+  const int out_cols = p.down ? p.H : p.max_width, vecs = out_cols / 4;
+  const long long slice = p.rows * p.ldp;
+  const bool vec = (p.ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+  const bool gated = p.act == ACT_SWIGLU;
+  for (long long i = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x; i < p.rows * vecs;
        i += static_cast<long long>(gridDim.x) * kThreads) {
-    const long long row = i / vec;
-    const int c = 4 * static_cast<int>(i % vec);
-    // the last expert that starts at or before this row (empty ones share a start)
-    int e = 0;
-    for (int step = kMaxExperts / 2; step > 0; step >>= 1)
-      if (e + step < p.E && m.base[e + step] <= row) e += step;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    const int cols = p.down ? p.H : m.width[e];
-    if (row >= m.base[e] && row < static_cast<long long>(m.base[e]) + m.n[e] && c < cols) {
-      const int ns = ceil_div(ceil_div(p.down ? m.width[e] : p.H, kRound), q);
-      const float* src = p.part + row * p.ldp + c;
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-      for (int z = 0; z < ns; ++z) {
-        const float4 d = __ldcg(reinterpret_cast<const float4*>(src + z * stride));
-        a.x += d.x; a.y += d.y; a.z += d.z; a.w += d.w;
-        if (p.act == ACT_SWIGLU) {
-          const float4 f = __ldcg(reinterpret_cast<const float4*>(src + z * stride + m.width[e]));
-          b.x += f.x; b.y += f.y; b.z += f.z; b.w += f.w;
+    const int row = static_cast<int>(i / vecs), c = 4 * static_cast<int>(i % vecs);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (active > 0) {
+      const int e = find_item(base_s, active, row);
+      if (row >= base_s[e] && row - base_s[e] < n_s[e] && (p.down || c < width_s[e])) {
+        const int ns = ceil_div(ceil_div(p.down ? width_s[e] : p.H, kRound), q);
+        const float* src = p.part + row * p.ldp + (gated ? c / 32 * kTile + c % 32 : c);
+        float4 b = v;
+#pragma unroll 4
+        for (int z = 0; z < ns; ++z) {
+          add4(v, __ldcg(reinterpret_cast<const float4*>(src + z * slice)));
+          if (gated) add4(b, __ldcg(reinterpret_cast<const float4*>(src + z * slice + 32)));
         }
-      }
-      if (p.act == ACT_SWIGLU) {
-        v[0] = act_gated(a.x, b.x); v[1] = act_gated(a.y, b.y);
-        v[2] = act_gated(a.z, b.z); v[3] = act_gated(a.w, b.w);
-      } else {
-        v[0] = act_plain(a.x, p.act); v[1] = act_plain(a.y, p.act);
-        v[2] = act_plain(a.z, p.act); v[3] = act_plain(a.w, p.act);
+        if (gated)
+          v = make_float4(act_gated(v.x, b.x), act_gated(v.y, b.y), act_gated(v.z, b.z),
+                          act_gated(v.w, b.w));
+        else
+          v = make_float4(act_plain(v.x, p.act), act_plain(v.y, p.act), act_plain(v.z, p.act),
+                          act_plain(v.w, p.act));
       }
     }
-    T* d = static_cast<T*>(p.out) + row * p.ldo + c;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) d[j] = from_f<T>(v[j]);
+    store4<T>(static_cast<T*>(p.out) + row * p.ldo + c, v, vec);
   }
 }
 
@@ -802,10 +1300,16 @@ __global__ void __launch_bounds__(kThreads) few_group_sum_kernel(const GroupPara
 long long align_up(long long v, long long a) { return (v + a - 1) / a * a; }
 
 struct LayerPlan {
-  long long mask, sel, wgt, info, ticket, u, y, bytes;
+  long long plan, slot, row, wgt, ticket, u, h, y, bytes;
   long long ldu;
   int slices;
 };
+
+// Columns of a product's partial sums: whole tiles.
+long long padded_columns(long long width, int act) {
+  const int n = tile_outputs(act);
+  return (width + n - 1) / n * kTile;
+}
 
 // Slices of a reduction the workspace holds: 64 MB of partial sums, or one slice.
 int slice_limit(long long floats) {
@@ -816,7 +1320,7 @@ int slice_limit(long long floats) {
 LayerPlan layer_plan(int T, int H, int E, int k, int max_width, int act) {
   LayerPlan p{};
   const long long A = static_cast<long long>(T) * k;
-  p.ldu = static_cast<long long>(act == ACT_SWIGLU ? 2 : 1) * max_width;
+  p.ldu = padded_columns(max_width, act);
   p.slices = slice_limit(A * (p.ldu > H ? p.ldu : H));
   long long at = 0;
   auto take = [&](long long bytes) {
@@ -824,12 +1328,13 @@ LayerPlan layer_plan(int T, int H, int E, int k, int max_width, int act) {
     at = align_up(at + bytes, 128);
     return here;
   };
-  p.mask = take(8ll * E);
-  p.sel = take(4 * A);
+  p.plan = take(4ll * (PLAN_WORDS + kActiveArrays * E));
+  p.slot = take(4 * A);
+  p.row = take(4 * A);
   p.wgt = take(4 * A);
-  p.info = take(16);
   p.ticket = take(4ll * ceil_div(H, kTile));
   p.u = take(4 * p.slices * A * p.ldu);
+  p.h = take(4 * A * max_width);  // two 16-bit values or one fp32
   p.y = take(4 * p.slices * A * H);
   p.bytes = at;
   return p;
@@ -841,11 +1346,12 @@ int current_device() {
 }
 
 // Shared memory above 48 KB has to be allowed once per kernel and device.
+constexpr int kSmemMax = 227 * 1024;
 template <typename K>
 bool allow_smem(K* kernel, std::atomic<unsigned long long>& done, int device) {
   const unsigned long long bit = 1ull << device;
   if (done.load(std::memory_order_acquire) & bit) return true;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) !=
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax) !=
       cudaSuccess)
     return false;
   done.fetch_or(bit, std::memory_order_release);
@@ -854,7 +1360,7 @@ bool allow_smem(K* kernel, std::atomic<unsigned long long>& done, int device) {
 
 // 8-CTA clusters that are resident together at one CTA an SM.
 template <typename K>
-int resident_clusters(K* kernel, std::atomic<int>* known, int device, size_t smem) {
+int resident_clusters(K* kernel, std::atomic<int>* known, int device) {
   int n = known[device].load(std::memory_order_acquire);
   if (n > 0) return n;
   cudaLaunchAttribute attr[1];
@@ -865,7 +1371,7 @@ int resident_clusters(K* kernel, std::atomic<int>* known, int device, size_t sme
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(num_sms() / kCluster * kCluster));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = kSmemMax;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) return -1;
@@ -874,26 +1380,62 @@ int resident_clusters(K* kernel, std::atomic<int>* known, int device, size_t sme
   return n;
 }
 
+PFN_cuTensorMapEncodeTiled_v12000 encode_tiled() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  });
+  return fn;
+}
+
+// Boxes of 4 KB (gated: two of 2 KB side by side) of a contiguous weight.
+bool weight_map(CUtensorMap* map, const void* w, int dtype, long long rows, long long cols,
+                bool gated) {
+  const auto fn = encode_tiled();
+  if (!fn) return false;
+  const int es = dtype == 2 ? 4 : 2;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols * es)};
+  const cuuint32_t box[2] = {gated ? 32u : 64u, dtype == 2 ? 16u : 32u};
+  const cuuint32_t step[2] = {1, 1};
+  return fn(map,
+            dtype == 2   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+            : dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                         : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+            2, const_cast<void*>(w), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            dtype == 2 ? CU_TENSOR_MAP_SWIZZLE_NONE
+            : gated    ? CU_TENSOR_MAP_SWIZZLE_64B
+                       : CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename L, int NG>
-int launch_layer(const LayerParams& p, cudaStream_t st) {
+int launch_layer(LayerParams& p, cudaStream_t st) {
   static std::atomic<unsigned long long> up_ok{0}, down_ok{0};
   static std::atomic<int> clusters[64];
-  constexpr int TOK = Shape<L, NG>::kTok;
   const int dev = current_device();
   if (dev < 0) return kStatusCuda;
   auto* up = few_up_kernel<L, NG>;
   auto* down = few_down_kernel<L, NG>;
   if (!allow_smem(up, up_ok, dev) || !allow_smem(down, down_ok, dev)) return kStatusCuda;
-  const int lde = ceil_div(p.E, 16) * 16, tiles = lde / 16;
+  const int lde = ceil_div(p.E, 16) * 16, tiles = lde / 16, A = p.T * p.k;
   const int ksub = kWarps / tiles > 1 ? kWarps / tiles : 1;
-  const size_t red = sizeof(float) * kWarps * TOK * kRedLd;
-  const size_t part = sizeof(float) * ksub * p.T * lde;
-  const size_t up_smem = sizeof(UpSmem) + sizeof(float) * p.T * lde + (red > part ? red : part);
-  const size_t down_smem = sizeof(DownSmem) + red;
-  const int n = resident_clusters(up, clusters, dev, 227 * 1024);
+  const size_t route = sizeof(float) * (1 + ksub) * p.T * lde, work = kWorkBytes<L, NG>;
+  p.smem_work = static_cast<int>(route > work ? route : work);
+  const size_t up_smem = p.smem_work + sizeof(UpSmem) + 8 * A;
+  const size_t down_smem = work + sizeof(Common) + 12 * A;
+  if (up_smem > kSmemMax || down_smem > kSmemMax) return kStatusUnsupported;
+  const int n = resident_clusters(up, clusters, dev), sms = num_sms();
   if (n < 1) return kStatusCuda;
+  p.down_teams = sms * kTeams;
 
-  cudaLaunchAttribute attr[2];
+  cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = kCluster;
   attr[0].val.clusterDim.y = 1;
@@ -908,14 +1450,21 @@ int launch_layer(const LayerParams& p, cudaStream_t st) {
   if (cudaLaunchKernelEx(&cfg, up, p) != cudaSuccess) return kStatusCuda;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(static_cast<unsigned>(num_sms()));
+  cfg.gridDim = dim3(static_cast<unsigned>(sms));
   cfg.dynamicSmemBytes = down_smem;
   if (cudaLaunchKernelEx(&cfg, down, p) != cudaSuccess) return kStatusCuda;
+  if (p.T > kAddTokens) {
+    cfg.gridDim = dim3(static_cast<unsigned>(ceil_div(p.H, 4 * kSumThreads)),
+                       static_cast<unsigned>(p.T));
+    cfg.blockDim = dim3(kSumThreads);
+    cfg.dynamicSmemBytes = 0;
+    if (cudaLaunchKernelEx(&cfg, few_sum_kernel<L>, p) != cudaSuccess) return kStatusCuda;
+  }
   return cudaPeekAtLastError() == cudaSuccess ? kStatusOk : kStatusCuda;
 }
 
 template <typename L>
-int layer_for_tokens(const LayerParams& p, cudaStream_t st) {
+int layer_for_tokens(LayerParams& p, cudaStream_t st) {
   return p.T <= 8 ? launch_layer<L, 1>(p, st) : launch_layer<L, 2>(p, st);
 }
 
@@ -933,7 +1482,7 @@ int launch_group(const GroupParams& p, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(num_sms()));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = sizeof(Meta) + sizeof(float) * kWarps * Shape<L, NG>::kTok * kRedLd;
+  cfg.dynamicSmemBytes = kWorkBytes<L, NG> + sizeof(GroupSmem);
   cfg.stream = st;
   if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) return kStatusCuda;
   const long long vecs = p.rows * ((p.down ? p.H : p.max_width) / 4);
@@ -956,6 +1505,9 @@ bool layer_sizes_ok(long long T, long long H, int E, int k, long long max_width,
          E <= kMaxExperts && k >= 1 && k <= E && k <= kMaxTopK && max_width >= 16 &&
          max_width % 16 == 0 && max_width <= kMaxWidth && act >= 0 && act <= 2;
 }
+
+constexpr long long kGroupHeader = 4 * (PLAN_WORDS + 3 * kMaxExperts);
+static_assert(kGroupHeader % 128 == 0, "partial sums follow");
 
 }  // namespace
 
@@ -993,13 +1545,15 @@ int few_tokens(const void* x, long long T, long long ldx, long long H, const voi
   p.shift = shift;
   p.blocks2 = static_cast<int>(blocks2); p.groups2 = static_cast<int>(groups2);
   p.out = out; p.ldo = ldo;
-  p.mask = reinterpret_cast<unsigned long long*>(b + plan.mask);
-  p.sel = reinterpret_cast<int*>(b + plan.sel);
+  p.plan = reinterpret_cast<int*>(b + plan.plan);
+  p.slot = reinterpret_cast<int*>(b + plan.slot);
+  p.row = reinterpret_cast<int*>(b + plan.row);
   p.wgt = reinterpret_cast<float*>(b + plan.wgt);
-  p.info = reinterpret_cast<int*>(b + plan.info);
   p.ticket = reinterpret_cast<int*>(b + plan.ticket);
   p.u = reinterpret_cast<float*>(b + plan.u);
   p.ldu = plan.ldu;
+  p.h = b + plan.h;
+  p.ldh = dtype == 2 ? max_width : 2 * max_width;
   p.y = reinterpret_cast<float*>(b + plan.y);
   p.max_slices = plan.slices;
   p.status = status;
@@ -1008,15 +1562,23 @@ int few_tokens(const void* x, long long T, long long ldx, long long H, const voi
     if (dtype == 1) return layer_for_tokens<Int4<__half>>(p, st);
     return kStatusUnsupported;
   }
+  if (dtype < 0 || dtype > 2) return kStatusUnsupported;
+  const bool gated = act == ACT_SWIGLU;
+  if (!weight_map(&p.map1, w1, dtype, H, total, gated) ||
+      !weight_map(&p.map2, w2, dtype, total / (gated ? 2 : 1), H, false))
+    return kStatusCuda;
   if (dtype == 0) return layer_for_tokens<Dense16<__nv_bfloat16>>(p, st);
   if (dtype == 1) return layer_for_tokens<Dense16<__half>>(p, st);
-  if (dtype == 2) return launch_layer<Dense32, 2>(p, st);
-  return kStatusUnsupported;
+  return launch_layer<Dense32, 2>(p, st);
 }
 
-long long grouped_int4_workspace(long long rows, long long cols) {
-  if (rows < 0 || rows > 65536 || cols < 16 || cols % 16 != 0 || cols > 2 * kMaxWidth) return -1;
-  return 128 + 4ll * slice_limit(rows * cols) * rows * cols;
+long long grouped_int4_workspace(long long rows, long long H, long long max_width, int act,
+                                 int down) {
+  if (rows < 0 || rows > 65536 || H < 16 || H % 16 != 0 || H > kMaxWidth || max_width < 16 ||
+      max_width % 16 != 0 || max_width > kMaxWidth || act < 0 || act > 2 || (down && act != 0))
+    return -1;
+  const long long cols = padded_columns(down ? H : max_width, act);
+  return kGroupHeader + 4ll * slice_limit(rows * cols) * rows * cols;
 }
 
 int grouped_int4(const void* x, long long rows, long long ldx, const void* w, const void* s,
@@ -1025,17 +1587,14 @@ int grouped_int4(const void* x, long long rows, long long ldx, const void* w, co
                  long long max_width, int act, int down, void* out, long long ldo, void* ws,
                  long long ws_bytes, int dtype, int* status, cudaStream_t st) {
   const int shift = group_shift(group);
-  const int gated = act == ACT_SWIGLU ? 2 : 1;
-  const long long cols = down ? H : gated * max_width, in = down ? max_width : H;
-  if (rows < 0 || rows > 65536 || H < 16 || H % 16 != 0 || H > kMaxWidth || total < 16 ||
-      total % 16 != 0 || total > (1ll << 30) || E < 1 || E > kMaxExperts || max_width < 16 ||
-      max_width % 16 != 0 || max_width > kMaxWidth || act < 0 || act > 2 || (down && act != 0) ||
-      shift == 0 || blocks < 0 || groups < 0 || blocks > (1 << 30) || groups > (1 << 30))
+  const long long need = grouped_int4_workspace(rows, H, max_width, act, down);
+  if (need < 0 || total < 16 || total % 16 != 0 || total > (1ll << 30) || E < 1 ||
+      E > kMaxExperts || shift == 0 || blocks < 0 || groups < 0 || blocks > (1 << 30) || groups > (1 << 30))
     return kStatusBadArg;
   if (rows == 0) return kStatusOk;
-  if (!x || !w || !s || !tok_off || !off || !out || !ws || ldx < in || ldx % 8 != 0 ||
+  if (!x || !w || !s || !tok_off || !off || !out || !ws || ldx < (down ? max_width : H) || ldx % 8 != 0 ||
       ldo < (down ? H : max_width) || !aligned16(x) || !aligned16(w) || !aligned16(s) ||
-      !aligned16(ws) || ws_bytes < grouped_int4_workspace(rows, cols))
+      !aligned16(ws) || ws_bytes < need)
     return kStatusBadArg;
   GroupParams p{};
   p.x = x; p.ldx = ldx; p.rows = rows; p.w = w; p.s = s;
@@ -1043,10 +1602,10 @@ int grouped_int4(const void* x, long long rows, long long ldx, const void* w, co
   p.E = E; p.H = static_cast<int>(H); p.total = static_cast<int>(total);
   p.max_width = static_cast<int>(max_width); p.act = act; p.down = down;
   p.shift = shift; p.blocks = static_cast<int>(blocks); p.groups = static_cast<int>(groups);
-  p.info = static_cast<int*>(ws);
-  p.part = reinterpret_cast<float*>(static_cast<unsigned char*>(ws) + 128);
-  p.ldp = cols;
-  p.max_slices = slice_limit(rows * cols);
+  p.plan = static_cast<int*>(ws);
+  p.part = reinterpret_cast<float*>(static_cast<unsigned char*>(ws) + kGroupHeader);
+  p.ldp = padded_columns(down ? H : max_width, act);
+  p.max_slices = slice_limit(rows * p.ldp);
   p.out = out; p.ldo = ldo; p.status = status;
   if (dtype == 0)
     return rows <= 8 ? launch_group<Int4<__nv_bfloat16>, 1>(p, st)

@@ -3,14 +3,15 @@
 //
 // With few rows per expert the products are bound by reading the weights once
 // (at 8 tokens: 16 flops per 2-byte weight against the ~250 that would balance
-// HBM and the tensor pipe), so the layout is chosen for the loads: a lane takes
-// 16-byte vectors straight from global memory into registers (no shared
-// memory, no barrier in the loop), a warp-wide load covers four 128-byte row
-// pieces, and the next step's vectors are in flight while the current ones are
-// multiplied.  The multiply is m16n8k16 with the weights as the 16-row operand
-// and the tokens as its 8 columns: any assignment of reduction rows to the
-// instruction's k slots is right as long as both operands share it, so the
-// lane's registers become fragments with one byte permute per weight pair.
+// HBM and the tensor pipe), so what counts is bytes in flight and instructions a
+// byte.  Every warp streams its own rows of a strip through a ring in shared
+// memory, one bulk copy (4 KB: 32 rows x 64 columns of 16-bit weights) a step,
+// issued by one lane; no other warp touches the ring, so the loop has no block
+// barrier and the ring runs on into the warp's next strip.  The multiply is
+// m16n8k16 with the weights as the 16-row operand and the tokens as its 8
+// columns.  (Register double buffering instead of the ring held half the bytes in
+// flight; per-lane asynchronous copies took five times the instructions: the
+// 128-expert layer at 64 tokens ran 722 and 1580 us a call.)
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -97,14 +98,56 @@ __device__ __forceinline__ void mma<__half>(float (&d)[4], const uint32_t (&a)[4
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Weights are read once: past L1, first to leave L2 (what is read again, the
-// token vectors and partial sums, stays).
+// 16 bytes that are read once: past L1.
 __device__ __forceinline__ uint4 ld_stream(const void* p) {
   uint4 v;
   asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0,%1,%2,%3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "l"(p));
   return v;
+}
+
+// ------------------------------------------------------------- bulk copies
+// Contiguous bytes to shared memory (addresses and size in multiples of 16).
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
+                                          uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void box_load(uint32_t dst, const void* tmap, int c0, int c1,
+                                         uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(tmap), "r"(c0), "r"(c1), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
+  asm volatile("{ .reg .b64 st; mbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1; }" ::"r"(bar),
+               "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t lds4(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void ldsm_trans(uint32_t (&a)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
+               : "r"(addr)
+               : "memory");
 }
 
 // -------------------------------------------------------------- activations
@@ -123,163 +166,200 @@ __device__ __forceinline__ float act_gated(float gate, float up) {
 }
 
 // ------------------------------------------------------------ token vectors
-// Where the multiplied vectors come from.  A lane asks for 8 consecutive
-// reduction elements of one row; rows past the count and elements past the end
-// are zero (never read), so nothing beyond a vector enters a sum.
+// The multiplied vectors.  A warp's lane g = lane / 4 holds rows g, g + 8, ..;
+// rows past the count are zero (never read), so nothing beyond a vector enters a
+// sum.
 
-// Rows of a matrix of the storage type (the layer's tokens, through an index
-// list, or the rows of a grouped product).
+// Index of the n-th (from 0) set bit, by halves.
+__device__ __forceinline__ int nth_bit(unsigned long long mask, int n) {
+  unsigned m = static_cast<unsigned>(mask);
+  int at = 0;
+  const int low = __popc(m);
+  if (n >= low) {
+    n -= low;
+    m = static_cast<unsigned>(mask >> 32);
+    at = 32;
+  }
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) {
+    const int c = __popc(m & ((1u << s) - 1));
+    if (n >= c) {
+      n -= c;
+      m >>= s;
+      at += s;
+    }
+  }
+  return at;
+}
+
+// Rows of a matrix of the storage type: the layer's tokens (the set bits of a
+// mask), or the rows of a grouped product.
 template <typename T>
 struct RowSource {
   static constexpr int kParts = 1;  // 16-bit operands per value
   const T* x;
   long long ld;
-  const int* list;  // row of the k-th vector (null: first + k)
+  unsigned long long mask;  // 0: rows first, first + 1, ..
   int first;
   __device__ __forceinline__ const T* row(int i) const {
-    return x + static_cast<long long>(list ? list[first + i] : first + i) * ld;
+    return x + static_cast<long long>(mask ? nth_bit(mask, first + i) : first + i) * ld;
   }
-  __device__ __forceinline__ void load8(const T* r, int k, uint4 (&b)[1]) const {
-    b[0] = *reinterpret_cast<const uint4*>(r + k);
-  }
-  __device__ __forceinline__ void load8f(const T* r, int k, float (&v)[8]) const {
-    const float4 a = *reinterpret_cast<const float4*>(r + k);
-    const float4 c = *reinterpret_cast<const float4*>(r + k + 4);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = c.x; v[5] = c.y; v[6] = c.z; v[7] = c.w;
-  }
+  static constexpr int half = 0;
 };
 
-// The activated intermediate, from the partial sums of the up product: the
-// slices are added in order and the activation applied on the way in.  For
-// 16-bit weights the fp32 value is split in two 16-bit operands (value and
-// remainder, about 2^-17 relative), multiplied one after the other: the
-// intermediate is never rounded to the storage type, and the second multiply
-// is free beside the weight loads.  In fp16 a value above 65504 is infinite, as
-// it is in the layer's forward, which stores it.
+// The layer's intermediate, already activated.  For 16-bit weights each fp32
+// value is held as two 16-bit operands (value and remainder: 2^-16 relative in
+// bf16, 2^-22 in fp16), multiplied one after the other: the intermediate is not
+// rounded to the storage type, and the second multiply is free beside the weight
+// loads.  In fp16 a value above 65504 is infinite, as it is in the layer's
+// forward, which stores it.  A row: [values | remainders].
 template <typename T>
-struct PartialSource {
+struct HiddenSource {
   static constexpr int kParts = 2;
-  const float* u;  // [slices][rows][ld]
-  long long ld, slice_stride;
-  int slices, first, act, width;  // width: the gated activation's second operand
-  __device__ __forceinline__ const float* row(int i) const {
-    return u + static_cast<long long>(first + i) * ld;
-  }
-  __device__ __forceinline__ void sum8(const float* r, float (&v)[8]) const {
-    float4 a = *reinterpret_cast<const float4*>(r);
-    float4 c = *reinterpret_cast<const float4*>(r + 4);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = c.x; v[5] = c.y; v[6] = c.z; v[7] = c.w;
-#pragma unroll 4
-    for (int s = 1; s < slices; ++s) {
-      r += slice_stride;
-      a = *reinterpret_cast<const float4*>(r);
-      c = *reinterpret_cast<const float4*>(r + 4);
-      v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-      v[4] += c.x; v[5] += c.y; v[6] += c.z; v[7] += c.w;
-    }
-  }
-  __device__ __forceinline__ void load8f(const float* r, int k, float (&v)[8]) const {
-    sum8(r + k, v);
-    if (act == ACT_SWIGLU) {
-      float up[8];
-      sum8(r + k + width, up);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = act_gated(v[i], up[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = act_plain(v[i], act);
-    }
-  }
-  __device__ __forceinline__ void load8(const float* r, int k, uint4 (&b)[2]) const {
-    float v[8];
-    load8f(r, k, v);
-    uint32_t hi[4], lo[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      hi[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
-      const float2 h = unpack2<T>(hi[i]);
-      // an infinite or NaN value has no remainder
-      const float l0 = v[2 * i] - h.x, l1 = v[2 * i + 1] - h.y;
-      lo[i] = pack2<T>(fabsf(h.x) <= 3.4e38f ? l0 : 0.f, fabsf(h.y) <= 3.4e38f ? l1 : 0.f);
-    }
-    b[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    b[1] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+  const T* h;
+  long long ld;
+  int half;  // remainders this far behind the values
+  int first;
+  __device__ __forceinline__ const T* row(int i) const {
+    return h + static_cast<long long>(first + i) * ld;
   }
 };
+template <typename T>
+__device__ __forceinline__ void hidden_store4(T* row, int half, int c, const float (&v)[4]) {
+  uint32_t hi[2], lo[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    hi[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+    const float2 h = unpack2<T>(hi[i]);
+    // an infinite or NaN value has no remainder
+    lo[i] = pack2<T>(fabsf(h.x) <= 3.4e38f ? v[2 * i] - h.x : 0.f,
+                     fabsf(h.y) <= 3.4e38f ? v[2 * i + 1] - h.y : 0.f);
+  }
+  *reinterpret_cast<uint2*>(row + c) = make_uint2(hi[0], hi[1]);
+  *reinterpret_cast<uint2*>(row + half + c) = make_uint2(lo[0], lo[1]);
+}
+template <>
+__device__ __forceinline__ void hidden_store4<float>(float* row, int, int c, const float (&v)[4]) {
+  *reinterpret_cast<float4*>(row + c) = make_float4(v[0], v[1], v[2], v[3]);
+}
 
 // ------------------------------------------------------------------ weights
-// A strip: the reduction rows [0, rows) of one expert's weights and 64 of its
-// columns (fewer at the right edge; a multiple of 16 always).
+// A strip: reduction rows up to `end` of one expert's weights and 64 of its
+// columns, in two halves of 32: side by side, or (a gated activation) 32 gate
+// columns and the 32 up columns they go with, `jump` further right.  `lo` and `hi`
+// of each half's columns exist, in multiples of 16; the sums of others are
+// meaningless and nobody reads them.
+struct Strip {
+  int row, col;        // matrix row of reduction row 0; first column
+  int end;             // reduction rows
+  int lo, hi, jump;
+  int kb, sg, groups;  // 4-bit: first block row; first group, number of groups
+};
 
-// 16-bit weights, row-major.  One step is 32 rows: lane (g = lane / 4,
-// t = lane % 4) loads columns 8g..8g+7 of rows 8t..8t+7.  Multiply (i, s), i < 4,
-// s < 2, takes columns 8g + 2i and 8g + 2i + 1 as its rows g and g + 8 and
-// reduction rows 8t + 4s .. 8t + 4s + 3 as lane t's k slots.
+// What a matrix is to the copies.
+struct Matrix {
+  const void* map;     // dense: tensor map (boxes of 64, gated 32, columns)
+  const void* w;       // 4-bit: packed blocks, scales
+  const void* scales;
+  int cols;
+  int shift;           // log2 of the group
+  int gated;
+};
+
+// 16-bit weights, row-major.  One step is a box of 32 rows x 64 columns, 128-byte
+// swizzled (gated: two of 32 columns, 64-byte swizzled).  Lane t = lane % 4 has
+// reduction rows 16 s + 4 t .. + 3 as its k slots of multiply s: for t < 2 the
+// first two as the instruction's slots 2t, 2t + 1 and the others as 2t + 8, 2t + 9,
+// for t >= 2 the other way round, which makes the eight rows of each transposed
+// 8 x 8 load different modulo 8 (no bank conflict) and a lane's token elements four
+// in a row.
 template <typename T>
 struct Dense16 {
   using Elem = T;
   static constexpr int kStep = 32;
-  struct Strip {
-    const T* w;  // first row, first column of the strip
-    long long ld;
-    int rows, cols;
-  };
-  struct Frag {
-    uint4 v[8];
-  };
-  static __device__ __forceinline__ void load(const Strip& s, int k0, int lane, Frag& f) {
-    const int g = lane >> 2, k = k0 + 8 * (lane & 3);
-    const bool ok = 8 * g < s.cols && k < s.rows;  // rows and columns come in 8s
-    const T* p = s.w + static_cast<long long>(k) * s.ld + 8 * g;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f.v[i] = ok ? ld_stream(p + i * s.ld) : make_uint4(0, 0, 0, 0);
-  }
-  template <int NG, typename Src>
-  static __device__ __forceinline__ void step(float (&acc)[4][NG][4], const Frag& f,
-                                              const Strip& s, int k0, int lane, const Src& src,
-                                              int count) {
-    const int g = lane >> 2, k = k0 + 8 * (lane & 3);
-    uint4 b[NG][Src::kParts];
-#pragma unroll
-    for (int n = 0; n < NG; ++n) {
-#pragma unroll
-      for (int p = 0; p < Src::kParts; ++p) b[n][p] = make_uint4(0, 0, 0, 0);
-      if (8 * n + g < count && k < s.rows) src.load8(src.row(8 * n + g), k, b[n]);
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t* r0 = reinterpret_cast<const uint32_t*>(&f.v[4 * h]);
-      const uint32_t* r1 = reinterpret_cast<const uint32_t*>(&f.v[4 * h + 1]);
-      const uint32_t* r2 = reinterpret_cast<const uint32_t*>(&f.v[4 * h + 2]);
-      const uint32_t* r3 = reinterpret_cast<const uint32_t*>(&f.v[4 * h + 3]);
+  static constexpr int kStage = 4096;  // bytes of a step in the ring
+  template <int NG>
+  static constexpr int kDepth = 2;     // steps in the ring
+  template <int NG>
+  static constexpr int kTokens = 8 * NG;
+  // per-lane offsets into a stage
+  struct Lane {
+    uint32_t off[4];  // of multiply i's 16 columns
+    uint32_t half;    // bytes of 16 rows
+    __device__ __forceinline__ Lane(int lane, int gated) {
+      const int mi = lane >> 3, j = lane & 7, t = j >> 1;
+      const int row = 4 * t + 2 * ((mi >> 1) ^ (t >> 1)) + (j & 1);
+      half = gated ? 1024 : 2048;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t a[4] = {__byte_perm(r0[i], r1[i], 0x5410), __byte_perm(r0[i], r1[i], 0x7632),
-                               __byte_perm(r2[i], r3[i], 0x5410), __byte_perm(r2[i], r3[i], 0x7632)};
+        const int c = 2 * i + (mi & 1);  // 8-column chunk
+        off[i] = gated ? (c >> 2) * 2048 + row * 64 + (((c & 3) ^ (row >> 1 & 3)) << 4)
+                       : row * 128 + ((c ^ (row & 7)) << 4);
+      }
+    }
+  };
+  static __device__ __forceinline__ void issue(const Matrix& m, const Strip& s, int k, uint32_t stage,
+                                               uint32_t bar) {
+    expect_bytes(bar, kStage);
+    box_load(stage, m.map, s.col, s.row + k, bar);
+    if (m.gated) box_load(stage + 2048, m.map, s.col + s.jump, s.row + k, bar);
+  }
+  template <int NG, typename Src>
+  struct Vectors {
+    const T* r[NG];
+    uint2 b[NG][Src::kParts][2];
+    __device__ __forceinline__ void rows(const Src& src, int count, int lane) {
+      const int g = lane >> 2;
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+        r[n] = 8 * n + g < count ? src.row(8 * n + g) + 4 * (lane & 3) : nullptr;
+    }
+    __device__ __forceinline__ void load(const Src& src, const Strip& s, int k, int lane) {
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int p = 0; p < Src::kParts; ++p)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint2 v = make_uint2(0u, 0u);
+            if (r[n] && k + 16 * h < s.end)
+              v = *reinterpret_cast<const uint2*>(r[n] + p * src.half + k + 16 * h);
+            b[n][p][h] = (lane & 2) ? make_uint2(v.y, v.x) : v;
+          }
+    }
+  };
+  template <int NG, typename Src>
+  static __device__ __forceinline__ void step(float (&acc)[4][NG][4], const Lane& l,
+                                              const Matrix&, const Strip& s, int k, uint32_t stage,
+                                              int, const Vectors<NG, Src>& v) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (h && k + 16 >= s.end) break;  // rows beyond are another expert's
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t a[4];
+        ldsm_trans(a, stage + h * l.half + l.off[i]);
 #pragma unroll
         for (int n = 0; n < NG; ++n)
 #pragma unroll
           for (int p = 0; p < Src::kParts; ++p)
-            mma<T>(acc[i][n], a, h ? b[n][p].z : b[n][p].x, h ? b[n][p].w : b[n][p].y);
+            mma<T>(acc[i][n], a, v.b[n][p][h].x, v.b[n][p][h].y);
       }
     }
   }
-  // red[token][64 columns] (row stride kRedLd) of this warp's sums
-  template <int NG, int LD>
+  // The lane's sums to (ADD: added to) red[token][64 columns], row stride LD.
+  template <int NG, int LD, bool ADD>
   static __device__ __forceinline__ void store(const float (&acc)[4][NG][4], int lane, float* red) {
     const int g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int n = 0; n < NG; ++n)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float* p = red + (8 * n + 2 * t + j) * LD + 8 * g;
-        *reinterpret_cast<float4*>(p) =
-            make_float4(acc[0][n][j], acc[0][n][j + 2], acc[1][n][j], acc[1][n][j + 2]);
-        *reinterpret_cast<float4*>(p + 4) =
-            make_float4(acc[2][n][j], acc[2][n][j + 2], acc[3][n][j], acc[3][n][j + 2]);
-      }
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float* p = red + (8 * n + 2 * t + (c & 1)) * LD + 16 * i + 8 * (c >> 1) + g;
+          *p = ADD ? *p + acc[i][n][c] : acc[i][n][c];
+        }
   }
 };
 
@@ -294,58 +374,80 @@ template <typename T>
 struct Int4 {
   using Elem = T;
   static constexpr int kStep = 64;
-  struct Strip {
-    const uint4* w;   // first block row, first column block of the strip
-    long long ld;     // blocks a block row
-    const T* scales;  // first group, first column
-    long long lds;
-    int rows, cols, shift, groups;  // 2^shift rows a group
+  static constexpr int kStage = 2048 + 2 * 128;  // weights, then scales of two groups
+  template <int NG>
+  static constexpr int kDepth = 4;
+  template <int NG>
+  static constexpr int kTokens = 8 * NG;
+  struct Lane {
+    __device__ __forceinline__ Lane(int, int) {}
   };
-  struct Frag {
-    uint4 v[4];
-    uint32_t sc[2][4];
-  };
-  static __device__ __forceinline__ void load(const Strip& s, int k0, int lane, Frag& f) {
-    const uint4* p = s.w + (static_cast<long long>(k0 >> 6) * s.ld) * 32 + lane;
-    const bool in = k0 < s.rows;
-    const int g0 = min(k0 >> s.shift, s.groups - 1);
-    const T* sp = s.scales + static_cast<long long>(g0) * s.lds + 2 * (lane >> 2);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool ok = in && 16 * i < s.cols;
-      f.v[i] = ok ? ld_stream(p + 32 * i) : make_uint4(0, 0, 0, 0);
-      f.sc[0][i] = ok ? __ldg(reinterpret_cast<const uint32_t*>(sp + 16 * i)) : 0u;
-    }
-    if (s.shift == 5) {
-      const int g1 = min(g0 + 1, s.groups - 1);
-      const T* sq = s.scales + static_cast<long long>(g1) * s.lds + 2 * (lane >> 2);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        f.sc[1][i] = in && 16 * i < s.cols ? __ldg(reinterpret_cast<const uint32_t*>(sq + 16 * i)) : 0u;
+  static __device__ __forceinline__ void issue(const Matrix& m, const Strip& s, int k, uint32_t stage,
+                                               uint32_t bar) {
+    const long long nb = m.cols / 16;
+    const char* w = static_cast<const char*>(m.w) + ((s.kb + (k >> 6)) * nb + s.col / 16) * 512;
+    const int g0 = min(k >> m.shift, s.groups - 1);
+    const T* sc = static_cast<const T*>(m.scales) +
+                  static_cast<long long>(s.sg + g0) * m.cols + s.col;
+    // a second group in the step, unless the weight ends before it
+    const bool two = m.shift == 5;
+    const long long next = g0 + 1 < s.groups ? m.cols : 0;
+    const int n = s.lo + s.hi;
+    expect_bytes(bar, 32 * n + (two ? 4 : 2) * n);
+    if (m.gated) {
+      bulk_load(stage, w, 32 * s.lo, bar);
+      bulk_load(stage + 1024, w + 32ll * s.jump, 32 * s.hi, bar);
+      bulk_load(stage + 2048, sc, 2 * s.lo, bar);
+      bulk_load(stage + 2048 + 64, sc + s.jump, 2 * s.hi, bar);
+      if (two) {
+        bulk_load(stage + 2176, sc + next, 2 * s.lo, bar);
+        bulk_load(stage + 2176 + 64, sc + next + s.jump, 2 * s.hi, bar);
+      }
     } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) f.sc[1][i] = f.sc[0][i];
+      bulk_load(stage, w, 32 * n, bar);
+      bulk_load(stage + 2048, sc, 2 * n, bar);
+      if (two) bulk_load(stage + 2176, sc + next, 2 * n, bar);
     }
   }
+  template <int NG, typename Src>
+  struct Vectors {
+    const T* r[NG];
+    uint4 b[2][NG][Src::kParts];
+    __device__ __forceinline__ void rows(const Src& src, int count, int lane) {
+      const int g = lane >> 2;
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+        r[n] = 8 * n + g < count ? src.row(8 * n + g) + 8 * (lane & 3) : nullptr;
+    }
+    __device__ __forceinline__ void load(const Src& src, const Strip& s, int k, int lane) {
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int p = 0; p < Src::kParts; ++p)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            b[h][n][p] = make_uint4(0, 0, 0, 0);
+            if (r[n] && k + 32 * h + 8 * (lane & 3) < s.end)
+              b[h][n][p] = *reinterpret_cast<const uint4*>(r[n] + p * src.half + k + 32 * h);
+          }
+    }
+  };
   // nibbles j and j + 4 of w as two 16-bit numbers q - 8 (exact: 128 + q, or
   // 1024 + q, is the number whose low mantissa bits are q)
   static __device__ __forceinline__ uint32_t nibbles(uint32_t w, int j);
   template <int NG, typename Src>
-  static __device__ __forceinline__ void step(float (&acc)[4][NG][4], const Frag& f,
-                                              const Strip& s, int k0, int lane, const Src& src,
-                                              int count) {
+  static __device__ __forceinline__ void step(float (&acc)[4][NG][4], const Lane&,
+                                              const Matrix& m, const Strip&, int, uint32_t stage,
+                                              int lane, const Vectors<NG, Src>& v) {
+    const bool two = m.shift == 5;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {  // 32 rows each
-      const int g = lane >> 2, k = k0 + 32 * h + 8 * (lane & 3);
-      uint4 b[NG][Src::kParts];
+    for (int i = 0; i < 4; ++i) {
+      const uint4 f = lds16(stage + 512 * i + 16 * lane);
+      const uint32_t* word = reinterpret_cast<const uint32_t*>(&f);
+      const uint32_t sc0 = lds4(stage + 2048 + 32 * i + 4 * (lane >> 2));
+      const uint32_t sc1 = two ? lds4(stage + 2176 + 32 * i + 4 * (lane >> 2)) : sc0;
 #pragma unroll
-      for (int n = 0; n < NG; ++n) {
-#pragma unroll
-        for (int p = 0; p < Src::kParts; ++p) b[n][p] = make_uint4(0, 0, 0, 0);
-        if (8 * n + g < count && k < s.rows) src.load8(src.row(8 * n + g), k, b[n]);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int h = 0; h < 2; ++h) {  // 32 rows each
         float part[NG][4];
 #pragma unroll
         for (int n = 0; n < NG; ++n)
@@ -353,15 +455,16 @@ struct Int4 {
           for (int c = 0; c < 4; ++c) part[n][c] = 0.f;
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          const uint32_t w = reinterpret_cast<const uint32_t*>(&f.v[i])[2 * h + q];
+          const uint32_t w = word[2 * h + q];
           const uint32_t a[4] = {nibbles(w, 0), nibbles(w, 1), nibbles(w, 2), nibbles(w, 3)};
 #pragma unroll
           for (int n = 0; n < NG; ++n)
 #pragma unroll
             for (int p = 0; p < Src::kParts; ++p)
-              mma<T>(part[n], a, q ? b[n][p].z : b[n][p].x, q ? b[n][p].w : b[n][p].y);
+              mma<T>(part[n], a, q ? v.b[h][n][p].z : v.b[h][n][p].x,
+                     q ? v.b[h][n][p].w : v.b[h][n][p].y);
         }
-        const float2 sc = unpack2<T>(f.sc[h][i]);
+        const float2 sc = unpack2<T>(h ? sc1 : sc0);
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
           acc[i][n][0] += sc.x * part[n][0];
@@ -372,7 +475,7 @@ struct Int4 {
       }
     }
   }
-  template <int NG, int LD>
+  template <int NG, int LD, bool ADD>
   static __device__ __forceinline__ void store(const float (&acc)[4][NG][4], int lane, float* red) {
     const int g = lane >> 2, t = lane & 3;
 #pragma unroll
@@ -381,8 +484,16 @@ struct Int4 {
       for (int j = 0; j < 2; ++j) {
         float* p = red + (8 * n + 2 * t + j) * LD + 2 * g;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<float2*>(p + 16 * i) = make_float2(acc[i][n][j], acc[i][n][j + 2]);
+        for (int i = 0; i < 4; ++i) {
+          float2* d = reinterpret_cast<float2*>(p + 16 * i);
+          float2 a = make_float2(acc[i][n][j], acc[i][n][j + 2]);
+          if (ADD) {
+            const float2 x = *d;
+            a.x += x.x;
+            a.y += x.y;
+          }
+          *d = a;
+        }
       }
   }
 };
@@ -404,51 +515,72 @@ __device__ __forceinline__ uint32_t Int4<__half>::nibbles(uint32_t w, int j) {
 }
 
 // fp32 weights: plain FMAs (the tensor pipe's tf32 would drop 13 bits of both
-// operands).  One step is 16 rows: half-warp p loads columns 4c..4c+3 (c =
-// lane % 16) of rows 8p..8p+7; the token values are the same for all lanes of a
-// half-warp (one broadcast load each).  The halves are added at the end.
+// operands).  One step is a box of 16 rows x 64 columns (gated: two of 32): half-warp
+// p takes columns 4c..4c+3 (c = lane % 16) of rows 8p..8p+7; the token values are
+// the same for all lanes of a half-warp (broadcast loads).  The halves are added
+// at the end.
 struct Dense32 {
   using Elem = float;
   static constexpr int kStep = 16;
-  struct Strip {
-    const float* w;
-    long long ld;
-    int rows, cols;
+  static constexpr int kStage = 4096;
+  template <int NG>
+  static constexpr int kDepth = 2;
+  template <int NG>
+  static constexpr int kTokens = 4 * NG;  // acc[4][NG][4]: 4 NG tokens x 4 columns
+  struct Lane {
+    uint32_t off, ld;
+    __device__ __forceinline__ Lane(int lane, int gated) {
+      const int p = lane >> 4, c = lane & 15;
+      ld = gated ? 128 : 256;
+      off = gated ? (c >> 3) * 2048 + p * 1024 + (c & 7) * 16 : p * 2048 + c * 16;
+    }
   };
-  struct Frag {
-    uint4 v[8];
-  };
-  static __device__ __forceinline__ void load(const Strip& s, int k0, int lane, Frag& f) {
-    const int c = 4 * (lane & 15), k = k0 + 8 * (lane >> 4);
-    const bool ok = c < s.cols && k < s.rows;
-    const float* p = s.w + static_cast<long long>(k) * s.ld + c;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f.v[i] = ok ? ld_stream(p + i * s.ld) : make_uint4(0, 0, 0, 0);
+  static __device__ __forceinline__ void issue(const Matrix& m, const Strip& s, int k, uint32_t stage,
+                                               uint32_t bar) {
+    expect_bytes(bar, kStage);
+    box_load(stage, m.map, s.col, s.row + k, bar);
+    if (m.gated) box_load(stage + 2048, m.map, s.col + s.jump, s.row + k, bar);
   }
-  // acc[token][column]: NG is 2 here for 8 tokens of 4 columns (32 sums)
   template <int NG, typename Src>
-  static __device__ __forceinline__ void step(float (&acc)[4][NG][4], const Frag& f,
-                                              const Strip& s, int k0, int lane, const Src& src,
-                                              int count) {
+  struct Vectors {
+    const float* r[4 * NG];
+    __device__ __forceinline__ void rows(const Src& src, int count, int) {
+#pragma unroll
+      for (int t = 0; t < 4 * NG; ++t) r[t] = t < count ? src.row(t) : nullptr;
+    }
+    __device__ __forceinline__ void load(const Src&, const Strip&, int, int) {}
+  };
+  template <int NG, typename Src>
+  static __device__ __forceinline__ void step(float (&acc)[4][NG][4], const Lane& l,
+                                              const Matrix&, const Strip& s, int k0, uint32_t stage,
+                                              int lane, const Vectors<NG, Src>& v) {
     const int k = k0 + 8 * (lane >> 4);
-    if (k >= s.rows) return;
+    if (k >= s.end) return;
+    float4 w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint4 f = lds16(stage + l.off + i * l.ld);
+      w[i] = *reinterpret_cast<const float4*>(&f);
+    }
 #pragma unroll
     for (int t = 0; t < 4 * NG; ++t) {
-      if (t >= count) break;
-      float v[8];
-      src.load8f(src.row(t), k, v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float4 w = *reinterpret_cast<const float4*>(&f.v[i]);
+      if (v.r[t]) {
+        const float* x = v.r[t] + k;
+        const float4 x0 = *reinterpret_cast<const float4*>(x);
+        const float4 x1 = *reinterpret_cast<const float4*>(x + 4);
+        const float xs[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
         float(&a)[4] = acc[t / NG][t % NG];
-        a[0] = fmaf(v[i], w.x, a[0]);
-        a[1] = fmaf(v[i], w.y, a[1]);
-        a[2] = fmaf(v[i], w.z, a[2]);
-        a[3] = fmaf(v[i], w.w, a[3]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          a[0] = fmaf(xs[i], w[i].x, a[0]);
+          a[1] = fmaf(xs[i], w[i].y, a[1]);
+          a[2] = fmaf(xs[i], w[i].z, a[2]);
+          a[3] = fmaf(xs[i], w[i].w, a[3]);
+        }
       }
     }
   }
-  template <int NG, int LD>
+  template <int NG, int LD, bool ADD>
   static __device__ __forceinline__ void store(const float (&acc)[4][NG][4], int lane, float* red) {
 #pragma unroll
     for (int t = 0; t < 4 * NG; ++t) {
@@ -456,41 +588,17 @@ struct Dense32 {
       float v[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) v[c] = a[c] + __shfl_xor_sync(0xffffffffu, a[c], 16);
-      if (lane < 16)
-        *reinterpret_cast<float4*>(red + t * LD + 4 * lane) = make_float4(v[0], v[1], v[2], v[3]);
+      if (lane < 16) {
+        float4* d = reinterpret_cast<float4*>(red + t * LD + 4 * lane);
+        if (ADD) {
+          const float4 x = *d;
+          v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+        }
+        *d = make_float4(v[0], v[1], v[2], v[3]);
+      }
     }
   }
 };
-
-// One warp's share of a strip: steps begin + wr * kStep, + stride, ... below
-// s.rows, the next step's weights loading while one is multiplied; its sums go
-// to red[token][column].
-template <typename L, int NG, int STRIDE, int LD, typename Src>
-__device__ __forceinline__ void product(const typename L::Strip& s, const Src& src, int count,
-                                        int k, int lane, float* red) {
-  float acc[4][NG][4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int n = 0; n < NG; ++n)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) acc[i][n][c] = 0.f;
-  typename L::Frag f0, f1;
-  if (k < s.rows) {
-    L::load(s, k, lane, f0);
-    while (true) {
-      if (k + STRIDE < s.rows) L::load(s, k + STRIDE, lane, f1);
-      L::template step<NG>(acc, f0, s, k, lane, src, count);
-      k += STRIDE;
-      if (k >= s.rows) break;
-      if (k + STRIDE < s.rows) L::load(s, k + STRIDE, lane, f0);
-      L::template step<NG>(acc, f1, s, k, lane, src, count);
-      k += STRIDE;
-      if (k >= s.rows) break;
-    }
-  }
-  L::template store<NG, LD>(acc, lane, red);
-}
 
 }  // namespace few
 }  // namespace moe

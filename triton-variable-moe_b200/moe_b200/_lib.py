@@ -100,7 +100,7 @@ _SIGS = {
     "moe_int4_quantize": [_P, _L, _L, _L, _I, _I, _P, _I, _P, _P, _I, _P],
     "moe_int4_pack": [_P, _L, _L, _L, _I, _P, _I, _P, _P],
     "moe_int4_dequantize": [_P, _P, _L, _L, _I, _P, _I, _P, _L, _I, _P],
-    "moe_grouped_gemv_int4_workspace_bytes": [_L, _L],
+    "moe_grouped_gemv_int4_workspace_bytes": [_L, _L, _L, _I, _I],
     "moe_grouped_gemv_int4": [_P, _L, _L, _P, _P, _I, _L, _L, _L, _L, _P, _P, _P, _I, _L, _I, _I, _P,
                               _L, _P, _L, _I, _P, _P],
 }

@@ -273,8 +273,8 @@ def _gemv(name, x, q, tok_off, w_off, expert_widths, tok_cnt, hidden, max_width,
         return out
     x = row_view(x)
     tok_off, w_off, tok_cnt = _meta(tok_off), _meta(w_off), _meta(tok_cnt)
-    prod = hidden if down else max_width * (2 if activation == "swiglu" else 1)
-    ws_bytes = int(lib.moe_grouped_gemv_int4_workspace_bytes(rows, prod))
+    ws_bytes = int(lib.moe_grouped_gemv_int4_workspace_bytes(
+        rows, hidden, max_width, ACT_CODE[activation], 1 if down else 0))
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     with on_device(dev):
         ev = _ev_begin()
