@@ -9,6 +9,8 @@ Each reference returns (value, bound).  The bound follows the kernels' arithmeti
     smallest step 2^-24;
   * the routing weight: sigmoid and one division, 2^-20 relative, plus the error of
     its logit (its derivative is at most 1/4 of it, absolutely; p(1-p) relative 1-p).
+  * 4-bit weights: the sums hold terms of (31 + 24) scales in bf16, (143 + 136) in
+    fp16, for a weight (q - 8) scale, so their magnitudes are taken with those.
 First-order terms are carried through the activation; nothing is fitted.
 """
 
@@ -56,8 +58,15 @@ def clear_choice(x, router, k):
     return bool(((gap > 2 * err) | (gap == 0)).all())
 
 
-def layer(x, router, w1, w2, offsets, k, norm, act):
-    """offsets: host list of w1's column offsets.  Returns (out, bound) in fp64."""
+def int4_terms(scales, dtype):
+    """Magnitudes of the terms in the sums of 4-bit weights, from the scale of each."""
+    return scales.double().abs() * (55 if dtype == torch.bfloat16 else 279)
+
+
+def layer(x, router, w1, w2, offsets, k, norm, act, m1=None, m2=None):
+    """offsets: host list of w1's column offsets; m1, m2: magnitudes of the summed
+    terms (default: of the weights).  Returns (out, bound) in fp64."""
+    m1, m2 = w1 if m1 is None else m1, w2 if m2 is None else m2
     dt = x.dtype
     half = HALF_STEP[dt]
     gated = 2 if act == "swiglu" else 1
@@ -80,12 +89,13 @@ def layer(x, router, w1, w2, offsets, k, norm, act):
             continue
         a, b = offsets[e], offsets[e + 1]
         w1e, w2e = w1[:, a:b].double(), w2[a // gated:b // gated].double()
+        m1e, m2e = m1[:, a:b].double().abs(), m2[a // gated:b // gated].double().abs()
         u = xd[t] @ w1e
-        h, dh = activate(u, (xd[t].abs() @ w1e.abs()) * adds(H, dt), act)
+        h, dh = activate(u, (xd[t].abs() @ m1e) * adds(H, dt), act)
         if dt != torch.float32:
             dh = dh + h.abs() * half * half + (2.0**-24 if dt == torch.float16 else 0.0)
         y = h @ w2e
-        mag = h.abs() @ w2e.abs()
+        mag = h.abs() @ m2e
         dy = dh @ w2e.abs() + mag * adds(b - a, dt)
         g, dg = p[t, slot, None], perr[t, slot, None]
         out[t] += g * y
@@ -93,8 +103,9 @@ def layer(x, router, w1, w2, offsets, k, norm, act):
     return out, err + out.abs() * half * (1 + 2.0**-10) + (2.0**-24 if dt == torch.float16 else 1e-38)
 
 
-def grouped(x, w, row_ranges, offsets, max_width, act, down):
-    """row_ranges: [(first, count)] an expert; w: fp64-able matrix."""
+def grouped(x, w, row_ranges, offsets, max_width, act, down, m=None):
+    """row_ranges: [(first, count)] an expert; w: fp64-able matrix; m: as layer's."""
+    m = w if m is None else m
     dt = x.dtype
     half = HALF_STEP[dt]
     gated = 2 if act == "swiglu" else 1
@@ -110,7 +121,8 @@ def grouped(x, w, row_ranges, offsets, max_width, act, down):
         if down:
             xe = xe[:, :b - a]
         u = xe @ we
-        h, dh = activate(u, (xe.abs() @ we.abs()) * adds(xe.shape[1], dt), act)
+        me = (m[a:b] if down else m[:, a:b]).double().abs()
+        h, dh = activate(u, (xe.abs() @ me) * adds(xe.shape[1], dt), act)
         c = cols if down else (b - a) // gated
         out[r:r + n, :c] = h
         err[r:r + n, :c] = dh + h.abs() * half * (1 + 2.0**-10)

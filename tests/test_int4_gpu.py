@@ -17,14 +17,18 @@ def weight(K, N, dtype, seed=0, std=0.05):
     return (torch.randn(K, N, generator=g) * std).to("cuda", dtype)
 
 
-def values(codes, scales, group, segments):
-    """(q - 8) * scale in fp64."""
+def spread(scales, group, segments):
+    """The scale of every weight, in fp64."""
     gid, base = [], 0
     for n in segments:
         gid += [base + i // group for i in range(n)]
         base += -(-n // group)
-    gid = torch.tensor(gid, device=codes.device)
-    return (codes.double() - 8) * scales.double()[gid]
+    return scales.double()[torch.tensor(gid, device=scales.device)]
+
+
+def values(codes, scales, group, segments):
+    """(q - 8) * scale in fp64."""
+    return (codes.double() - 8) * spread(scales, group, segments)
 
 
 def offsets(segments):
@@ -116,7 +120,7 @@ def test_strided_weight(device):
 
 
 def quantized(p, act, group):
-    """Int4 weights of make()'s layer, and their exact values."""
+    """Int4 weights of make()'s layer, their exact values, and their terms' magnitudes."""
     from moe_b200.kernels import quantize_int4
 
     gated = 2 if act == "swiglu" else 1
@@ -125,7 +129,9 @@ def quantized(p, act, group):
     seg2 = [b - a for a, b in zip(rows, rows[1:])]
     c1, s1 = ref.quantize(p["w1"], group, [p["w1"].shape[0]], p["w1"].dtype)
     c2, s2 = ref.quantize(p["w2"], group, seg2, p["w2"].dtype)
-    return q1, q2, values(c1, s1, group, [p["w1"].shape[0]]), values(c2, s2, group, seg2)
+    seg1, dt = [p["w1"].shape[0]], p["w1"].dtype
+    return (q1, q2, values(c1, s1, group, seg1), values(c2, s2, group, seg2),
+            ref.int4_terms(spread(s1, group, seg1), dt), ref.int4_terms(spread(s2, group, seg2), dt))
 
 
 LAYERS = [
@@ -145,10 +151,10 @@ def test_layer_on_int4_experts(T, H, sizes, k, norm, act, dtype, group, device):
     from moe_b200.kernels import check_device_status, moe_few_tokens
 
     p = make(T, H, sizes, dtype, act, seed=4, k=k)
-    q1, q2, v1, v2 = quantized(p, act, group)
+    q1, q2, v1, v2, m1, m2 = quantized(p, act, group)
     off = torch.tensor(p["off"], dtype=torch.int32, device=device)
     out = moe_few_tokens(p["x"], p["router"], q1, q2, off, p["max_width"], k, norm, act)
-    r, b = ref.layer(p["x"], p["router"], v1, v2, p["off"], k, norm, act)
+    r, b = ref.layer(p["x"], p["router"], v1, v2, p["off"], k, norm, act, m1, m2)
     ref.assert_within(out, r, b, "out")
     assert torch.equal(out, moe_few_tokens(p["x"], p["router"], q1, q2, off, p["max_width"], k,
                                            norm, act))
@@ -175,7 +181,7 @@ def test_grouped_products(counts, slack, H, sizes, act, dtype, group, down, devi
     if down:
         act = "none"
     p = make(1, H, sizes, dtype, act, seed=5)
-    q1, q2, v1, v2 = quantized(p, act, group)
+    q1, q2, v1, v2, m1, m2 = quantized(p, act, group)
     widths, E, mw = widths_of(sizes), len(counts), p["max_width"]
     start = offsets([c + slack for c in counts])
     rows = start[-1] + 2
@@ -192,7 +198,8 @@ def test_grouped_products(counts, slack, H, sizes, act, dtype, group, down, devi
         out = grouped_gemv_down_int4(x, q2, tok, off, wid, cnt, H)
     else:
         out = grouped_gemv_up_int4(x, q1, tok, off, wid, cnt, mw, activation=act)
-    r, b = ref.grouped(x, v2 if down else v1, list(zip(start, counts)), p["off"], mw, act, down)
+    r, b = ref.grouped(x, v2 if down else v1, list(zip(start, counts)), p["off"], mw, act, down,
+                       m2 if down else m1)
     ref.assert_within(out, r, b, "out")
     if slack == 0:  # without counts: all of an expert's rows
         again = (grouped_gemv_down_int4(x, q2, tok, off, wid, None, H) if down else
@@ -209,7 +216,7 @@ def test_products_make_the_layer(device):
     from moe_b200.kernels._ops import router_topk
 
     p = make(6, 256, [(4, 128), (4, 64)], BF, seed=8)
-    q1, q2, _, _ = quantized(p, "relu_squared", 64)
+    q1, q2, *_ = quantized(p, "relu_squared", 64)
     i32 = dict(dtype=torch.int32, device=device)
     off = torch.tensor(p["off"], **i32)
     wid = torch.tensor([128] * 4 + [64] * 4, **i32)
@@ -237,7 +244,9 @@ def test_module_on_int4_experts(device):
             c1, s1 = ref.quantize(m.w1, group, [128], BF)
             c2, s2 = ref.quantize(m.w2, group, seg, BF)
             r, b = ref.layer(x.reshape(-1, 128), m.router.weight, values(c1, s1, group, [128]),
-                             values(c2, s2, group, seg), m.expert_offsets, 2, True, "relu_squared")
+                             values(c2, s2, group, seg), m.expert_offsets, 2, True, "relu_squared",
+                             ref.int4_terms(spread(s1, group, [128]), BF),
+                             ref.int4_terms(spread(s2, group, seg), BF))
             ref.assert_within(out.reshape(-1, 128), r, b, f"group {group}")
 
 
@@ -246,7 +255,7 @@ def test_grouped_offsets_that_do_not_fit(device):
     from moe_b200.kernels import check_device_status, grouped_gemv_up_int4
 
     p = make(1, 64, [(2, 32)], BF)
-    q1, _, _, _ = quantized(p, "none", 32)
+    q1, *_ = quantized(p, "none", 32)
     i32 = dict(dtype=torch.int32, device=device)
     x = torch.randn(4, 64, device=device, dtype=BF)
     off, wid = torch.tensor([0, 32, 64], **i32), torch.tensor([32, 32], **i32)
@@ -266,7 +275,7 @@ def test_graph_capture_of_products(device):
     from moe_b200.kernels import grouped_gemv_up_int4
 
     p = make(1, 256, [(4, 128)], BF)
-    q1, _, _, _ = quantized(p, "relu_squared", 64)
+    q1, *_ = quantized(p, "relu_squared", 64)
     i32 = dict(dtype=torch.int32, device=device)
     tok, off = torch.tensor([0, 2, 2, 3, 5], **i32), torch.tensor(p["off"], **i32)
     wid = torch.tensor([128] * 4, **i32)
@@ -312,7 +321,7 @@ def test_refusals(device):
     with pytest.raises(TypeError):
         Int4Weight(q.packed, q.scales.float(), 64, 64, 32)
     p = make(2, 64, [(4, 32)], BF)
-    q1, q2, _, _ = quantized(p, "none", 32)
+    q1, q2, *_ = quantized(p, "none", 32)
     off = torch.tensor(p["off"], dtype=torch.int32, device=device)
 
     def layer(a, b, x=p["x"]):

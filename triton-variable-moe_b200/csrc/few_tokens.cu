@@ -12,15 +12,15 @@
 // once from HBM; nothing else is large.  At one token of a small layer the
 // bytes take about a microsecond and the chain launch -> router -> up -> down
 // -> sum is what costs, so there are two launches, no host step and no memset:
-//   up kernel    Every 8-CTA cluster computes the routing for itself (each CTA
-//                an eighth of the hidden size, the sums exchanged over
+//   up kernel    Every cluster of 2 to 8 CTAs computes the routing for itself (each
+//                CTA its part of the hidden size, the sums exchanged over
 //                distributed shared memory): it costs one or two microseconds of
 //                L2 reads and needs no launch and no grid-wide wait of its own.
 //                Then the grid's teams of four warps share the items (expert,
-//                64-column tile, up to 8 NG of its tokens).  With few items each
-//                is cut into slices of the reduction, all in one cluster; the
-//                team that finishes an item's last slice (a counter in shared
-//                memory) adds them in order, applies the activation and writes h.
+//                64-column tile, up to 8 NG of its tokens).  Items that do not make
+//                a whole wave are cut into slices of the reduction, all in one
+//                cluster; the team that finishes an item's last slice (a counter in
+//                shared memory) adds them in order.  Then the activation, and h.
 //   down kernel  The units (slice of an expert's width, 64-column tile of the
 //                hidden size).  The team that finishes a column tile's last unit
 //                (a counter per tile, zeroed by the up kernel) adds the tile's
@@ -36,6 +36,7 @@
 #include <atomic>
 #include <cstdint>
 #include <mutex>
+#include <type_traits>
 
 #include "few_tokens.cuh"
 #include "moe_internal.h"
@@ -50,16 +51,16 @@ using namespace few;
 constexpr int kMaxTokens = 64;    // one 64-bit mask of tokens an expert
 constexpr int kMaxExperts = 256;
 constexpr int kMaxTopK = 32;
-constexpr int kCluster = 8;
+constexpr int kMaxCluster = 8;
 constexpr int kThreads = 512;     // 16 warps: at 128 registers a thread the SM is full
 constexpr int kWarps = kThreads / 32;
 constexpr int kTeam = 4;          // warps that share a unit (they split its reduction)
 constexpr int kTeams = kWarps / kTeam;
 constexpr int kTeamThreads = kTeam * 32;
+constexpr int kMaxLocal = kMaxCluster * kTeams;  // sliced items of a cluster: under a wave
 constexpr int kTile = 64;         // columns of a unit
 constexpr int kRedLd = kTile + 4;
 constexpr int kMaxSlices = 16;
-constexpr int kMaxLocal = 256;    // sliced items of a cluster
 constexpr int kMaxDepth = 4;
 constexpr int kAddTokens = 8;     // up to this many, the down kernel writes the output
 constexpr int kMaxWidth = 32768;  // hidden size and expert width: item counts stay 32-bit
@@ -101,10 +102,11 @@ struct LayerParams {
   int blocks2, groups2;      // block rows and groups of the packed w2
   int down_teams;            // teams of the down kernel's grid
   int smem_work;             // up kernel: bytes before its UpSmem
+  int cluster;               // its CTAs a cluster
   void* out;
   long long ldo;
   // workspace
-  int* plan;                 // [PLAN_WORDS], then kActiveArrays x [E]
+  int* plan;                 // [PLAN_WORDS], then an Active
   int* slot;                 // [T * k] active expert of an assignment (-1: none)
   int* row;                  // [T * k] its expert-sorted row
   float* wgt;                // [T * k]
@@ -174,6 +176,7 @@ struct Unit {
   int row;             // first of them in expert-sorted order
   int e, tile, slice;  // active expert, column tile, slice of the reduction
   int pass;            // first vector within the expert
+  int local;           // up kernel: the cluster's item that this is a slice of, or -1
   __device__ __forceinline__ void set(const Place& w, int vectors) {
     e = static_cast<int>(w.a & 255);
     tile = static_cast<int>(w.a >> 8 & 4095);
@@ -226,14 +229,17 @@ __device__ __forceinline__ bool ring_wait(uint32_t bar, uint32_t parity, volatil
   return true;
 }
 
-// Runs units i, i + stride, ... < total of a team.  Every warp copies its steps
-// (begin + (wr + 4 j) kStep) into its ring as far ahead as it is deep, on into its
-// next units, so the loads go on during the reduction and the output of a unit.
-// place(i) finds a unit, unit(place) describes it, source(unit) gives its vectors, and
-// finish(i, unit) finds the unit's sums in red (see unit_sum) between team barriers.
+// Runs the `total` units of a team.  Every warp copies its steps (begin + (wr + 4 j)
+// kStep) into its ring as far ahead as it is deep, on into its next units, so the
+// loads go on during the reduction and the output of a unit.  place(n) finds the
+// team's n-th unit, unit(place) describes it, source(unit) gives its vectors, and
+// finish(unit) finds the unit's sums in red (see unit_sum) between team barriers.
+template <int N>
+using Int = std::integral_constant<int, N>;
+
 template <typename L, int NG, typename Find, typename MakeUnit, typename MakeSource,
           typename Finish>
-__device__ __forceinline__ void run_units(int i, int stride, int total, const Matrix& m,
+__device__ __forceinline__ void run_units(int total, const Matrix& m,
                                           unsigned char* work, float* red, Common& c, Find place,
                                           MakeUnit unit, MakeSource source, Finish finish) {
   constexpr int kRows = kTeam * L::kStep, TOK = L::template kTokens<NG>;
@@ -244,13 +250,9 @@ __device__ __forceinline__ void run_units(int i, int stride, int total, const Ma
   const uint32_t bars = smem_u32(&c.bar[wid][0]);
   const typename L::Lane at(lane, m.gated);
   using Src = decltype(source(unit(Place())));
-  const int start = i;
-  // the n-th unit of the team
   auto nth = [&](int n, Place& mine) {
-    if (n % 32 == 0) {
-      const int first = start + (n + lane) * stride;
-      if (first < total) mine = place(first);
-    }
+    if (n % 32 == 0 && n + lane < total) mine = place(n + lane);
+    __syncwarp();
     Place q;
     q.a = __shfl_sync(0xffffffffu, mine.a, n % 32);
     q.b = __shfl_sync(0xffffffffu, mine.b, n % 32);
@@ -258,12 +260,11 @@ __device__ __forceinline__ void run_units(int i, int stride, int total, const Ma
   };
 
   int copied = 0, used = 0;  // steps
-  // the copying side: strip of the team's cn-th unit, next step at row ck
-  int cn = -1, ck = 0;
+  // the copying side: the team's cn-th unit, next step at row ck
+  int cn = -1, ck = 0, cend = 0;
   bool more = true;
   Place ahead(0, 0, 0, 0), here(0, 0, 0, 0);
-  Unit cu;
-  cu.strip.end = 0;
+  typename L::Cursor cursor;
   // the multiplying side
   int k = 0, n = -1;
   Unit u;
@@ -273,25 +274,41 @@ __device__ __forceinline__ void run_units(int i, int stride, int total, const Ma
   Src src;
   while (true) {
     while (more && copied - used < D) {
-      if (ck >= cu.strip.end) {
-        ++cn;
-        more = start + cn * stride < total && !c.abort;
+      if (ck >= cend) {
+        more = ++cn < total && !*static_cast<volatile int*>(&c.abort);
         if (more) {
-          cu = nth(cn, ahead);
+          const Unit cu = nth(cn, ahead);
           ck = cu.begin + wr * L::kStep;
+          cend = cu.strip.end;
+          if (ck < cend) cursor.set(m, cu.strip, ck);
         }
       } else {
         const int slot = copied % D;
-        if (lane == 0) L::issue(m, cu.strip, ck, ring + slot * L::kStage, bars + 8 * slot);
+        if (lane == 0) cursor.issue(m, ring + slot * L::kStage, bars + 8 * slot);
         ++copied;
         ck += kRows;
+        cursor.template next<kRows>(m);
       }
     }
     if (k < u.strip.end) {
+      // (the vectors of each half load during the half before)
       const int slot = used % D;
-      v.load(src, u.strip, k, lane);
-      if (used < copied) ring_wait(bars + 8 * slot, (used / D) & 1, &c.abort);
-      L::template step<NG, Src>(acc, at, m, u.strip, k, ring + slot * L::kStage, lane, v);
+      const uint32_t stage = ring + slot * L::kStage;
+      auto step = [&](auto groups, auto parts) {
+        constexpr int G = decltype(groups)::value, P = decltype(parts)::value;
+        v.template load<G, P>(1, src, u.strip.end, k, lane);
+        if (used < copied) ring_wait(bars + 8 * slot, (used / D) & 1, &c.abort);
+        L::template half<G, P, NG, Src>(0, acc, at, m, u.strip.end, k, stage, lane, v);
+        v.template load<G, P>(0, src, u.strip.end, k + kRows, lane);
+        L::template half<G, P, NG, Src>(1, acc, at, m, u.strip.end, k, stage, lane, v);
+      };
+      // only the columns and parts that the unit has
+      if (NG > 1 && u.count > 8)
+        step(Int<NG>(), Int<Src::kParts>());
+      else if (Src::kParts == 2 && u.count > 4)
+        step(Int<1>(), Int<2>());
+      else
+        step(Int<1>(), Int<1>());
       __syncwarp();  // the step has been read by every lane: its place is free
       ++used;
       k += kRows;
@@ -303,15 +320,20 @@ __device__ __forceinline__ void run_units(int i, int stride, int total, const Ma
         team_sync(team);
         if (wr < 2) L::template store<NG, kRedLd, true>(acc, lane, mine);
         team_sync(team);
-        finish(i, u);
+        finish(u);
         team_sync(team);
-        i += stride;
       }
-      if (i >= total) break;
-      u = nth(++n, here);
+      if (++n >= total) break;
+      u = nth(n, here);
       k = u.begin + wr * L::kStep;
       src = source(u);
       v.rows(src, u.count, lane);
+      if (NG > 1 && u.count > 8)
+        v.template load<NG, Src::kParts>(0, src, u.strip.end, k, lane);
+      else if (Src::kParts == 2 && u.count > 4)
+        v.template load<1, 2>(0, src, u.strip.end, k, lane);
+      else
+        v.template load<1, 1>(0, src, u.strip.end, k, lane);
 #pragma unroll
       for (int a = 0; a < 4; ++a)
 #pragma unroll
@@ -528,25 +550,42 @@ __device__ __forceinline__ unsigned order_key(float v) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-// One warp chooses the k experts of a token from its logits (value j of lane l
-// is expert 32 j + l).  Lane s < k gets the s-th expert and its weight.
-__device__ __forceinline__ void choose(const float (&v)[kMaxExperts / 32], int E, int k, int norm,
-                                       int* sel, float* wgt) {
+// One warp chooses the k experts of token t from the cluster's partial logits (value
+// j of lane l is expert 32 j + l) and tells every CTA of the cluster.
+template <int J, typename Smem>
+__device__ __forceinline__ void choose(const LayerParams& p, cg::cluster_group& cluster, float* log,
+                                       int lde, int t, Smem& sm, int* sel_s, float* wgt_s) {
   const int lane = threadIdx.x & 31;
-  unsigned key[kMaxExperts / 32];
+  float v[J];
+  unsigned key[J];
 #pragma unroll
-  for (int j = 0; j < kMaxExperts / 32; ++j) key[j] = 32 * j + lane < E ? order_key(v[j]) : 0u;
+  for (int j = 0; j < J; ++j) v[j] = 0.f;
+  for (int c = 0; c < p.cluster; c += 2) {
+    const float* q0 = cluster.map_shared_rank(log, c) + t * lde;
+    const float* q1 = cluster.map_shared_rank(log, c + 1) + t * lde;
+    float a[J], b[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int e = min(32 * j + lane, p.E - 1);
+      a[j] = q0[e];
+      b[j] = q1[e];
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j) v[j] = v[j] + a[j] + b[j];
+  }
+#pragma unroll
+  for (int j = 0; j < J; ++j) key[j] = 32 * j + lane < p.E ? order_key(v[j]) : 0u;
   float mine = 0.f;
-  int idx = 0;
-  for (int s = 0; s < k; ++s) {
-    unsigned best = 0;
+  int sel = 0;
+  for (int s = 0; s < p.k; ++s) {
+    unsigned best = key[0];
 #pragma unroll
-    for (int j = 0; j < kMaxExperts / 32; ++j) best = max(best, key[j]);
+    for (int j = 1; j < J; ++j) best = max(best, key[j]);
     best = __reduce_max_sync(0xffffffffu, best);
     unsigned at = 0xffffffffu;
     float val = 0.f;
 #pragma unroll
-    for (int j = kMaxExperts / 32 - 1; j >= 0; --j)
+    for (int j = J - 1; j >= 0; --j)
       if (key[j] == best) {
         at = 32 * j + lane;
         val = v[j];
@@ -554,21 +593,29 @@ __device__ __forceinline__ void choose(const float (&v)[kMaxExperts / 32], int E
     const unsigned e = __reduce_min_sync(0xffffffffu, at);  // ties: the lower index
     val = __shfl_sync(0xffffffffu, val, e & 31);
 #pragma unroll
-    for (int j = 0; j < kMaxExperts / 32; ++j)
+    for (int j = 0; j < J; ++j)
       if (e == 32u * j + lane) key[j] = 0u;
     if (lane == s) {
       mine = val;
-      idx = static_cast<int>(e);
+      sel = static_cast<int>(e);
     }
   }
-  float w = 1.f / (1.f + expf(-mine));
-  if (norm) {
-    float sum = 0.f;  // in rank order
-    for (int s = 0; s < k; ++s) sum += __shfl_sync(0xffffffffu, w, s);
+  float w = lane < p.k ? 1.f / (1.f + expf(-mine)) : 0.f;
+  if (p.norm) {
+    float sum = w;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     w = w / (sum + 1e-20f);
   }
-  *sel = idx;
-  *wgt = w;
+  if (lane < p.k) {
+    for (int c = 0; c < p.cluster; ++c) {
+      cluster.map_shared_rank(sel_s, c)[t * p.k + lane] = sel;
+      cluster.map_shared_rank(wgt_s, c)[t * p.k + lane] = w;
+      // (32-bit words: 64-bit atomics of several CTAs on one shared word lose bits)
+      atomicOr(reinterpret_cast<unsigned*>(cluster.map_shared_rank(sm.mask, c) + sel) + (t >> 5),
+               1u << (t & 31));
+    }
+  }
 }
 
 // ---- the layer's active experts ----------------------------------------------
@@ -580,69 +627,97 @@ struct alignas(16) UpSmem {
   int slot[kMaxExperts];  // active expert of an expert (-1: none)
   int base[kMaxExperts];  // first expert-sorted row of an expert
   int ticket[kMaxLocal];  // slices done of the cluster's items (rank 0's is used)
+  int kb[kMaxExperts];    // packed w2 (otherwise 0): first block row, first group,
+  int sg[kMaxExperts];
+  int fits[kMaxExperts];  // and whether the expert lies in it
 };
 static_assert(sizeof(UpSmem) % 16 == 0, "16-byte vectors follow");
+
+// Whether an expert's offsets [a, b) fit the matrices, and its width.
+__device__ __forceinline__ bool expert_width(int a, int b, int total, int max_width, int act,
+                                             int* width) {
+  const int gated = act == ACT_SWIGLU ? 1 : 0;  // log2
+  const int step = (16 << gated) - 1;
+  const bool ok = a >= 0 && b >= a && b <= total && ((a | b) & step) == 0 &&
+                  (b - a) >> gated <= max_width;
+  *width = ok ? (b - a) >> gated : 0;
+  return ok;
+}
 
 // One warp: from the token masks and the offsets, the experts that have rows and
 // columns, and their (pass, tile) items.  Offsets that leave the matrices, or are
 // not in steps of 16, empty the expert and set the status word.
 template <int TOK>
 __device__ __forceinline__ void find_active(const LayerParams& p, UpSmem& s) {
-  const int lane = threadIdx.x & 31;
-  const int gated = p.act == ACT_SWIGLU ? 2 : 1;
-  int active = 0, base = 0, item = 0, kb = 0, sg = 0;
+  const int lane = threadIdx.x & 31, outputs = p.act == ACT_SWIGLU ? 5 : 6;  // log2
+  static_assert((kMaxTokens / 8 * kMaxTopK + kMaxExperts) * (kMaxWidth / 32) <= 1 << 20,
+                "20 bits of items, 12 of rows");
+  unsigned sums = 0;
+  int active = 0;
 #pragma unroll 1
   for (int e0 = 0; e0 < p.E; e0 += 32) {
     const int e = e0 + lane;
     int n = 0, a = 0, w = 0;
     bool ok = true;
+    unsigned long long mask = 0;
     if (e < p.E) {
-      n = __popcll(s.mask[e]);
+      mask = s.mask[e];
+      n = __popcll(mask);
       a = s.off[e];
-      const int b = s.off[e + 1];
-      ok = a >= 0 && b >= a && b <= p.total && a % (16 * gated) == 0 &&
-           (b - a) % (16 * gated) == 0 && (b - a) / gated <= p.max_width;
-      w = ok ? (b - a) / gated : 0;
-    }
-    int total;
-    const int my_base = base + warp_scan(n, &total);
-    base += total;
-    int my_kb = 0, my_sg = 0;
-    if (p.shift) {
-      const int blocks = ceil_div(w, 64), groups = group_count(w, p.shift);
-      my_kb = kb + warp_scan(blocks, &total);
-      kb += total;
-      my_sg = sg + warp_scan(groups, &total);
-      sg += total;
-      // a packed w2 quantised for other offsets
-      if (my_kb + blocks > p.blocks2 || my_sg + groups > p.groups2) ok = false;
+      ok = expert_width(a, s.off[e + 1], p.total, p.max_width, p.act, &w) && s.fits[e];
     }
     if (!ok && p.status && blockIdx.x == 0) *p.status = kStatusBadArg;
     const bool here = ok && n > 0 && w > 0;
-    const int my_items = here ? ceil_div(n, TOK) * ceil_div(w, tile_outputs(p.act)) : 0;
-    const int my_item = item + warp_scan(my_items, &total);
-    item += total;
+    const int items = here ? ceil_div(n, TOK) * ((w + (1 << outputs) - 1) >> outputs) : 0;
+    int total;
+    const unsigned mine =
+        sums + static_cast<unsigned>(warp_scan(static_cast<int>(items | static_cast<unsigned>(n) << 20), &total));
+    sums += static_cast<unsigned>(total);
     const unsigned who = __ballot_sync(0xffffffffu, here);
     const int at = active + __popc(who & ((1u << lane) - 1));
     active += __popc(who);
+    const int base = static_cast<int>(mine >> 20);
     if (e < p.E) {
       s.slot[e] = here ? at : -1;
-      s.base[e] = my_base;
+      s.base[e] = base;
     }
     if (here) {
       s.c.act.n[at] = n;
-      s.c.act.base[at] = my_base;
+      s.c.act.base[at] = base;
       s.c.act.first[at] = a;
       s.c.act.width[at] = w;
-      s.c.act.kb[at] = my_kb;
-      s.c.act.sg[at] = my_sg;
-      s.c.act.item[at] = my_item;
-      s.act_mask[at] = s.mask[e];
+      s.c.act.kb[at] = s.kb[e];
+      s.c.act.sg[at] = s.sg[e];
+      s.c.act.item[at] = static_cast<int>(mine & 0xfffffu);
+      s.act_mask[at] = mask;
     }
   }
   if (lane == 0) {
     s.c.plan[0] = active;
-    s.c.plan[1] = item;
+    s.c.plan[1] = static_cast<int>(sums & 0xfffffu);
+  }
+}
+
+// One warp, while others route: where each expert's rows of a packed w2 start, and
+// whether they lie in it (not when it was quantised for other offsets).
+__device__ __forceinline__ void find_packed(const LayerParams& p, UpSmem& s) {
+  const int lane = threadIdx.x & 31;
+  int kb = 0, sg = 0;
+#pragma unroll 1
+  for (int e0 = 0; e0 < p.E; e0 += 32) {
+    const int e = e0 + lane;
+    int w = 0, total;
+    if (e < p.E) expert_width(s.off[e], s.off[e + 1], p.total, p.max_width, p.act, &w);
+    const int blocks = ceil_div(w, 64), groups = group_count(w, p.shift);
+    const int my_kb = kb + warp_scan(blocks, &total);
+    kb += total;
+    const int my_sg = sg + warp_scan(groups, &total);
+    sg += total;
+    if (e < p.E) {
+      s.kb[e] = my_kb;
+      s.sg[e] = my_sg;
+      s.fits[e] = my_kb + blocks <= p.blocks2 && my_sg + groups <= p.groups2;
+    }
   }
 }
 
@@ -667,7 +742,7 @@ __device__ __forceinline__ void plan_down(const LayerParams& p, const Active& ac
     if (j < active) n = ceil_div(act.n[j], TOK) * ceil_div(ceil_div(act.width[j], ROUND), len);
     const int before = items + warp_scan(n, &total);
     items += total;
-    if (j < active) p.plan[PLAN_WORDS + 6 * p.E + j] = before;
+    if (j < active) p.plan[PLAN_WORDS + 6 * kMaxExperts + j] = before;
   }
   if (lane == 0) {
     p.plan[PLAN_ACTIVE] = active;
@@ -698,65 +773,50 @@ __global__ void __launch_bounds__(kThreads, 1)
   // every block of this grid runs by the time the last one gets here
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   for (int e = tid; e <= p.E; e += kThreads) s.off[e] = p.off[e];
-  for (int e = tid; e < p.E; e += kThreads) s.mask[e] = 0;
+  for (int e = tid; e < p.E; e += kThreads) {
+    s.mask[e] = 0;
+    s.kb[e] = s.sg[e] = 0;
+    s.fits[e] = 1;
+  }
   for (int i = tid; i < kMaxLocal; i += kThreads) s.ticket[i] = 0;
   ring_init<L::template kDepth<NG>>(s.c);
 
-  // routing: an eighth of the hidden size, then tokens rank, rank + 8, ...
-  const int per = ceil_div(ceil_div(p.H, 32), kCluster) * 32;
+  // routing: this CTA's part of the hidden size, then tokens rank, rank + cluster, ...
+  const int per = ceil_div(ceil_div(p.H, 32), p.cluster) * 32;
   partial_logits<T>(p, min(rank * per, p.H), min((rank + 1) * per, p.H), part, log, lde);
   cluster.sync();
-  for (int t = rank + kCluster * wid; t < p.T; t += kCluster * kWarps) {
-    float v[kMaxExperts / 32];
-#pragma unroll
-    for (int j = 0; j < kMaxExperts / 32; ++j) {
-      v[j] = 0.f;
-      if (32 * j < p.E) {
-        const int e = min(32 * j + lane, p.E - 1);
-        float q[kCluster];
-#pragma unroll
-        for (int c = 0; c < kCluster; ++c) q[c] = cluster.map_shared_rank(log, c)[t * lde + e];
-#pragma unroll
-        for (int c = 0; c < kCluster; ++c) v[j] += q[c];
-      }
-    }
-    int sel;
-    float wgt;
-    choose(v, p.E, p.k, p.norm, &sel, &wgt);
-    if (lane < p.k) {
-#pragma unroll
-      for (int c = 0; c < kCluster; ++c) {
-        cluster.map_shared_rank(sel_s, c)[t * p.k + lane] = sel;
-        cluster.map_shared_rank(wgt_s, c)[t * p.k + lane] = wgt;
-        // (32-bit words: 64-bit atomics of several CTAs on one shared word lose bits)
-        atomicOr(reinterpret_cast<unsigned*>(cluster.map_shared_rank(s.mask, c) + sel) + (t >> 5),
-                 1u << (t & 31));
-      }
-    }
+  if (p.shift && wid == kWarps - 1) find_packed(p, s);
+  for (int t = rank + p.cluster * wid; t < p.T; t += p.cluster * kWarps) {
+    if (p.E <= 32)
+      choose<1>(p, cluster, log, lde, t, s, sel_s, wgt_s);
+    else if (p.E <= 64)
+      choose<2>(p, cluster, log, lde, t, s, sel_s, wgt_s);
+    else if (p.E <= 128)
+      choose<4>(p, cluster, log, lde, t, s, sel_s, wgt_s);
+    else
+      choose<8>(p, cluster, log, lde, t, s, sel_s, wgt_s);
   }
   cluster.sync();
 
-  const int clusters = gridDim.x / kCluster, teams = gridDim.x * kTeams;
+  const int clusters = gridDim.x / p.cluster, teams = gridDim.x * kTeams;
   const int rounds = ceil_div(p.H, kRound);
   if (wid == 0) {
     find_active<TOK>(p, s);
     __syncwarp();
-    // whole items over all teams, or slices of a cluster's items over its teams
-    const int U = s.c.plan[1], local = ceil_div(U, clusters);
-    const long long whole = static_cast<long long>(ceil_div(U, teams)) * (4 * rounds + 2);
-    int len = rounds;
-    if (local <= kMaxLocal && rounds > 1) {
-      const int sliced = min(p.max_slices, rounds);
-      const int cut = lane + 2;  // slices
-      long long cost = 0x7fffffffll;
-      if (cut <= sliced)
-        cost = static_cast<long long>(ceil_div(local * cut, kCluster * kTeams)) *
-                   (4 * ceil_div(rounds, cut) + 5) + 3;
-      const unsigned best = __reduce_min_sync(0xffffffffu, static_cast<unsigned>(cost));
-      const int at = __ffs(__ballot_sync(0xffffffffu, static_cast<unsigned>(cost) == best)) - 1;
-      if (static_cast<long long>(best) < whole) len = ceil_div(rounds, at + 2);
-    }
-    if (lane == 0) s.c.plan[2] = len;
+    // Whole items, a wave of them over all teams at a time; the rest whole too, or in
+    // slices of a cluster's items over its teams.  Lane l weighs l + 1 slices, in
+    // quarter rounds: a unit's own cost is half a round, a slice's with the joining
+    // another three quarters.
+    const int rest = s.c.plan[1] % teams;
+    const int local = ceil_div(rest, clusters), cut = lane + 1;
+    int cost = 0x7fffffff;
+    if (cut == 1)
+      cost = 4 * rounds + 2;
+    else if (cut <= min(p.max_slices, rounds))
+      cost = ceil_div(local * cut, p.cluster * kTeams) * (4 * ceil_div(rounds, cut) + 5) + 3;
+    const int best = __reduce_min_sync(0xffffffffu, cost);
+    const int at = __ffs(__ballot_sync(0xffffffffu, cost == best));
+    if (lane == 0) s.c.plan[2] = ceil_div(rounds, at);
   }
   fence_proxy_async_smem();  // the routing's use of the rings, before copies into them
   __syncthreads();
@@ -773,45 +833,56 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = tid; i < ceil_div(p.H, kTile); i += kThreads) p.ticket[i] = 0;
     for (int j = tid; j < active; j += kThreads) {
       int* d = p.plan + PLAN_WORDS + j;
-      d[0 * p.E] = s.c.act.n[j];
-      d[1 * p.E] = s.c.act.base[j];
-      d[2 * p.E] = s.c.act.first[j];
-      d[3 * p.E] = s.c.act.width[j];
-      d[4 * p.E] = s.c.act.kb[j];
-      d[5 * p.E] = s.c.act.sg[j];
+      d[0 * kMaxExperts] = s.c.act.n[j];
+      d[1 * kMaxExperts] = s.c.act.base[j];
+      d[2 * kMaxExperts] = s.c.act.first[j];
+      d[3 * kMaxExperts] = s.c.act.width[j];
+      d[4 * kMaxExperts] = s.c.act.kb[j];
+      d[5 * kMaxExperts] = s.c.act.sg[j];
     }
     if (wid == kWarps - 1) plan_down<TOK, kRound>(p, s.c.act, active);
   }
 
-  // item of unit i: the whole grid's, or (sliced) every `clusters`-th item for this
-  // cluster, slices of one item on different CTAs
+  // the team's units: its items of the whole waves, then its slices of the cluster's
+  // items (every `clusters`-th of the rest; neighbouring slices on different CTAs)
   const int team = wid / kTeam, tt = tid % kTeamThreads;
-  const int mine = blockIdx.x / kCluster;
-  int start, stride, total;
+  const int me = blockIdx.x * kTeams + team, waves = U / teams, rest = U % teams;
+  const int mine = blockIdx.x / p.cluster, start = team * p.cluster + rank;
+  const int group = p.cluster * kTeams;
+  int total = waves;
   if (slices == 1) {
-    start = blockIdx.x * kTeams + team;
-    stride = teams;
-    total = U;
+    total += me < rest;
   } else {
-    start = team * kCluster + rank;
-    stride = kCluster * kTeams;
-    total = U > mine ? ceil_div(U - mine, clusters) * slices : 0;
+    const int units = rest > mine ? ceil_div(rest - mine, clusters) * slices : 0;
+    if (units > start) total += ceil_div(units - start, group);
   }
   const Active& act = s.c.act;
-  auto place = [&](int i) {
-    const int item = slices == 1 ? i : mine + clusters * (i / slices);
+  constexpr unsigned kSliced = 1u << 31;  // of Place::b; then the cluster's item << 8
+  auto place = [&](int n) {
+    int item = n * teams + me, sl = 0;
+    unsigned flags = 0;
+    if (n >= waves && slices > 1) {
+      const int i = start + (n - waves) * group, local = i / slices;
+      sl = i - local * slices;
+      item = waves * teams + mine + clusters * local;
+      flags = kSliced | static_cast<unsigned>(local) << 8;
+    }
     const int e = find_item(act.item, active, item), r = item - act.item[e];
-    const int tiles = ceil_div(act.width[e], tile_outputs(p.act));
-    return Place(e, r % tiles, slices == 1 ? 0 : i % slices, r / tiles);
+    const int tiles = ceil_div(act.width[e], tile_outputs(p.act)), pass = r / tiles;
+    Place w(e, r - pass * tiles, sl, pass);
+    w.b |= flags;
+    return w;
   };
   auto unit = [&](const Place& w) {
     Unit u;
     u.set(w, TOK);
+    u.pass = static_cast<int>(w.b & 255) * TOK;
+    u.local = w.b & kSliced ? static_cast<int>(w.b >> 8 & 255) : -1;
     const int width = act.width[u.e];
     u.count = min(act.n[u.e] - u.pass, TOK);
     u.row = act.base[u.e] + u.pass;
     u.begin = u.slice * q * kRound;
-    u.strip.end = min(p.H, u.begin + q * kRound);
+    u.strip.end = u.local < 0 ? p.H : min(p.H, u.begin + q * kRound);
     up_strip(u.strip, act.first[u.e], width, p.act, u.tile, p.H, p.shift);
     return u;
   };
@@ -838,8 +909,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   const int vecs = tile_outputs(p.act) / 4;
   const Matrix m{&p.map1, p.w1, p.s1, p.total, p.shift, p.act == ACT_SWIGLU};
-  run_units<L, NG>(start, stride, total, m, work, red, s.c, place, unit, source, [&](int i, const Unit& u) {
-    if (slices == 1) {
+  run_units<L, NG>(total, m, work, red, s.c, place, unit, source, [&](const Unit& u) {
+    if (u.local < 0) {
       for (int j = tt; j < u.count * vecs; j += kTeamThreads)
         emit(u, j / vecs, 4 * (j % vecs),
              [&](int tok, int c) { return unit_sum<TOK>(red, tok, c); });
@@ -856,7 +927,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tt == 0) {
       __threadfence();  // the team's sums, before the count
       s.c.last[team] =
-          atomicAdd(cluster.map_shared_rank(s.ticket, 0) + i / slices, 1) == slices - 1;
+          atomicAdd(cluster.map_shared_rank(s.ticket, 0) + u.local, 1) == slices - 1;
       __threadfence();  // and the other teams' sums, after it
     }
     team_sync(team);
@@ -895,9 +966,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (tid < 3) s.plan[tid] = p.plan[tid];
-  for (int i = tid; i < kActiveArrays * p.E; i += kThreads) {
-    const int j = i / p.E;
-    (&s.act.n[0])[j * kMaxExperts + i - j * p.E] = p.plan[PLAN_WORDS + i];
+  static_assert(sizeof(Active) == 4 * kActiveArrays * kMaxExperts && kThreads == 2 * kMaxExperts,
+                "two arrays a pass");
+  if (tid % kMaxExperts < p.E) {
+#pragma unroll
+    for (int i = tid; i < kActiveArrays * kMaxExperts; i += kThreads)
+      reinterpret_cast<int*>(&s.act)[i] = p.plan[PLAN_WORDS + i];
   }
   for (int a = tid; a < A; a += kThreads) {
     slot_s[a] = p.slot[a];
@@ -924,7 +998,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Eight column tiles (1 KB of a row) at a time: neighbouring teams read
   // neighbouring pieces, and the tiles finish one block after another, so that
   // only the last block's final sums have nothing to overlap.
-  auto place = [&](int i) {
+  const int me = blockIdx.x * kTeams + team, teams = gridDim.x * kTeams;
+  auto place = [&](int n) {
+    const int i = me + n * teams;
     const int block = i / (8 * items), r = i - block * 8 * items;
     const int nb = min(8, tiles - 8 * block), it = r / nb;
     const int e = find_item(act.item, active, it), j = it - act.item[e];
@@ -952,17 +1028,23 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int share = p.T == 1 ? 8 : p.T == 2 ? 4 : p.T <= 4 ? 2 : 1;
   const Matrix m{&p.map2, p.w2, p.s2, p.H, p.shift, 0};
   run_units<L, NG>(
-      blockIdx.x * kTeams + team, gridDim.x * kTeams, items * tiles, m, work, red, s, place, unit,
-      source,
-      [&](int, const Unit& u) {
+      items * tiles > me ? ceil_div(items * tiles - me, teams) : 0, m, work, red, s, place, unit,
+      source, [&](const Unit& u) {
         const int cols = p.H - u.tile * kTile;
         float* y = p.y + u.tile * kTile;
+        // (with the remainders' columns, see HiddenSource)
+        const bool split = sizeof(T) == 2 && u.count <= 4;
+        auto down_sum = [&](int tok, int c) {
+          float4 v = unit_sum<TOK>(red, tok, c);
+          if (split) add4(v, unit_sum<TOK>(red, tok + 4, c));
+          return v;
+        };
         for (int j = tt; j < u.count * (kTile / 4); j += kTeamThreads) {
           const int tok = j / (kTile / 4), c = 4 * (j % (kTile / 4));
           if (c < cols)
             *reinterpret_cast<float4*>(y + u.slice * slice +
                                        static_cast<long long>(u.row + tok) * p.H + c) =
-                unit_sum<TOK>(red, tok, c);
+                down_sum(tok, c);
         }
         if (!add) return;
         team_sync(team);
@@ -1040,13 +1122,14 @@ __global__ void __launch_bounds__(kSumThreads) few_sum_kernel(const __grid_const
   __shared__ float wgt_s[kMaxTopK];
   const int t = blockIdx.y, tid = threadIdx.x;
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid < p.k) {
     const int a = t * p.k + tid, slot = p.slot[a];
     row_s[tid] = p.row[a];
     wgt_s[tid] = p.wgt[a];
     parts_s[tid] = 0;
     if (slot >= 0)
-      parts_s[tid] = ceil_div(ceil_div(p.plan[PLAN_WORDS + 3 * p.E + slot], kRound),
+      parts_s[tid] = ceil_div(ceil_div(p.plan[PLAN_WORDS + 3 * kMaxExperts + slot], kRound),
                               p.plan[PLAN_LENGTH]);
   }
   __syncthreads();
@@ -1207,7 +1290,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 
   const int team = wid / kTeam, tt = tid % kTeamThreads;
-  auto place = [&](int i) {
+  const int me = blockIdx.x * kTeams + team, units = s.c.plan[1];
+  auto place = [&](int n) {
+    const int i = me + n * teams;
     const int e = find_item(act.item, active, i), r = i - act.item[e], width = act.width[e];
     const int tiles = p.down ? ceil_div(p.H, kTile) : ceil_div(width, outputs);
     const int ns = ceil_div(ceil_div(p.down ? width : p.H, kRound), q);
@@ -1232,8 +1317,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   float* red = reinterpret_cast<float*>(work + kRingBytes<L, NG>) + team * kRedFloats<L, NG>;
   const Matrix m{nullptr, p.w, p.s, p.down ? p.H : p.total, p.shift, p.act == ACT_SWIGLU};
-  run_units<L, NG>(blockIdx.x * kTeams + team, teams, s.c.plan[1], m, work, red, s.c, place, unit, source,
-                   [&](int, const Unit& u) {
+  run_units<L, NG>(units > me ? ceil_div(units - me, teams) : 0, m, work, red, s.c, place, unit,
+                   source, [&](const Unit& u) {
                      float* dst = p.part +
                                   (static_cast<long long>(u.slice) * p.rows + u.row) * p.ldp +
                                   u.tile * kTile;
@@ -1257,6 +1342,7 @@ __global__ void __launch_bounds__(kThreads)
   constexpr int kRound = kTeam * L::kStep;
   __shared__ int n_s[kMaxExperts], base_s[kMaxExperts], width_s[kMaxExperts], head[2];
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   for (int j = threadIdx.x; j < p.E; j += kThreads) {
     n_s[j] = p.plan[PLAN_WORDS + j];
     base_s[j] = p.plan[PLAN_WORDS + p.E + j];
@@ -1317,7 +1403,7 @@ int slice_limit(long long floats) {
   return static_cast<int>(n < 1 ? 1 : n > kMaxSlices ? kMaxSlices : n);
 }
 
-LayerPlan layer_plan(int T, int H, int E, int k, int max_width, int act) {
+LayerPlan layer_plan(int T, int H, int k, int max_width, int act) {
   LayerPlan p{};
   const long long A = static_cast<long long>(T) * k;
   p.ldu = padded_columns(max_width, act);
@@ -1328,7 +1414,7 @@ LayerPlan layer_plan(int T, int H, int E, int k, int max_width, int act) {
     at = align_up(at + bytes, 128);
     return here;
   };
-  p.plan = take(4ll * (PLAN_WORDS + kActiveArrays * E));
+  p.plan = take(4ll * PLAN_WORDS + static_cast<long long>(sizeof(Active)));
   p.slot = take(4 * A);
   p.row = take(4 * A);
   p.wgt = take(4 * A);
@@ -1358,26 +1444,33 @@ bool allow_smem(K* kernel, std::atomic<unsigned long long>& done, int device) {
   return true;
 }
 
-// 8-CTA clusters that are resident together at one CTA an SM.
+// CTAs of clusters of `size` that are resident together at one CTA an SM.
 template <typename K>
-int resident_clusters(K* kernel, std::atomic<int>* known, int device) {
-  int n = known[device].load(std::memory_order_acquire);
+int resident_ctas(K* kernel, std::atomic<int>* known, int size) {
+  int n = known->load(std::memory_order_acquire);
   if (n > 0) return n;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kCluster;
+  attr[0].val.clusterDim.x = size;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(num_sms() / kCluster * kCluster));
+  cfg.gridDim = dim3(static_cast<unsigned>(num_sms() / size * size));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kSmemMax;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) return -1;
-  if (n > num_sms() / kCluster) n = num_sms() / kCluster;
-  known[device].store(n, std::memory_order_release);
-  return n;
+  if (n > num_sms() / size) n = num_sms() / size;
+  known->store(n * size, std::memory_order_release);
+  return n * size;
+}
+
+// CTAs a cluster of the up kernel.  Every cluster reads the whole router weight, so
+// larger clusters read less of it; but 8 CTAs fit together on only 120 of 148 SMs
+// (4: 132, 2: all).
+int cluster_size(long long router_bytes) {
+  return router_bytes <= (256 << 10) ? 2 : router_bytes <= (512 << 10) ? 4 : 8;
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_tiled() {
@@ -1418,7 +1511,7 @@ bool weight_map(CUtensorMap* map, const void* w, int dtype, long long rows, long
 template <typename L, int NG>
 int launch_layer(LayerParams& p, cudaStream_t st) {
   static std::atomic<unsigned long long> up_ok{0}, down_ok{0};
-  static std::atomic<int> clusters[64];
+  static std::atomic<int> resident[64][kMaxCluster + 1];
   const int dev = current_device();
   if (dev < 0) return kStatusCuda;
   auto* up = few_up_kernel<L, NG>;
@@ -1431,25 +1524,27 @@ int launch_layer(LayerParams& p, cudaStream_t st) {
   const size_t up_smem = p.smem_work + sizeof(UpSmem) + 8 * A;
   const size_t down_smem = work + sizeof(Common) + 12 * A;
   if (up_smem > kSmemMax || down_smem > kSmemMax) return kStatusUnsupported;
-  const int n = resident_clusters(up, clusters, dev), sms = num_sms();
+  p.cluster = cluster_size(static_cast<long long>(p.E) * p.H * sizeof(typename L::Elem));
+  const int n = resident_ctas(up, &resident[dev][p.cluster], p.cluster), sms = num_sms();
   if (n < 1) return kStatusCuda;
   p.down_teams = sms * kTeams;
 
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kCluster;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(n * kCluster));
+  cfg.gridDim = dim3(static_cast<unsigned>(n));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = up_smem;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   if (cudaLaunchKernelEx(&cfg, up, p) != cudaSuccess) return kStatusCuda;
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs = 1;
   cfg.gridDim = dim3(static_cast<unsigned>(sms));
   cfg.dynamicSmemBytes = down_smem;
   if (cudaLaunchKernelEx(&cfg, down, p) != cudaSuccess) return kStatusCuda;
@@ -1484,14 +1579,14 @@ int launch_group(const GroupParams& p, cudaStream_t st) {
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kWorkBytes<L, NG> + sizeof(GroupSmem);
   cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) return kStatusCuda;
   const long long vecs = p.rows * ((p.down ? p.H : p.max_width) / 4);
   long long blocks = (vecs + kThreads - 1) / kThreads;
   if (blocks > 4ll * num_sms()) blocks = 4ll * num_sms();
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
   cfg.dynamicSmemBytes = 0;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, sum, p) != cudaSuccess) return kStatusCuda;
   return cudaPeekAtLastError() == cudaSuccess ? kStatusOk : kStatusCuda;
 }
@@ -1514,7 +1609,7 @@ static_assert(kGroupHeader % 128 == 0, "partial sums follow");
 long long few_tokens_workspace(long long T, long long H, int E, int k, long long max_width,
                                int act) {
   if (!layer_sizes_ok(T, H, E, k, max_width, act)) return -1;
-  return layer_plan(static_cast<int>(T), static_cast<int>(H), E, k, static_cast<int>(max_width), act)
+  return layer_plan(static_cast<int>(T), static_cast<int>(H), k, static_cast<int>(max_width), act)
       .bytes;
 }
 
@@ -1533,7 +1628,7 @@ int few_tokens(const void* x, long long T, long long ldx, long long H, const voi
       (shift && (!s1 || !s2 || !aligned16(s1) || !aligned16(s2) || blocks2 < 0 || groups2 < 0 ||
                  blocks2 > (1 << 30) || groups2 > (1 << 30))))
     return kStatusBadArg;
-  const LayerPlan plan = layer_plan(static_cast<int>(T), static_cast<int>(H), E, k,
+  const LayerPlan plan = layer_plan(static_cast<int>(T), static_cast<int>(H), k,
                                     static_cast<int>(max_width), act);
   if (ws_bytes < plan.bytes || !aligned16(ws)) return kStatusBadArg;
   unsigned char* b = static_cast<unsigned char*>(ws);

@@ -53,6 +53,11 @@ __device__ __forceinline__ float from_f<float>(float v) {
 }
 
 template <typename T>
+constexpr bool kIsBf16 = false;
+template <>
+constexpr bool kIsBf16<__nv_bfloat16> = true;
+
+template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);
 template <>
 __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
@@ -75,27 +80,27 @@ __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
   return __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
 
-// d += a (16 x 16) * b (16 x 8), fp32 accumulation.
+// d = a (16 x 16) * b (16 x 8) + c, fp32 accumulation.
 template <typename T>
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                    uint32_t b1);
-template <>
-__device__ __forceinline__ void mma<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4],
-                                                   uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-      "{%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+                                    uint32_t b1, const float (&c)[4]) {
+  if constexpr (kIsBf16<T>)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]),
+          "f"(c[2]), "f"(c[3]));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]),
+          "f"(c[2]), "f"(c[3]));
 }
-template <>
-__device__ __forceinline__ void mma<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                            uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-      "{%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+template <typename T>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                    uint32_t b1) {
+  mma<T>(d, a, b0, b1, d);
 }
 
 // 16 bytes that are read once: past L1.
@@ -136,6 +141,11 @@ __device__ __forceinline__ uint4 lds16(uint32_t a) {
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "r"(a)
                : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
   return v;
 }
 __device__ __forceinline__ uint32_t lds4(uint32_t a) {
@@ -213,6 +223,10 @@ struct RowSource {
 // rounded to the storage type, and the second multiply is free beside the weight
 // loads.  In fp16 a value above 65504 is infinite, as it is in the layer's
 // forward, which stores it.  A row: [values | remainders].
+//
+// A unit of up to 4 vectors holds their remainders in the instruction's other four
+// columns (one multiply for both; `split`), and the sums of columns j and j + 4 are
+// added at the end.
 template <typename T>
 struct HiddenSource {
   static constexpr int kParts = 2;
@@ -298,54 +312,65 @@ struct Dense16 {
       }
     }
   };
-  static __device__ __forceinline__ void issue(const Matrix& m, const Strip& s, int k, uint32_t stage,
-                                               uint32_t bar) {
-    expect_bytes(bar, kStage);
-    box_load(stage, m.map, s.col, s.row + k, bar);
-    if (m.gated) box_load(stage + 2048, m.map, s.col + s.jump, s.row + k, bar);
-  }
+  // Where the copies of a strip are: the step at row k, then every `rows` further.
+  struct Cursor {
+    int col, jump, row;
+    __device__ __forceinline__ void set(const Matrix&, const Strip& s, int k) {
+      col = s.col;
+      jump = s.jump;
+      row = s.row + k;
+    }
+    template <int ROWS>
+    __device__ __forceinline__ void next(const Matrix&) {
+      row += ROWS;
+    }
+    __device__ __forceinline__ void issue(const Matrix& m, uint32_t stage, uint32_t bar) const {
+      expect_bytes(bar, kStage);
+      box_load(stage, m.map, col, row, bar);
+      if (m.gated) box_load(stage + 2048, m.map, col + jump, row, bar);
+    }
+  };
+  // The vectors' elements of half h (16 rows) of a step.
   template <int NG, typename Src>
   struct Vectors {
     const T* r[NG];
-    uint2 b[NG][Src::kParts][2];
+    uint2 b[2][NG][Src::kParts];
     __device__ __forceinline__ void rows(const Src& src, int count, int lane) {
       const int g = lane >> 2;
 #pragma unroll
       for (int n = 0; n < NG; ++n)
         r[n] = 8 * n + g < count ? src.row(8 * n + g) + 4 * (lane & 3) : nullptr;
+      if (Src::kParts == 2 && count <= 4)
+        r[0] = (g & 3) < count ? src.row(g & 3) + (g & 4 ? src.half : 0) + 4 * (lane & 3) : nullptr;
     }
-    __device__ __forceinline__ void load(const Src& src, const Strip& s, int k, int lane) {
+    template <int G, int P>
+    __device__ __forceinline__ void load(int h, const Src& src, int end, int k, int lane) {
 #pragma unroll
-      for (int n = 0; n < NG; ++n)
+      for (int n = 0; n < G; ++n)
 #pragma unroll
-        for (int p = 0; p < Src::kParts; ++p)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint2 v = make_uint2(0u, 0u);
-            if (r[n] && k + 16 * h < s.end)
-              v = *reinterpret_cast<const uint2*>(r[n] + p * src.half + k + 16 * h);
-            b[n][p][h] = (lane & 2) ? make_uint2(v.y, v.x) : v;
-          }
+        for (int p = 0; p < P; ++p) {
+          uint2 v = make_uint2(0u, 0u);
+          if (r[n] && k + 16 * h < end)
+            v = *reinterpret_cast<const uint2*>(r[n] + p * src.half + k + 16 * h);
+          b[h][n][p] = (lane & 2) ? make_uint2(v.y, v.x) : v;
+        }
     }
   };
-  template <int NG, typename Src>
-  static __device__ __forceinline__ void step(float (&acc)[4][NG][4], const Lane& l,
-                                              const Matrix&, const Strip& s, int k, uint32_t stage,
-                                              int, const Vectors<NG, Src>& v) {
+  // One half of a step for the first G groups of vectors and P of their parts.
+  template <int G, int P, int NG, typename Src>
+  static __device__ __forceinline__ void half(int h, float (&acc)[4][NG][4], const Lane& l,
+                                              const Matrix&, int end, int k, uint32_t stage, int,
+                                              const Vectors<NG, Src>& v) {
+    if (h && k + 16 >= end) return;  // rows beyond are another expert's
+    uint32_t a[4][4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (h && k + 16 >= s.end) break;  // rows beyond are another expert's
+    for (int i = 0; i < 4; ++i) ldsm_trans(a[i], stage + h * l.half + l.off[i]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t a[4];
-        ldsm_trans(a, stage + h * l.half + l.off[i]);
+    for (int p = 0; p < P; ++p)
 #pragma unroll
-        for (int n = 0; n < NG; ++n)
+      for (int n = 0; n < G; ++n)
 #pragma unroll
-          for (int p = 0; p < Src::kParts; ++p)
-            mma<T>(acc[i][n], a, v.b[n][p][h].x, v.b[n][p][h].y);
-      }
-    }
+        for (int i = 0; i < 4; ++i) mma<T>(acc[i][n], a[i], v.b[h][n][p].x, v.b[h][n][p].y);
   }
   // The lane's sums to (ADD: added to) red[token][64 columns], row stride LD.
   template <int NG, int LD, bool ADD>
@@ -365,11 +390,21 @@ struct Dense16 {
 
 // 4-bit weights in the packed layout (see int4.cu): blocks of 64 rows x 16
 // columns, 16 bytes a lane.  Word s of a lane's vector feeds the multiply of
-// the block's rows 32 (s / 2) + 8t + 4 (s % 2) .. + 3; its nibbles j and j + 4
-// are operand register j (columns 2g, 2g + 1 as the instruction's rows g and
-// g + 8).  A nibble q is held as the exact 16-bit number q - 8 and multiplied
-// unscaled; the fp32 sums of each group are scaled as they are added up, so the
-// scales are never rounded into the weights.  One step is 64 rows.
+// the block's rows 32 (s / 2) + 8t + 4 (s % 2) .. + 3; rotated right by 4 j, its bits
+// 3..6 and 19..22 are the two codes of operand register j (columns 2g, 2g + 1 as the
+// instruction's rows g and g + 8).
+//
+// With those bits as the top of a mantissa and a constant exponent, a code q is the
+// 16-bit number B + 8 q (B = 128 in bf16, 1024 in fp16) after one rotation and one
+// logic instruction for two codes.  What is wanted, 8 (q - 8), is that less
+// B + 64, and the sum of (B + 64) x over the rows is the same for every column: one
+// product with a constant operand gives it, and the sums start from its negative.
+// (Subtracting in the operands instead is exact to the bit but costs another
+// instruction for two codes, where the 1.7 codes a cycle and lane that HBM delivers
+// leave 4 or 5.)  The fp32 sums carry terms of up to 31 + 24 (fp16: 143 + 136) steps
+// for a weight of up to 8: 2^-19 of the sum of magnitudes at worst.  The sums of each
+// group are scaled as they are added up, so the scales are never rounded into the
+// weights.  One step is 64 rows.
 template <typename T>
 struct Int4 {
   using Elem = T;
@@ -382,33 +417,52 @@ struct Int4 {
   struct Lane {
     __device__ __forceinline__ Lane(int, int) {}
   };
-  static __device__ __forceinline__ void issue(const Matrix& m, const Strip& s, int k, uint32_t stage,
-                                               uint32_t bar) {
-    const long long nb = m.cols / 16;
-    const char* w = static_cast<const char*>(m.w) + ((s.kb + (k >> 6)) * nb + s.col / 16) * 512;
-    const int g0 = min(k >> m.shift, s.groups - 1);
-    const T* sc = static_cast<const T*>(m.scales) +
-                  static_cast<long long>(s.sg + g0) * m.cols + s.col;
-    // a second group in the step, unless the weight ends before it
-    const bool two = m.shift == 5;
-    const long long next = g0 + 1 < s.groups ? m.cols : 0;
-    const int n = s.lo + s.hi;
-    expect_bytes(bar, 32 * n + (two ? 4 : 2) * n);
-    if (m.gated) {
-      bulk_load(stage, w, 32 * s.lo, bar);
-      bulk_load(stage + 1024, w + 32ll * s.jump, 32 * s.hi, bar);
-      bulk_load(stage + 2048, sc, 2 * s.lo, bar);
-      bulk_load(stage + 2048 + 64, sc + s.jump, 2 * s.hi, bar);
-      if (two) {
-        bulk_load(stage + 2176, sc + next, 2 * s.lo, bar);
-        bulk_load(stage + 2176 + 64, sc + next + s.jump, 2 * s.hi, bar);
-      }
-    } else {
-      bulk_load(stage, w, 32 * n, bar);
-      bulk_load(stage + 2048, sc, 2 * n, bar);
-      if (two) bulk_load(stage + 2176, sc + next, 2 * n, bar);
+  struct Cursor {
+    const char* w;
+    const T* sc;
+    int lo, hi, jump;
+    int left;  // groups after this step's first
+    __device__ __forceinline__ void set(const Matrix& m, const Strip& s, int k) {
+      const long long nb = m.cols / 16;
+      const int g = k >> m.shift;
+      w = static_cast<const char*>(m.w) + ((s.kb + (k >> 6)) * nb + s.col / 16) * 512;
+      sc = static_cast<const T*>(m.scales) + static_cast<long long>(s.sg + g) * m.cols + s.col;
+      lo = s.lo;
+      hi = s.hi;
+      jump = s.jump;
+      left = s.groups - g - 1;
     }
-  }
+    template <int ROWS>
+    __device__ __forceinline__ void next(const Matrix& m) {
+      static_assert(ROWS % 128 == 0, "whole groups");
+      const int g = ROWS >> m.shift;
+      w += static_cast<long long>(m.cols) * (ROWS / 64 * 32);
+      sc += static_cast<long long>(m.cols) * g;
+      left -= g;
+    }
+    __device__ __forceinline__ void issue(const Matrix& m, uint32_t stage, uint32_t bar) const {
+      // a second group in the step, unless the weight ends before it
+      const bool two = m.shift == 5;
+      const T* sd = left > 0 ? sc + m.cols : sc;
+      const int n = lo + hi;
+      expect_bytes(bar, (two ? 36 : 34) * n);
+      if (m.gated) {
+        bulk_load(stage, w, 32 * lo, bar);
+        bulk_load(stage + 1024, w + 32ll * jump, 32 * hi, bar);
+        bulk_load(stage + 2048, sc, 2 * lo, bar);
+        bulk_load(stage + 2048 + 64, sc + jump, 2 * hi, bar);
+        if (two) {
+          bulk_load(stage + 2176, sd, 2 * lo, bar);
+          bulk_load(stage + 2176 + 64, sd + jump, 2 * hi, bar);
+        }
+      } else {
+        bulk_load(stage, w, 32 * n, bar);
+        bulk_load(stage + 2048, sc, 2 * n, bar);
+        if (two) bulk_load(stage + 2176, sd, 2 * n, bar);
+      }
+    }
+  };
+  // The vectors' elements of half h (32 rows) of a step.
   template <int NG, typename Src>
   struct Vectors {
     const T* r[NG];
@@ -418,59 +472,80 @@ struct Int4 {
 #pragma unroll
       for (int n = 0; n < NG; ++n)
         r[n] = 8 * n + g < count ? src.row(8 * n + g) + 8 * (lane & 3) : nullptr;
+      if (Src::kParts == 2 && count <= 4)
+        r[0] = (g & 3) < count ? src.row(g & 3) + (g & 4 ? src.half : 0) + 8 * (lane & 3) : nullptr;
     }
-    __device__ __forceinline__ void load(const Src& src, const Strip& s, int k, int lane) {
+    template <int G, int P>
+    __device__ __forceinline__ void load(int h, const Src& src, int end, int k, int lane) {
 #pragma unroll
-      for (int n = 0; n < NG; ++n)
+      for (int n = 0; n < G; ++n)
 #pragma unroll
-        for (int p = 0; p < Src::kParts; ++p)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            b[h][n][p] = make_uint4(0, 0, 0, 0);
-            if (r[n] && k + 32 * h + 8 * (lane & 3) < s.end)
-              b[h][n][p] = *reinterpret_cast<const uint4*>(r[n] + p * src.half + k + 32 * h);
-          }
+        for (int p = 0; p < P; ++p) {
+          b[h][n][p] = make_uint4(0, 0, 0, 0);
+          if (r[n] && k + 32 * h + 8 * (lane & 3) < end)
+            b[h][n][p] = *reinterpret_cast<const uint4*>(r[n] + p * src.half + k + 32 * h);
+        }
     }
   };
-  // nibbles j and j + 4 of w as two 16-bit numbers q - 8 (exact: 128 + q, or
-  // 1024 + q, is the number whose low mantissa bits are q)
-  static __device__ __forceinline__ uint32_t nibbles(uint32_t w, int j);
-  template <int NG, typename Src>
-  static __device__ __forceinline__ void step(float (&acc)[4][NG][4], const Lane&,
-                                              const Matrix& m, const Strip&, int, uint32_t stage,
+  // codes j of w as B + 8 q, and the operand of -(B + 64)
+  static constexpr uint32_t kBase = kIsBf16<T> ? 0x43004300u : 0x64006400u;
+  static constexpr uint32_t kMinus = kIsBf16<T> ? 0xc340c340u : 0xe440e440u;
+  static __device__ __forceinline__ void operands(uint32_t (&a)[4], uint32_t w) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      a[j] = ((j ? __funnelshift_r(w, w, 4 * j) : w) & 0x00780078u) | kBase;
+  }
+  // One half of a step for the first G groups of vectors and P of their parts.
+  template <int G, int P, int NG, typename Src>
+  static __device__ __forceinline__ void half(int h, float (&acc)[4][NG][4], const Lane&,
+                                              const Matrix& m, int end, int k, uint32_t stage,
                                               int lane, const Vectors<NG, Src>& v) {
-    const bool two = m.shift == 5;
+    if (h && k + 32 >= end) return;
+    float minus[G][4] = {};
+    const uint32_t minus_op[4] = {kMinus, kMinus, kMinus, kMinus};
+    const uint32_t scales = stage + 2048 + 4 * (lane >> 2) + (h && m.shift == 5 ? 128 : 0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint4 f = lds16(stage + 512 * i + 16 * lane);
-      const uint32_t* word = reinterpret_cast<const uint32_t*>(&f);
-      const uint32_t sc0 = lds4(stage + 2048 + 32 * i + 4 * (lane >> 2));
-      const uint32_t sc1 = two ? lds4(stage + 2176 + 32 * i + 4 * (lane >> 2)) : sc0;
+    for (int q = 0; q < 2; ++q)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {  // 32 rows each
-        float part[NG][4];
+      for (int p = 0; p < P; ++p)
 #pragma unroll
-        for (int n = 0; n < NG; ++n)
+        for (int n = 0; n < G; ++n)
+          mma<T>(minus[n], minus_op, q ? v.b[h][n][p].z : v.b[h][n][p].x,
+                 q ? v.b[h][n][p].w : v.b[h][n][p].y);
+    constexpr int kBlocks = G == 1 ? 4 : 2;  // interleaved, as registers allow
 #pragma unroll
-          for (int c = 0; c < 4; ++c) part[n][c] = 0.f;
+    for (int i0 = 0; i0 < 4; i0 += kBlocks) {
+      uint2 w[kBlocks];
+      float part[kBlocks][G][4];
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const uint32_t w = word[2 * h + q];
-          const uint32_t a[4] = {nibbles(w, 0), nibbles(w, 1), nibbles(w, 2), nibbles(w, 3)};
+      for (int i = 0; i < kBlocks; ++i) w[i] = lds8(stage + 512 * (i0 + i) + 16 * lane + 8 * h);
 #pragma unroll
-          for (int n = 0; n < NG; ++n)
+      for (int q = 0; q < 2; ++q)
 #pragma unroll
-            for (int p = 0; p < Src::kParts; ++p)
-              mma<T>(part[n], a, q ? v.b[h][n][p].z : v.b[h][n][p].x,
-                     q ? v.b[h][n][p].w : v.b[h][n][p].y);
+        for (int i = 0; i < kBlocks; ++i) {
+          uint32_t a[4];
+          operands(a, q ? w[i].y : w[i].x);
+#pragma unroll
+          for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int n = 0; n < G; ++n) {
+              if (q == 0 && p == 0)
+                mma<T>(part[i][n], a, v.b[h][n][p].x, v.b[h][n][p].y, minus[n]);
+              else
+                mma<T>(part[i][n], a, q ? v.b[h][n][p].z : v.b[h][n][p].x,
+                       q ? v.b[h][n][p].w : v.b[h][n][p].y);
+            }
         }
-        const float2 sc = unpack2<T>(h ? sc1 : sc0);
 #pragma unroll
-        for (int n = 0; n < NG; ++n) {
-          acc[i][n][0] += sc.x * part[n][0];
-          acc[i][n][1] += sc.x * part[n][1];
-          acc[i][n][2] += sc.y * part[n][2];
-          acc[i][n][3] += sc.y * part[n][3];
+      for (int i = 0; i < kBlocks; ++i) {
+        const float2 sc = unpack2<T>(lds4(scales + 32 * (i0 + i)));
+#pragma unroll
+        for (int n = 0; n < G; ++n) {
+          float(&d)[4] = acc[i0 + i][n];
+          d[0] += sc.x * part[i][n][0];
+          d[1] += sc.x * part[i][n][1];
+          d[2] += sc.y * part[i][n][2];
+          d[3] += sc.y * part[i][n][3];
         }
       }
     }
@@ -486,7 +561,7 @@ struct Int4 {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float2* d = reinterpret_cast<float2*>(p + 16 * i);
-          float2 a = make_float2(acc[i][n][j], acc[i][n][j + 2]);
+          float2 a = make_float2(0.125f * acc[i][n][j], 0.125f * acc[i][n][j + 2]);
           if (ADD) {
             const float2 x = *d;
             a.x += x.x;
@@ -497,23 +572,6 @@ struct Int4 {
       }
   }
 };
-template <>
-__device__ __forceinline__ uint32_t Int4<__nv_bfloat16>::nibbles(uint32_t w, int j) {
-  uint32_t v = ((w >> (4 * j)) & 0x000f000fu) | 0x43004300u;
-  const uint32_t off = 0x43084308u;  // 136
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v),
-                                   *reinterpret_cast<const __nv_bfloat162*>(&off));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-template <>
-__device__ __forceinline__ uint32_t Int4<__half>::nibbles(uint32_t w, int j) {
-  uint32_t v = ((w >> (4 * j)) & 0x000f000fu) | 0x64006400u;
-  const uint32_t off = 0x64086408u;  // 1032
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&v),
-                            *reinterpret_cast<const __half2*>(&off));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-
 // fp32 weights: plain FMAs (the tensor pipe's tf32 would drop 13 bits of both
 // operands).  One step is a box of 16 rows x 64 columns (gated: two of 32): half-warp
 // p takes columns 4c..4c+3 (c = lane % 16) of rows 8p..8p+7; the token values are
@@ -535,12 +593,24 @@ struct Dense32 {
       off = gated ? (c >> 3) * 2048 + p * 1024 + (c & 7) * 16 : p * 2048 + c * 16;
     }
   };
-  static __device__ __forceinline__ void issue(const Matrix& m, const Strip& s, int k, uint32_t stage,
-                                               uint32_t bar) {
-    expect_bytes(bar, kStage);
-    box_load(stage, m.map, s.col, s.row + k, bar);
-    if (m.gated) box_load(stage + 2048, m.map, s.col + s.jump, s.row + k, bar);
-  }
+  // Where the copies of a strip are: the step at row k, then every `rows` further.
+  struct Cursor {
+    int col, jump, row;
+    __device__ __forceinline__ void set(const Matrix&, const Strip& s, int k) {
+      col = s.col;
+      jump = s.jump;
+      row = s.row + k;
+    }
+    template <int ROWS>
+    __device__ __forceinline__ void next(const Matrix&) {
+      row += ROWS;
+    }
+    __device__ __forceinline__ void issue(const Matrix& m, uint32_t stage, uint32_t bar) const {
+      expect_bytes(bar, kStage);
+      box_load(stage, m.map, col, row, bar);
+      if (m.gated) box_load(stage + 2048, m.map, col + jump, row, bar);
+    }
+  };
   template <int NG, typename Src>
   struct Vectors {
     const float* r[4 * NG];
@@ -548,14 +618,16 @@ struct Dense32 {
 #pragma unroll
       for (int t = 0; t < 4 * NG; ++t) r[t] = t < count ? src.row(t) : nullptr;
     }
-    __device__ __forceinline__ void load(const Src&, const Strip&, int, int) {}
+    template <int G, int P>
+    __device__ __forceinline__ void load(int, const Src&, int, int, int) {}
   };
-  template <int NG, typename Src>
-  static __device__ __forceinline__ void step(float (&acc)[4][NG][4], const Lane& l,
-                                              const Matrix&, const Strip& s, int k0, uint32_t stage,
+  // One half of a step for the first G groups of vectors and P of their parts.
+  template <int G, int P, int NG, typename Src>
+  static __device__ __forceinline__ void half(int h, float (&acc)[4][NG][4], const Lane& l,
+                                              const Matrix&, int end, int k0, uint32_t stage,
                                               int lane, const Vectors<NG, Src>& v) {
     const int k = k0 + 8 * (lane >> 4);
-    if (k >= s.end) return;
+    if (h || k >= end) return;  // (one part: all 16 rows)
     float4 w[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {

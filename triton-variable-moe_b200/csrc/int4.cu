@@ -10,10 +10,10 @@
 //
 // Packed layout: blocks of 64 rows x 16 columns in 512 bytes, block rows of N / 16
 // blocks, every segment starting a new block row.  Lane l = 4 g + t of a warp
-// owns 16 bytes of a block; nibbles j and j + 4 of its word s are rows
-// 32 (s / 2) + 8 t + 4 (s % 2) + 2 (j / 2) and the next, column 2 g + j % 2: the
-// operand registers of m16n8k16 in order, so a product loads fragments as they
-// lie, 512 contiguous bytes a warp.
+// owns 16 bytes of a block; bits 3 + 4 j (and 19 + 4 j, around the end) of its word s
+// are rows 32 (s / 2) + 8 t + 4 (s % 2) + 2 (j / 2) and the next, column 2 g + j % 2: a
+// product loads its fragments as they lie, 512 contiguous bytes a warp, and gets the
+// codes to the top of 16-bit mantissas by rotating (few_tokens.cuh).
 //
 // All three are one pass over memory (2.5 bytes a weight at 16 bits) and HBM
 // bound: a CTA takes 128 rows x 64 columns, 16 KB in flight in four vectors a
@@ -60,6 +60,14 @@ __device__ __forceinline__ Where locate(const Segments& s, int chunk, int shift)
   const int row = s.row[lo] + c * kRows;
   return {row, min(kRows, s.row[lo + 1] - row), s.block[lo] + c * (kRows / 64),
           s.group[lo] + (c * kRows >> shift)};
+}
+
+// Where a word holds the code of its row i (0..3) and column c (0, 1).
+__device__ __forceinline__ int bit(int i, int c) {
+  return 3 + 4 * (c + 2 * (i >> 1)) + 16 * (i & 1);
+}
+__device__ __forceinline__ uint32_t place(uint32_t code, int i, int c) {
+  return __funnelshift_l(code, code, bit(i, c));
 }
 
 // The integer nearest to w / s, ties to even, exactly: the quotient's own
@@ -144,8 +152,7 @@ __global__ void __launch_bounds__(kThreadsQ)
         const int cc = 16 * nb + 2 * g + c;
         const float x = to_f<T>(tile[(r0 + i) * kLd + cc]), q = sc[(r0 + i) >> 5][cc];
         const int code = q > 0.f && q <= 3.4028234e38f ? nearest(x, q) + 8 : 8;
-        // rows i, i ^ 1 share a byte column: nibble c + 2 (i / 2), + 4 for odd i
-        v |= static_cast<uint32_t>(code) << (4 * (c + 2 * (i >> 1) + 4 * (i & 1)));
+        v |= place(code, i, c);
       }
     word[s] = v;
   }
@@ -176,7 +183,7 @@ __global__ void __launch_bounds__(kThreadsQ)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const uint32_t code = r0 + i < at.rows ? tile[(r0 + i) * kLd + 16 * nb + 2 * g + c] & 15u : 8u;
-        v |= code << (4 * (c + 2 * (i >> 1) + 4 * (i & 1)));
+        v |= place(code, i, c);
       }
     word[s] = v;
   }
@@ -214,7 +221,7 @@ __global__ void __launch_bounds__(kThreadsQ)
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const int q = static_cast<int>(word[s] >> (4 * (c + 2 * (i >> 1) + 4 * (i & 1))) & 15u) - 8;
+          const int q = static_cast<int>(__funnelshift_r(word[s], word[s], bit(i, c)) & 15u) - 8;
           tile[(r0 + i) * kLd + 16 * nb + 2 * g + c] =
               from_f<S>(static_cast<float>(q) * s2[s >> 1][c]);
         }

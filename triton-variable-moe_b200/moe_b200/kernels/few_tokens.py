@@ -17,9 +17,9 @@ from __future__ import annotations
 
 import torch
 
-from .._lib import ACT_CODE, DTYPE_CODE, check, lib, stream_handle
+from .._lib import ACT_CODE, DTYPE_CODE, check, lib
 from ._ops import _count, _ev_begin, _ev_end, _meta, status_buffer
-from .int4 import Int4Weight, on_device, refuse_grad, row_view
+from .int4 import Int4Weight, eager_only, on_device, refuse_grad, row_view, stream_of
 
 FEW_TOKENS_MAX = 64
 
@@ -60,7 +60,7 @@ def _check_weights(x, router, w1, w2, num_experts, hidden, max_width, gated):
     return w1, None, w2, None, 0, 0, 0, total
 
 
-@torch.compiler.disable
+@eager_only
 def moe_few_tokens(
     x: torch.Tensor,
     router_weight: torch.Tensor,
@@ -140,7 +140,7 @@ def moe_few_tokens(
             x.data_ptr(), T, x.stride(0) if T > 1 else H, H, pr, E, p1, s1, p2, s2, group, blocks,
             groups, total, off.data_ptr(), max_expert_width, top_k, 1 if norm_topk_prob else 0, act,
             out.data_ptr(), H, ws.data_ptr(), ws_bytes, DTYPE_CODE[x.dtype],
-            status_buffer(dev).data_ptr(), stream_handle(dev))
+            status_buffer(dev).data_ptr(), stream_of(dev))
         _ev_end(ev, "few_tokens")
     check(rc, "moe_few_tokens")
     _count(2)

@@ -17,16 +17,32 @@ All of it is for inference: nothing here is differentiable.
 from __future__ import annotations
 
 import ctypes
+import functools
 from collections.abc import Sequence
+from contextlib import nullcontext
 from dataclasses import dataclass, field
 
 import torch
 
-from .._lib import ACT_CODE, DTYPE_CODE, check, lib, ptr, stream_handle
+from .._lib import ACT_CODE, DTYPE_CODE, check, lib, ptr
 from ._ops import _count, _ev_begin, _ev_end, _meta, status_buffer
 
 GROUP_SIZES = (32, 64, 128)
 MAX_GEMV_ROWS = 65536
+
+
+def eager_only(fn):
+    """torch.compiler.disable for calls of a few microseconds: the disabled wrapper
+    (8 us a call) is taken only while a graph is being traced."""
+    disabled = torch.compiler.disable(fn)
+
+    @functools.wraps(fn)
+    def call(*args, **kwargs):
+        if torch.compiler.is_compiling():
+            return disabled(*args, **kwargs)
+        return fn(*args, **kwargs)
+
+    return call
 
 
 def refuse_grad(name: str, *tensors: torch.Tensor) -> None:
@@ -37,9 +53,18 @@ def refuse_grad(name: str, *tensors: torch.Tensor) -> None:
                                    "torch.no_grad() or torch.inference_mode()")
 
 
+_here = nullcontext()
+
+
 def on_device(device: torch.device):
     """Context in which `device` is the current CUDA device."""
-    return torch.cuda.device(device)
+    return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def stream_of(device: torch.device) -> int:
+    """The current stream's handle (torch.cuda.current_stream builds an object first,
+    2 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def row_view(x: torch.Tensor) -> torch.Tensor:
@@ -84,6 +109,14 @@ class Int4Weight:
             raise ValueError("packed and scales must be 16-byte aligned")
         object.__setattr__(self, "_host_offsets", host)
 
+    @classmethod
+    def _trusted(cls, packed, scales, rows, cols, group_size, row_offsets, host) -> "Int4Weight":
+        """From parts that this module has just made."""
+        self = object.__new__(cls)
+        self.__dict__.update(packed=packed, scales=scales, rows=rows, cols=cols,
+                             group_size=group_size, row_offsets=row_offsets, _host_offsets=host)
+        return self
+
     @property
     def dtype(self) -> torch.dtype:
         return self.scales.dtype
@@ -117,7 +150,7 @@ def _layout(rows: int, cols: int, group_size: int, row_offsets):
         n = len(row_offsets) - 1
         if not 1 <= n <= 256:
             raise ValueError(f"row_offsets must name 1 to 256 segments, got {n}")
-        if any(not 0 <= o < 2**31 for o in row_offsets):
+        if min(row_offsets) < 0 or max(row_offsets) >= 2**31:
             raise ValueError(f"row_offsets must lie in 0..{rows}")
         host = (ctypes.c_int32 * (n + 1))(*row_offsets)
     blocks, groups = ctypes.c_int64(), ctypes.c_int64()
@@ -139,7 +172,7 @@ def _offsets_tuple(row_offsets: Sequence[int] | None) -> tuple[int, ...] | None:
     return tuple(int(o) for o in row_offsets)
 
 
-@torch.compiler.disable
+@eager_only
 def quantize_int4(w: torch.Tensor, group_size: int = 64, row_offsets: Sequence[int] | None = None,
                   dtype: torch.dtype | None = None) -> Int4Weight:
     """Round w [K, N] to 4 bits: in each column, for every `group_size` rows,
@@ -169,14 +202,14 @@ def quantize_int4(w: torch.Tensor, group_size: int = 64, row_offsets: Sequence[i
         ev = _ev_begin()
         rc = lib.moe_int4_quantize(ptr(w), K, N, w.stride(0) if K > 1 else N, DTYPE_CODE[w.dtype],
                                    group_size, host, 1 if host is None else len(offsets) - 1,
-                                   ptr(packed), ptr(scales), DTYPE_CODE[dtype], stream_handle(dev))
+                                   ptr(packed), ptr(scales), DTYPE_CODE[dtype], stream_of(dev))
         _ev_end(ev, "quantize_int4")
     check(rc, "moe_int4_quantize")
     _count(1)
-    return Int4Weight(packed, scales, K, N, group_size, offsets)
+    return Int4Weight._trusted(packed, scales, K, N, group_size, offsets, host)
 
 
-@torch.compiler.disable
+@eager_only
 def pack_int4(codes: torch.Tensor, scales: torch.Tensor, group_size: int,
               row_offsets: Sequence[int] | None = None) -> Int4Weight:
     """An Int4Weight from uint8 codes [K, N] (the low 4 bits; 8 stands for zero)
@@ -201,14 +234,14 @@ def pack_int4(codes: torch.Tensor, scales: torch.Tensor, group_size: int,
         ev = _ev_begin()
         rc = lib.moe_int4_pack(ptr(codes), K, N, codes.stride(0) if K > 1 else N, group_size, host,
                                1 if host is None else len(offsets) - 1, ptr(packed),
-                               stream_handle(dev))
+                               stream_of(dev))
         _ev_end(ev, "pack_int4")
     check(rc, "moe_int4_pack")
     _count(1)
     return Int4Weight(packed, scales, K, N, group_size, offsets)
 
 
-@torch.compiler.disable
+@eager_only
 def dequantize_int4(q: Int4Weight) -> torch.Tensor:
     """The values (q - 8) * scale [K, N], rounded to the scales' type."""
     if not q.packed.is_cuda:
@@ -219,7 +252,7 @@ def dequantize_int4(q: Int4Weight) -> torch.Tensor:
         ev = _ev_begin()
         rc = lib.moe_int4_dequantize(ptr(q.packed), ptr(q.scales), q.rows, q.cols, q.group_size,
                                      host, n, ptr(out), q.cols, DTYPE_CODE[q.dtype],
-                                     stream_handle(q.device))
+                                     stream_of(q.device))
         _ev_end(ev, "dequantize_int4")
     check(rc, "moe_int4_dequantize")
     _count(1)
@@ -283,14 +316,14 @@ def _gemv(name, x, q, tok_off, w_off, expert_widths, tok_cnt, hidden, max_width,
             q.group_size, q.packed.shape[0], q.scales.shape[0], hidden,
             q.rows if down else q.cols, ptr(tok_off), ptr(w_off), ptr(tok_cnt), E, max_width,
             ACT_CODE[activation], 1 if down else 0, ptr(out), out_cols, ptr(ws), ws_bytes,
-            DTYPE_CODE[x.dtype], ptr(status_buffer(dev)), stream_handle(dev))
+            DTYPE_CODE[x.dtype], ptr(status_buffer(dev)), stream_of(dev))
         _ev_end(ev, name)
     check(rc, "moe_grouped_gemv_int4")
     _count(2)
     return out
 
 
-@torch.compiler.disable
+@eager_only
 def grouped_gemv_up_int4(
     x: torch.Tensor,
     w1: Int4Weight,
@@ -314,7 +347,7 @@ def grouped_gemv_up_int4(
                  activation, False)
 
 
-@torch.compiler.disable
+@eager_only
 def grouped_gemv_down_int4(
     intermediate: torch.Tensor,
     w2: Int4Weight,
