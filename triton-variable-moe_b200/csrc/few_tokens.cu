@@ -21,6 +21,7 @@
 //                a whole wave are cut into slices of the reduction, all in one
 //                cluster; the team that finishes an item's last slice (a counter in
 //                shared memory) adds them in order.  Then the activation, and h.
+//                (More than 8 tokens: a router kernel runs first.)
 //   down kernel  The units (slice of an expert's width, 64-column tile of the
 //                hidden size).  The team that finishes a column tile's last unit
 //                (a counter per tile, zeroed by the up kernel) adds the tile's
@@ -102,10 +103,11 @@ struct LayerParams {
   int blocks2, groups2;      // block rows and groups of the packed w2
   int down_teams;            // teams of the down kernel's grid
   int smem_work;             // up kernel: bytes before its UpSmem
-  int cluster;               // its CTAs a cluster
+  int cluster;               // its CTAs a cluster (1: the router kernel ran)
   void* out;
   long long ldo;
   // workspace
+  int* sel;                  // [T * k] from the router kernel, or null
   int* plan;                 // [PLAN_WORDS], then an Active
   int* slot;                 // [T * k] active expert of an assignment (-1: none)
   int* row;                  // [T * k] its expert-sorted row
@@ -118,15 +120,6 @@ struct LayerParams {
   float* y;                  // [slices][T * k][H]
   int max_slices;
   int* status;
-};
-
-// What every kernel here keeps in shared memory (16-byte vectors follow it).
-struct alignas(16) Common {
-  Active act;
-  unsigned long long bar[kWarps][kMaxDepth];
-  int plan[4];  // number of active experts, items, rounds of a slice
-  int last[kTeams];
-  int abort;
 };
 
 // Exclusive prefix sum over a warp; `total` gets the sum.
@@ -156,33 +149,28 @@ __device__ __forceinline__ void team_sync(int team) {
   asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(kTeamThreads) : "memory");
 }
 
-// Where unit i lies.  Finding it takes a search and a few divisions, so a warp's
-// lanes do it for 32 units of their team at once and hand them out by shuffle.
-struct Place {
-  unsigned a, b;  // e | tile << 8 | slice << 20; pass
-  __device__ __forceinline__ Place() {}
-  __device__ __forceinline__ Place(int e, int tile, int slice, int pass)
-      : a(static_cast<unsigned>(e) | static_cast<unsigned>(tile) << 8 |
-          static_cast<unsigned>(slice) << 20),
-        b(static_cast<unsigned>(pass)) {}
-};
-static_assert(kMaxExperts <= 256 && kMaxWidth / 32 <= 4096, "bits of a place");
-
-// One unit of a team.
-struct Unit {
+// One unit of a team.  The first units of every team are worked out once, a thread each,
+// into a table in shared memory: by the warps themselves, twice (for the copies and for
+// the products), that is a few thousand cycles before the first byte.
+struct alignas(16) Unit {
   Strip strip;
   int begin;           // first reduction row
   int count;           // vectors
   int row;             // first of them in expert-sorted order
   int e, tile, slice;  // active expert, column tile, slice of the reduction
-  int pass;            // first vector within the expert
   int local;           // up kernel: the cluster's item that this is a slice of, or -1
-  __device__ __forceinline__ void set(const Place& w, int vectors) {
-    e = static_cast<int>(w.a & 255);
-    tile = static_cast<int>(w.a >> 8 & 4095);
-    slice = static_cast<int>(w.a >> 20);
-    pass = static_cast<int>(w.b) * vectors;
-  }
+};
+static_assert(sizeof(Unit) == 64, "four vectors");
+constexpr int kTable = 64;  // units a team
+
+// What every kernel here keeps in shared memory (16-byte vectors follow it).
+struct alignas(16) Common {
+  Active act;
+  unsigned long long bar[kWarps][kMaxDepth];
+  int plan[4];  // number of active experts, items, rounds of a slice
+  int last[kTeams];
+  int abort;
+  Unit table[kTeams][kTable];
 };
 
 // The strip of an up product's tile: 64 columns, or 32 gate and their 32 up columns.
@@ -231,16 +219,15 @@ __device__ __forceinline__ bool ring_wait(uint32_t bar, uint32_t parity, volatil
 
 // Runs the `total` units of a team.  Every warp copies its steps (begin + (wr + 4 j)
 // kStep) into its ring as far ahead as it is deep, on into its next units, so the
-// loads go on during the reduction and the output of a unit.  place(n) finds the
-// team's n-th unit, unit(place) describes it, source(unit) gives its vectors, and
-// finish(unit) finds the unit's sums in red (see unit_sum) between team barriers.
+// loads go on during the reduction and the output of a unit.  unit(n) works out the
+// team's n-th unit, source(unit) gives its vectors, and finish(unit) finds the unit's
+// sums in red (see unit_sum) between team barriers.
 template <int N>
 using Int = std::integral_constant<int, N>;
 
-template <typename L, int NG, typename Find, typename MakeUnit, typename MakeSource,
-          typename Finish>
+template <typename L, int NG, typename MakeUnit, typename MakeSource, typename Finish>
 __device__ __forceinline__ void run_units(int total, const Matrix& m,
-                                          unsigned char* work, float* red, Common& c, Find place,
+                                          unsigned char* work, float* red, Common& c,
                                           MakeUnit unit, MakeSource source, Finish finish) {
   constexpr int kRows = kTeam * L::kStep, TOK = L::template kTokens<NG>;
   constexpr int D = L::template kDepth<NG>;
@@ -249,35 +236,23 @@ __device__ __forceinline__ void run_units(int total, const Matrix& m,
   const uint32_t ring = smem_u32(work) + wid * (D * L::kStage);
   const uint32_t bars = smem_u32(&c.bar[wid][0]);
   const typename L::Lane at(lane, m.gated);
-  using Src = decltype(source(unit(Place())));
-  auto nth = [&](int n, Place& mine) {
-    if (n % 32 == 0 && n + lane < total) mine = place(n + lane);
-    __syncwarp();
-    Place q;
-    q.a = __shfl_sync(0xffffffffu, mine.a, n % 32);
-    q.b = __shfl_sync(0xffffffffu, mine.b, n % 32);
-    return unit(q);
-  };
+  using Src = decltype(source(unit(0)));
+  const int tt = threadIdx.x % kTeamThreads;
+  if (tt < min(total, kTable)) c.table[team][tt] = unit(tt);
+  team_sync(team);
+  auto nth = [&](int n) { return n < kTable ? c.table[team][n] : unit(n); };
 
   int copied = 0, used = 0;  // steps
   // the copying side: the team's cn-th unit, next step at row ck
   int cn = -1, ck = 0, cend = 0;
   bool more = true;
-  Place ahead(0, 0, 0, 0), here(0, 0, 0, 0);
   typename L::Cursor cursor;
-  // the multiplying side
-  int k = 0, n = -1;
-  Unit u;
-  u.strip.end = 0;
-  float acc[4][NG][4];
-  typename L::template Vectors<NG, Src> v;
-  Src src;
-  while (true) {
+  auto top_up = [&]() {
     while (more && copied - used < D) {
       if (ck >= cend) {
         more = ++cn < total && !*static_cast<volatile int*>(&c.abort);
         if (more) {
-          const Unit cu = nth(cn, ahead);
+          const Unit cu = nth(cn);
           ck = cu.begin + wr * L::kStep;
           cend = cu.strip.end;
           if (ck < cend) cursor.set(m, cu.strip, ck);
@@ -290,57 +265,58 @@ __device__ __forceinline__ void run_units(int total, const Matrix& m,
         cursor.template next<kRows>(m);
       }
     }
-    if (k < u.strip.end) {
-      // (the vectors of each half load during the half before)
-      const int slot = used % D;
-      const uint32_t stage = ring + slot * L::kStage;
-      auto step = [&](auto groups, auto parts) {
-        constexpr int G = decltype(groups)::value, P = decltype(parts)::value;
-        v.template load<G, P>(1, src, u.strip.end, k, lane);
-        if (used < copied) ring_wait(bars + 8 * slot, (used / D) & 1, &c.abort);
-        L::template half<G, P, NG, Src>(0, acc, at, m, u.strip.end, k, stage, lane, v);
-        v.template load<G, P>(0, src, u.strip.end, k + kRows, lane);
-        L::template half<G, P, NG, Src>(1, acc, at, m, u.strip.end, k, stage, lane, v);
-      };
-      // only the columns and parts that the unit has
-      if (NG > 1 && u.count > 8)
-        step(Int<NG>(), Int<Src::kParts>());
-      else if (Src::kParts == 2 && u.count > 4)
-        step(Int<1>(), Int<2>());
-      else
-        step(Int<1>(), Int<1>());
-      __syncwarp();  // the step has been read by every lane: its place is free
-      ++used;
-      k += kRows;
-    } else {
-      if (n >= 0) {
-        // warps 2 and 3 leave their sums, 0 and 1 add theirs to them
-        float* mine = red + (wr & 1) * TOK * kRedLd;
-        if (wr >= 2) L::template store<NG, kRedLd, false>(acc, lane, mine);
-        team_sync(team);
-        if (wr < 2) L::template store<NG, kRedLd, true>(acc, lane, mine);
-        team_sync(team);
-        finish(u);
-        team_sync(team);
-      }
-      if (++n >= total) break;
-      u = nth(n, here);
-      k = u.begin + wr * L::kStep;
-      src = source(u);
-      v.rows(src, u.count, lane);
-      if (NG > 1 && u.count > 8)
-        v.template load<NG, Src::kParts>(0, src, u.strip.end, k, lane);
-      else if (Src::kParts == 2 && u.count > 4)
-        v.template load<1, 2>(0, src, u.strip.end, k, lane);
-      else
-        v.template load<1, 1>(0, src, u.strip.end, k, lane);
+  };
+  top_up();
+  float acc[4][NG][4];
+  for (int n = 0; n < total; ++n) {
+    const Unit u = nth(n);
+    const Src src = source(u);
+    // with only the groups of columns, and parts, that the unit has
+    auto sums = [&](auto groups, auto parts) {
+      constexpr int G = decltype(groups)::value, P = decltype(parts)::value;
 #pragma unroll
       for (int a = 0; a < 4; ++a)
 #pragma unroll
-        for (int g = 0; g < NG; ++g)
+        for (int g = 0; g < G; ++g)
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[a][g][j] = 0.f;
-    }
+      const int k = u.begin + wr * L::kStep;
+      int left = u.strip.end - k;
+      typename L::template Vectors<NG, Src> v;
+      if (left > 0) {
+        v.template rows<G, P>(src, u.count, k, lane);
+        v.template load<G, P>(0, src, left, lane);
+      }
+      for (; left > 0; left -= kRows) {  // the vectors of each half load during the half before
+        const int slot = used % D;
+        const uint32_t stage = ring + slot * L::kStage;
+        v.template load<G, P>(1, src, left, lane);
+        if (used < copied) ring_wait(bars + 8 * slot, (used / D) & 1, &c.abort);
+        L::template half<G, P, NG, Src>(0, acc, at, m, left, stage, lane, v);
+        v.template advance<G>(kRows);
+        v.template load<G, P>(0, src, left - kRows, lane);
+        L::template half<G, P, NG, Src>(1, acc, at, m, left, stage, lane, v);
+        __syncwarp();  // the step has been read by every lane: its place is free
+        ++used;
+        top_up();
+      }
+      // warps 2 and 3 leave their sums, 0 and 1 add theirs to them
+      float* mine = red + (wr & 1) * TOK * kRedLd;
+      if (wr >= 2) L::template store<G, NG, kRedLd, false>(acc, lane, mine);
+      team_sync(team);
+      if (wr < 2) L::template store<G, NG, kRedLd, true>(acc, lane, mine);
+      team_sync(team);
+    };
+    if constexpr (!L::kGroups)
+      sums(Int<NG>(), Int<1>());
+    else if (NG > 1 && u.count > 8)
+      sums(Int<NG>(), Int<Src::kParts>());
+    else if (Src::kParts == 2 && u.count > 4)
+      sums(Int<1>(), Int<2>());
+    else
+      sums(Int<1>(), Int<1>());
+    finish(u);
+    team_sync(team);
   }
   // after an abort: copies still in flight land before the block ends
   for (; used < copied; ++used) {
@@ -431,91 +407,75 @@ __device__ __forceinline__ int plan_length(int most, int teams, int max_slices, 
 }
 
 // ---- routing --------------------------------------------------------------
-// This CTA's partial logits over reduction range [k_lo, k_hi): log[t][E16].
+// This CTA's partial logits of up to 8 tokens over reduction range [k_lo, k_hi):
+// log[t][E16].
 template <typename T>
-__device__ __forceinline__ void partial_logits(const LayerParams& p, int k_lo, int k_hi,
-                                               float* part, float* log, int lde) {
+__device__ __forceinline__ void partial_logits(const LayerParams& p, const T* x, int count,
+                                               int k_lo, int k_hi, float* part, float* log,
+                                               int lde) {
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int g = lane >> 2, t4 = lane & 3;
-  const T* x = static_cast<const T*>(p.x);
   const T* wr = static_cast<const T*>(p.router);
   const int tiles = lde / 16, ksub = max(1, kWarps / tiles);
-  // 16 experts x all tokens an item; ksub warps split its reduction
+  // 16 experts an item; ksub warps split its reduction
   for (int item = wid; item < tiles * ksub; item += kWarps) {
     const int et = item % tiles, ks = item / tiles;
     const int e0 = et * 16 + g, e1 = e0 + 8;
-    for (int tg0 = 0; tg0 < p.T; tg0 += 32) {
-      float acc[4][4];
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    constexpr int kBatch = 4;  // steps whose loads are issued together
+    for (int k0 = k_lo + 32 * ks; k0 < k_hi; k0 += 32 * ksub * kBatch) {
+      uint4 a[kBatch][2], b[kBatch];
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[n][c] = 0.f;
-      constexpr int kBatch = 2;  // steps whose loads are issued together
-      for (int k0 = k_lo + 32 * ks; k0 < k_hi; k0 += 32 * ksub * kBatch) {
-        uint4 a[kBatch][2], b[kBatch][4];
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          const int k = k0 + 32 * ksub * j + 8 * t4;
-          const bool in = k0 + 32 * ksub * j < k_hi && k < p.H;
-          const uint4 zero = make_uint4(0, 0, 0, 0);
-          a[j][0] = in && e0 < p.E
-                        ? *reinterpret_cast<const uint4*>(wr + static_cast<long long>(e0) * p.H + k)
-                        : zero;
-          a[j][1] = in && e1 < p.E
-                        ? *reinterpret_cast<const uint4*>(wr + static_cast<long long>(e1) * p.H + k)
-                        : zero;
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const int t = tg0 + 8 * n + g;
-            b[j][n] = in && t < p.T
-                          ? *reinterpret_cast<const uint4*>(x + static_cast<long long>(t) * p.ldx + k)
-                          : zero;
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          const uint32_t a0[4] = {a[j][0].x, a[j][1].x, a[j][0].y, a[j][1].y};
-          const uint32_t a1[4] = {a[j][0].z, a[j][1].z, a[j][0].w, a[j][1].w};
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            if (tg0 + 8 * n < p.T) {
-              mma<T>(acc[n], a0, b[j][n].x, b[j][n].y);
-              mma<T>(acc[n], a1, b[j][n].z, b[j][n].w);
-            }
-          }
-        }
+      for (int j = 0; j < kBatch; ++j) {
+        const int k = k0 + 32 * ksub * j + 8 * t4;
+        const bool in = k0 + 32 * ksub * j < k_hi && k < p.H;
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        a[j][0] = in && e0 < p.E
+                      ? *reinterpret_cast<const uint4*>(wr + static_cast<long long>(e0) * p.H + k)
+                      : zero;
+        a[j][1] = in && e1 < p.E
+                      ? *reinterpret_cast<const uint4*>(wr + static_cast<long long>(e1) * p.H + k)
+                      : zero;
+        b[j] = in && g < count
+                   ? *reinterpret_cast<const uint4*>(x + static_cast<long long>(g) * p.ldx + k)
+                   : zero;
       }
-      // rows of the result are experts, columns tokens
 #pragma unroll
-      for (int n = 0; n < 4; ++n)
+      for (int j = 0; j < kBatch; ++j) {
+        const uint32_t a0[4] = {a[j][0].x, a[j][1].x, a[j][0].y, a[j][1].y};
+        const uint32_t a1[4] = {a[j][0].z, a[j][1].z, a[j][0].w, a[j][1].w};
+        mma<T>(acc, a0, b[j].x, b[j].y);
+        mma<T>(acc, a1, b[j].z, b[j].w);
+      }
+    }
+    // rows of the result are experts, columns tokens
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int t = tg0 + 8 * n + 2 * t4 + j;
-          if (t < p.T) {
-            part[(ks * p.T + t) * lde + e0] = acc[n][j];
-            part[(ks * p.T + t) * lde + e1] = acc[n][j + 2];
-          }
-        }
+    for (int j = 0; j < 2; ++j) {
+      const int t = 2 * t4 + j;
+      if (t < count) {
+        part[(ks * count + t) * lde + e0] = acc[j];
+        part[(ks * count + t) * lde + e1] = acc[j + 2];
+      }
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < p.T * lde; i += kThreads) {
+  for (int i = threadIdx.x; i < count * lde; i += kThreads) {
     float s = part[i];
-    for (int q = 1; q < ksub; ++q) s += part[q * p.T * lde + i];
+    for (int q = 1; q < ksub; ++q) s += part[q * count * lde + i];
     log[i] = s;
   }
 }
 
 template <>
-__device__ __forceinline__ void partial_logits<float>(const LayerParams& p, int k_lo, int k_hi,
-                                                      float*, float* log, int lde) {
+__device__ __forceinline__ void partial_logits<float>(const LayerParams& p, const float* x,
+                                                      int count, int k_lo, int k_hi, float*,
+                                                      float* log, int lde) {
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  const float* x = static_cast<const float*>(p.x);
   const float* wr = static_cast<const float*>(p.router);
   const int hi = min(k_hi, p.H);
   for (int e = wid; e < p.E; e += kWarps) {
     const float* row = wr + static_cast<long long>(e) * p.H;
-    for (int t0 = 0; t0 < p.T; t0 += 8) {
+    for (int t0 = 0; t0 < count; t0 += 8) {
       float acc[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc[j] = 0.f;
@@ -523,7 +483,7 @@ __device__ __forceinline__ void partial_logits<float>(const LayerParams& p, int 
         const float4 w = *reinterpret_cast<const float4*>(row + k);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          if (t0 + j < p.T) {
+          if (t0 + j < count) {
             const float4 v =
                 *reinterpret_cast<const float4*>(x + static_cast<long long>(t0 + j) * p.ldx + k);
             acc[j] = fmaf(v.x, w.x, acc[j]);
@@ -537,7 +497,7 @@ __device__ __forceinline__ void partial_logits<float>(const LayerParams& p, int 
       for (int j = 0; j < 8; ++j) {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], o);
-        if (lane == 0 && t0 + j < p.T) log[(t0 + j) * lde + e] = acc[j];
+        if (lane == 0 && t0 + j < count) log[(t0 + j) * lde + e] = acc[j];
       }
     }
   }
@@ -550,28 +510,31 @@ __device__ __forceinline__ unsigned order_key(float v) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-// One warp chooses the k experts of token t from the cluster's partial logits (value
-// j of lane l is expert 32 j + l) and tells every CTA of the cluster.
-template <int J, typename Smem>
+// One warp chooses the k experts of row t of the cluster's partial logits (value j of
+// lane l is expert 32 j + l): lane s < k gets the s-th and its weight.
+template <int J>
 __device__ __forceinline__ void choose(const LayerParams& p, cg::cluster_group& cluster, float* log,
-                                       int lde, int t, Smem& sm, int* sel_s, float* wgt_s) {
+                                       int lde, int t, int* sel_out, float* wgt_out) {
   const int lane = threadIdx.x & 31;
   float v[J];
   unsigned key[J];
 #pragma unroll
   for (int j = 0; j < J; ++j) v[j] = 0.f;
-  for (int c = 0; c < p.cluster; c += 2) {
-    const float* q0 = cluster.map_shared_rank(log, c) + t * lde;
-    const float* q1 = cluster.map_shared_rank(log, c + 1) + t * lde;
-    float a[J], b[J];
+  const int ctas = static_cast<int>(cluster.num_blocks());
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int e = min(32 * j + lane, p.E - 1);
-      a[j] = q0[e];
-      b[j] = q1[e];
+  for (int c0 = 0; c0 < kMaxCluster; c0 += 4) {  // four CTAs' parts in flight
+    if (c0 >= ctas) break;
+    float a[4][J];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float* q = cluster.map_shared_rank(log, min(c0 + c, ctas - 1)) + t * lde;
+#pragma unroll
+      for (int j = 0; j < J; ++j) a[c][j] = q[min(32 * j + lane, p.E - 1)];
     }
 #pragma unroll
-    for (int j = 0; j < J; ++j) v[j] = v[j] + a[j] + b[j];
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int j = 0; j < J; ++j) v[j] += c0 + c < ctas ? a[c][j] : 0.f;
   }
 #pragma unroll
   for (int j = 0; j < J; ++j) key[j] = 32 * j + lane < p.E ? order_key(v[j]) : 0u;
@@ -607,22 +570,57 @@ __device__ __forceinline__ void choose(const LayerParams& p, cg::cluster_group& 
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     w = w / (sum + 1e-20f);
   }
-  if (lane < p.k) {
-    for (int c = 0; c < p.cluster; ++c) {
-      cluster.map_shared_rank(sel_s, c)[t * p.k + lane] = sel;
-      cluster.map_shared_rank(wgt_s, c)[t * p.k + lane] = w;
-      // (32-bit words: 64-bit atomics of several CTAs on one shared word lose bits)
-      atomicOr(reinterpret_cast<unsigned*>(cluster.map_shared_rank(sm.mask, c) + sel) + (t >> 5),
-               1u << (t & 31));
+  *sel_out = sel;
+  *wgt_out = w;
+}
+__device__ __forceinline__ void choose(const LayerParams& p, cg::cluster_group& cluster, float* log,
+                                       int lde, int t, int* sel, float* wgt) {
+  if (p.E <= 32)
+    choose<1>(p, cluster, log, lde, t, sel, wgt);
+  else if (p.E <= 64)
+    choose<2>(p, cluster, log, lde, t, sel, wgt);
+  else if (p.E <= 128)
+    choose<4>(p, cluster, log, lde, t, sel, wgt);
+  else
+    choose<8>(p, cluster, log, lde, t, sel, wgt);
+}
+
+// ---- router kernel (more than 8 tokens) ----------------------------------------
+// Every cluster of the up kernel would route all tokens (33 tokens, 64 experts: 7 us);
+// here a cluster of 8 CTAs has 8 of them, each CTA an eighth of the hidden size and
+// then one token to choose for.  The up kernel then needs no clusters and runs on all
+// SMs.
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1) few_router_kernel(const __grid_constant__ LayerParams p) {
+  extern __shared__ __align__(1024) unsigned char raw[];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = static_cast<int>(cluster.block_rank()), lane = threadIdx.x & 31;
+  const int t0 = blockIdx.x / kMaxCluster * kMaxCluster, count = min(kMaxCluster, p.T - t0);
+  const int lde = ceil_div(p.E, 16) * 16;
+  float* log = reinterpret_cast<float*>(raw);
+  float* part = log + count * lde;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int per = ceil_div(ceil_div(p.H, 32), kMaxCluster) * 32;
+  partial_logits<T>(p, static_cast<const T*>(p.x) + t0 * p.ldx, count, min(rank * per, p.H),
+                    min((rank + 1) * per, p.H), part, log, lde);
+  cluster.sync();
+  if (rank < count && threadIdx.x < 32) {
+    int sel;
+    float wgt;
+    choose(p, cluster, log, lde, rank, &sel, &wgt);
+    if (lane < p.k) {
+      p.sel[(t0 + rank) * p.k + lane] = sel;
+      p.wgt[(t0 + rank) * p.k + lane] = wgt;
     }
   }
+  cluster.sync();  // the parts stay until they have been read
 }
 
 // ---- the layer's active experts ----------------------------------------------
 struct alignas(16) UpSmem {
   Common c;
   unsigned long long mask[kMaxExperts];      // tokens of each expert
-  unsigned long long act_mask[kMaxExperts];  // of each active expert
   int off[kMaxExperts + 1];
   int slot[kMaxExperts];  // active expert of an expert (-1: none)
   int base[kMaxExperts];  // first expert-sorted row of an expert
@@ -689,7 +687,6 @@ __device__ __forceinline__ void find_active(const LayerParams& p, UpSmem& s) {
       s.c.act.kb[at] = s.kb[e];
       s.c.act.sg[at] = s.sg[e];
       s.c.act.item[at] = static_cast<int>(mine & 0xfffffu);
-      s.act_mask[at] = mask;
     }
   }
   if (lane == 0) {
@@ -765,11 +762,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   UpSmem& s = *reinterpret_cast<UpSmem*>(raw + p.smem_work);
   int* sel_s = reinterpret_cast<int*>(raw + p.smem_work + sizeof(UpSmem));
   float* wgt_s = reinterpret_cast<float*>(sel_s + A);
+  int* list = sel_s + 2 * A;  // token of each expert-sorted row
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = static_cast<int>(cluster.block_rank());
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
 
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // (the router kernel, if it ran, waited for the inputs)
+  if (!p.sel) asm volatile("griddepcontrol.wait;" ::: "memory");
   // every block of this grid runs by the time the last one gets here
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   for (int e = tid; e <= p.E; e += kThreads) s.off[e] = p.off[e];
@@ -781,22 +780,40 @@ __global__ void __launch_bounds__(kThreads, 1)
   for (int i = tid; i < kMaxLocal; i += kThreads) s.ticket[i] = 0;
   ring_init<L::template kDepth<NG>>(s.c);
 
-  // routing: this CTA's part of the hidden size, then tokens rank, rank + cluster, ...
-  const int per = ceil_div(ceil_div(p.H, 32), p.cluster) * 32;
-  partial_logits<T>(p, min(rank * per, p.H), min((rank + 1) * per, p.H), part, log, lde);
-  cluster.sync();
-  if (p.shift && wid == kWarps - 1) find_packed(p, s);
-  for (int t = rank + p.cluster * wid; t < p.T; t += p.cluster * kWarps) {
-    if (p.E <= 32)
-      choose<1>(p, cluster, log, lde, t, s, sel_s, wgt_s);
-    else if (p.E <= 64)
-      choose<2>(p, cluster, log, lde, t, s, sel_s, wgt_s);
-    else if (p.E <= 128)
-      choose<4>(p, cluster, log, lde, t, s, sel_s, wgt_s);
-    else
-      choose<8>(p, cluster, log, lde, t, s, sel_s, wgt_s);
+  unsigned* mask32 = reinterpret_cast<unsigned*>(s.mask);
+  if (p.sel) {
+    __syncthreads();
+    if (p.shift && wid == kWarps - 1) find_packed(p, s);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (int a = tid; a < A; a += kThreads) {
+      const int sel = p.sel[a], t = a / p.k;
+      sel_s[a] = sel;
+      wgt_s[a] = p.wgt[a];
+      atomicOr(mask32 + 2 * sel + (t >> 5), 1u << (t & 31));
+    }
+    __syncthreads();
+  } else {
+    // routing: this CTA's part of the hidden size, then tokens rank, rank + cluster, ...
+    const int per = ceil_div(ceil_div(p.H, 32), p.cluster) * 32;
+    partial_logits<T>(p, static_cast<const T*>(p.x), p.T, min(rank * per, p.H),
+                      min((rank + 1) * per, p.H), part, log, lde);
+    cluster.sync();
+    if (p.shift && wid == kWarps - 1) find_packed(p, s);
+    for (int t = rank + p.cluster * wid; t < p.T; t += p.cluster * kWarps) {
+      int sel;
+      float wgt;
+      choose(p, cluster, log, lde, t, &sel, &wgt);
+      if (lane < p.k) {
+        for (int c = 0; c < p.cluster; ++c) {
+          cluster.map_shared_rank(sel_s, c)[t * p.k + lane] = sel;
+          cluster.map_shared_rank(wgt_s, c)[t * p.k + lane] = wgt;
+          // (32-bit words: 64-bit atomics of several CTAs on one shared word lose bits)
+          atomicOr(cluster.map_shared_rank(mask32, c) + 2 * sel + (t >> 5), 1u << (t & 31));
+        }
+      }
+    }
+    cluster.sync();
   }
-  cluster.sync();
 
   const int clusters = gridDim.x / p.cluster, teams = gridDim.x * kTeams;
   const int rounds = ceil_div(p.H, kRound);
@@ -823,12 +840,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int active = s.c.plan[0], U = s.c.plan[1], q = s.c.plan[2];
   const int slices = ceil_div(rounds, q);
 
+  for (int a = tid; a < A; a += kThreads) {
+    const int e = sel_s[a], t = a / p.k;
+    list[s.base[e] + __popcll(s.mask[e] & ((1ull << t) - 1))] = t;
+  }
+  __syncthreads();
   if (blockIdx.x == gridDim.x - 1) {  // (the block that units come to last)
     for (int a = tid; a < A; a += kThreads) {
       const int e = sel_s[a], t = a / p.k;
       p.slot[a] = s.slot[e];
       p.row[a] = s.base[e] + __popcll(s.mask[e] & ((1ull << t) - 1));
-      p.wgt[a] = wgt_s[a];
+      if (!p.sel) p.wgt[a] = wgt_s[a];
     }
     for (int i = tid; i < ceil_div(p.H, kTile); i += kThreads) p.ticket[i] = 0;
     for (int j = tid; j < active; j += kThreads) {
@@ -857,37 +879,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (units > start) total += ceil_div(units - start, group);
   }
   const Active& act = s.c.act;
-  constexpr unsigned kSliced = 1u << 31;  // of Place::b; then the cluster's item << 8
-  auto place = [&](int n) {
-    int item = n * teams + me, sl = 0;
-    unsigned flags = 0;
-    if (n >= waves && slices > 1) {
-      const int i = start + (n - waves) * group, local = i / slices;
-      sl = i - local * slices;
-      item = waves * teams + mine + clusters * local;
-      flags = kSliced | static_cast<unsigned>(local) << 8;
-    }
-    const int e = find_item(act.item, active, item), r = item - act.item[e];
-    const int tiles = ceil_div(act.width[e], tile_outputs(p.act)), pass = r / tiles;
-    Place w(e, r - pass * tiles, sl, pass);
-    w.b |= flags;
-    return w;
-  };
-  auto unit = [&](const Place& w) {
+  auto unit = [&](int n) {
     Unit u;
-    u.set(w, TOK);
-    u.pass = static_cast<int>(w.b & 255) * TOK;
-    u.local = w.b & kSliced ? static_cast<int>(w.b >> 8 & 255) : -1;
-    const int width = act.width[u.e];
-    u.count = min(act.n[u.e] - u.pass, TOK);
-    u.row = act.base[u.e] + u.pass;
+    int item = n * teams + me;
+    u.slice = 0;
+    u.local = -1;
+    if (n >= waves && slices > 1) {
+      const int i = start + (n - waves) * group;
+      u.local = i / slices;
+      u.slice = i - u.local * slices;
+      item = waves * teams + mine + clusters * u.local;
+    }
+    u.e = find_item(act.item, active, item);
+    const int width = act.width[u.e], outputs = tile_outputs(p.act) == 32 ? 5 : 6;
+    const int tiles = (width + (1 << outputs) - 1) >> outputs, r = item - act.item[u.e];
+    const int pass = r / tiles;
+    u.tile = r - pass * tiles;
+    u.count = min(act.n[u.e] - pass * TOK, TOK);
+    u.row = act.base[u.e] + pass * TOK;
     u.begin = u.slice * q * kRound;
     u.strip.end = u.local < 0 ? p.H : min(p.H, u.begin + q * kRound);
     up_strip(u.strip, act.first[u.e], width, p.act, u.tile, p.H, p.shift);
     return u;
   };
   auto source = [&](const Unit& u) {
-    return RowSource<T>{static_cast<const T*>(p.x), p.ldx, s.act_mask[u.e], u.pass};
+    return RowSource<T>{static_cast<const T*>(p.x), p.ldx, list, u.row};
   };
   float* red = reinterpret_cast<float*>(work + kRingBytes<L, NG>) + team * kRedFloats<L, NG>;
   // activated sums of vector tok, from get(tok, column)
@@ -909,7 +925,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   const int vecs = tile_outputs(p.act) / 4;
   const Matrix m{&p.map1, p.w1, p.s1, p.total, p.shift, p.act == ACT_SWIGLU};
-  run_units<L, NG>(total, m, work, red, s.c, place, unit, source, [&](const Unit& u) {
+  run_units<L, NG>(total, m, work, red, s.c, unit, source, [&](const Unit& u) {
     if (u.local < 0) {
       for (int j = tt; j < u.count * vecs; j += kTeamThreads)
         emit(u, j / vecs, 4 * (j % vecs),
@@ -999,20 +1015,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   // neighbouring pieces, and the tiles finish one block after another, so that
   // only the last block's final sums have nothing to overlap.
   const int me = blockIdx.x * kTeams + team, teams = gridDim.x * kTeams;
-  auto place = [&](int n) {
+  auto unit = [&](int n) {
     const int i = me + n * teams;
     const int block = i / (8 * items), r = i - block * 8 * items;
     const int nb = min(8, tiles - 8 * block), it = r / nb;
-    const int e = find_item(act.item, active, it), j = it - act.item[e];
-    const int ns = ceil_div(ceil_div(act.width[e], kRound), q);
-    return Place(e, 8 * block + r % nb, j % ns, j / ns);
-  };
-  auto unit = [&](const Place& w) {
     Unit u;
-    u.set(w, TOK);
-    const int width = act.width[u.e];
-    u.count = min(act.n[u.e] - u.pass, TOK);
-    u.row = act.base[u.e] + u.pass;
+    u.e = find_item(act.item, active, it);
+    const int width = act.width[u.e], j = it - act.item[u.e];
+    const int ns = ceil_div(ceil_div(width, kRound), q), pass = j / ns;
+    u.tile = 8 * block + r - it * nb;
+    u.slice = j - pass * ns;
+    u.local = -1;
+    u.count = min(act.n[u.e] - pass * TOK, TOK);
+    u.row = act.base[u.e] + pass * TOK;
     u.begin = u.slice * q * kRound;
     u.strip.end = min(width, u.begin + q * kRound);
     down_strip(u.strip, act, u.e, act.first[u.e] / gated, u.tile, p.H, p.shift);
@@ -1028,8 +1043,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int share = p.T == 1 ? 8 : p.T == 2 ? 4 : p.T <= 4 ? 2 : 1;
   const Matrix m{&p.map2, p.w2, p.s2, p.H, p.shift, 0};
   run_units<L, NG>(
-      items * tiles > me ? ceil_div(items * tiles - me, teams) : 0, m, work, red, s, place, unit,
-      source, [&](const Unit& u) {
+      items * tiles > me ? ceil_div(items * tiles - me, teams) : 0, m, work, red, s, unit, source,
+      [&](const Unit& u) {
         const int cols = p.H - u.tile * kTile;
         float* y = p.y + u.tile * kTile;
         // (with the remainders' columns, see HiddenSource)
@@ -1291,19 +1306,19 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int team = wid / kTeam, tt = tid % kTeamThreads;
   const int me = blockIdx.x * kTeams + team, units = s.c.plan[1];
-  auto place = [&](int n) {
+  auto unit = [&](int n) {
     const int i = me + n * teams;
-    const int e = find_item(act.item, active, i), r = i - act.item[e], width = act.width[e];
-    const int tiles = p.down ? ceil_div(p.H, kTile) : ceil_div(width, outputs);
-    const int ns = ceil_div(ceil_div(p.down ? width : p.H, kRound), q);
-    return Place(e, r % tiles, r / tiles % ns, r / tiles / ns);
-  };
-  auto unit = [&](const Place& w) {
     Unit u;
-    u.set(w, TOK);
+    u.e = find_item(act.item, active, i);
     const int width = act.width[u.e], k_rows = p.down ? width : p.H;
-    u.count = min(act.n[u.e] - u.pass, TOK);
-    u.row = act.base[u.e] + u.pass;
+    const int tiles = p.down ? ceil_div(p.H, kTile) : ceil_div(width, outputs);
+    const int ns = ceil_div(ceil_div(k_rows, kRound), q), r = i - act.item[u.e];
+    const int j = r / tiles, pass = j / ns;
+    u.tile = r - j * tiles;
+    u.slice = j - pass * ns;
+    u.local = -1;
+    u.count = min(act.n[u.e] - pass * TOK, TOK);
+    u.row = act.base[u.e] + pass * TOK;
     u.begin = u.slice * q * kRound;
     u.strip.end = min(k_rows, u.begin + q * kRound);
     if (p.down)
@@ -1313,12 +1328,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     return u;
   };
   auto source = [&](const Unit& u) {
-    return RowSource<T>{static_cast<const T*>(p.x), p.ldx, 0ull, u.row};
+    return RowSource<T>{static_cast<const T*>(p.x), p.ldx, nullptr, u.row};
   };
   float* red = reinterpret_cast<float*>(work + kRingBytes<L, NG>) + team * kRedFloats<L, NG>;
   const Matrix m{nullptr, p.w, p.s, p.down ? p.H : p.total, p.shift, p.act == ACT_SWIGLU};
-  run_units<L, NG>(units > me ? ceil_div(units - me, teams) : 0, m, work, red, s.c, place, unit,
-                   source, [&](const Unit& u) {
+  run_units<L, NG>(units > me ? ceil_div(units - me, teams) : 0, m, work, red, s.c, unit, source,
+                   [&](const Unit& u) {
                      float* dst = p.part +
                                   (static_cast<long long>(u.slice) * p.rows + u.row) * p.ldp +
                                   u.tile * kTile;
@@ -1386,7 +1401,7 @@ __global__ void __launch_bounds__(kThreads)
 long long align_up(long long v, long long a) { return (v + a - 1) / a * a; }
 
 struct LayerPlan {
-  long long plan, slot, row, wgt, ticket, u, h, y, bytes;
+  long long plan, slot, row, wgt, ticket, sel, u, h, y, bytes;
   long long ldu;
   int slices;
 };
@@ -1419,6 +1434,7 @@ LayerPlan layer_plan(int T, int H, int k, int max_width, int act) {
   p.row = take(4 * A);
   p.wgt = take(4 * A);
   p.ticket = take(4ll * ceil_div(H, kTile));
+  p.sel = take(4 * A);
   p.u = take(4 * p.slices * A * p.ldu);
   p.h = take(4 * A * max_width);  // two 16-bit values or one fp32
   p.y = take(4 * p.slices * A * H);
@@ -1519,12 +1535,16 @@ int launch_layer(LayerParams& p, cudaStream_t st) {
   if (!allow_smem(up, up_ok, dev) || !allow_smem(down, down_ok, dev)) return kStatusCuda;
   const int lde = ceil_div(p.E, 16) * 16, tiles = lde / 16, A = p.T * p.k;
   const int ksub = kWarps / tiles > 1 ? kWarps / tiles : 1;
-  const size_t route = sizeof(float) * (1 + ksub) * p.T * lde, work = kWorkBytes<L, NG>;
+  const size_t route = p.T > kAddTokens ? 0 : sizeof(float) * (1 + ksub) * p.T * lde;
+  const size_t work = kWorkBytes<L, NG>;
   p.smem_work = static_cast<int>(route > work ? route : work);
-  const size_t up_smem = p.smem_work + sizeof(UpSmem) + 8 * A;
+  const size_t up_smem = p.smem_work + sizeof(UpSmem) + 12 * A;
   const size_t down_smem = work + sizeof(Common) + 12 * A;
   if (up_smem > kSmemMax || down_smem > kSmemMax) return kStatusUnsupported;
-  p.cluster = cluster_size(static_cast<long long>(p.E) * p.H * sizeof(typename L::Elem));
+  using T = typename L::Elem;
+  const bool router = p.T > kAddTokens;
+  if (!router) p.sel = nullptr;
+  p.cluster = router ? 1 : cluster_size(static_cast<long long>(p.E) * p.H * sizeof(T));
   const int n = resident_ctas(up, &resident[dev][p.cluster], p.cluster), sms = num_sms();
   if (n < 1) return kStatusCuda;
   p.down_teams = sms * kTeams;
@@ -1537,11 +1557,23 @@ int launch_layer(LayerParams& p, cudaStream_t st) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
+  cfg.stream = st;
+  cfg.attrs = attr;
+  if (router) {
+    static std::atomic<unsigned long long> router_ok{0};
+    auto* kernel = few_router_kernel<T>;
+    if (!allow_smem(kernel, router_ok, dev)) return kStatusCuda;
+    attr[1].val.clusterDim.x = kMaxCluster;
+    cfg.gridDim = dim3(static_cast<unsigned>(ceil_div(p.T, kMaxCluster) * kMaxCluster));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = sizeof(float) * (1 + ksub) * kMaxCluster * lde;
+    cfg.numAttrs = 2;
+    if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) return kStatusCuda;
+    attr[1].val.clusterDim.x = 1;
+  }
   cfg.gridDim = dim3(static_cast<unsigned>(n));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = up_smem;
-  cfg.stream = st;
-  cfg.attrs = attr;
   cfg.numAttrs = 2;
   if (cudaLaunchKernelEx(&cfg, up, p) != cudaSuccess) return kStatusCuda;
   cfg.numAttrs = 1;
@@ -1640,6 +1672,7 @@ int few_tokens(const void* x, long long T, long long ldx, long long H, const voi
   p.shift = shift;
   p.blocks2 = static_cast<int>(blocks2); p.groups2 = static_cast<int>(groups2);
   p.out = out; p.ldo = ldo;
+  p.sel = reinterpret_cast<int*>(b + plan.sel);
   p.plan = reinterpret_cast<int*>(b + plan.plan);
   p.slot = reinterpret_cast<int*>(b + plan.slot);
   p.row = reinterpret_cast<int*>(b + plan.row);

@@ -177,44 +177,23 @@ __device__ __forceinline__ float act_gated(float gate, float up) {
 
 // ------------------------------------------------------------ token vectors
 // The multiplied vectors.  A warp's lane g = lane / 4 holds rows g, g + 8, ..;
-// rows past the count are zero (never read), so nothing beyond a vector enters a
-// sum.
+// lanes past the count repeat the last row (their columns of the product are not
+// used), and elements past the reduction's end are zero (never read), so nothing
+// beyond a vector enters a sum.
 
-// Index of the n-th (from 0) set bit, by halves.
-__device__ __forceinline__ int nth_bit(unsigned long long mask, int n) {
-  unsigned m = static_cast<unsigned>(mask);
-  int at = 0;
-  const int low = __popc(m);
-  if (n >= low) {
-    n -= low;
-    m = static_cast<unsigned>(mask >> 32);
-    at = 32;
-  }
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) {
-    const int c = __popc(m & ((1u << s) - 1));
-    if (n >= c) {
-      n -= c;
-      m >>= s;
-      at += s;
-    }
-  }
-  return at;
-}
-
-// Rows of a matrix of the storage type: the layer's tokens (the set bits of a
-// mask), or the rows of a grouped product.
+// Rows of a matrix of the storage type: the layer's tokens (through the list of the
+// tokens of the expert-sorted rows), or the rows of a grouped product.
 template <typename T>
 struct RowSource {
   static constexpr int kParts = 1;  // 16-bit operands per value
+  static constexpr int half = 0;
   const T* x;
   long long ld;
-  unsigned long long mask;  // 0: rows first, first + 1, ..
+  const int* list;  // null: rows first, first + 1, ..
   int first;
   __device__ __forceinline__ const T* row(int i) const {
-    return x + static_cast<long long>(mask ? nth_bit(mask, first + i) : first + i) * ld;
+    return x + static_cast<long long>(list ? list[first + i] : first + i) * ld;
   }
-  static constexpr int half = 0;
 };
 
 // The layer's intermediate, already activated.  For 16-bit weights each fp32
@@ -291,6 +270,8 @@ template <typename T>
 struct Dense16 {
   using Elem = T;
   static constexpr int kStep = 32;
+  static constexpr bool kGroups = true;  // vectors in groups of 8 columns, of which a unit
+                                         // may have fewer
   static constexpr int kStage = 4096;  // bytes of a step in the ring
   template <int NG>
   static constexpr int kDepth = 2;     // steps in the ring
@@ -333,35 +314,39 @@ struct Dense16 {
   // The vectors' elements of half h (16 rows) of a step.
   template <int NG, typename Src>
   struct Vectors {
-    const T* r[NG];
+    const T* r[NG];  // at the step's first row
     uint2 b[2][NG][Src::kParts];
-    __device__ __forceinline__ void rows(const Src& src, int count, int lane) {
+    template <int G, int P>
+    __device__ __forceinline__ void rows(const Src& src, int count, int k, int lane) {
       const int g = lane >> 2;
 #pragma unroll
-      for (int n = 0; n < NG; ++n)
-        r[n] = 8 * n + g < count ? src.row(8 * n + g) + 4 * (lane & 3) : nullptr;
-      if (Src::kParts == 2 && count <= 4)
-        r[0] = (g & 3) < count ? src.row(g & 3) + (g & 4 ? src.half : 0) + 4 * (lane & 3) : nullptr;
+      for (int n = 0; n < G; ++n) r[n] = src.row(min(8 * n + g, count - 1)) + 4 * (lane & 3) + k;
+      if (Src::kParts == 2 && P == 1)
+        r[0] = src.row(min(g & 3, count - 1)) + (g & 4 ? src.half : 0) + 4 * (lane & 3) + k;
     }
     template <int G, int P>
-    __device__ __forceinline__ void load(int h, const Src& src, int end, int k, int lane) {
+    __device__ __forceinline__ void load(int h, const Src& src, int left, int lane) {
+      if (16 * h >= left) return;
 #pragma unroll
       for (int n = 0; n < G; ++n)
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-          uint2 v = make_uint2(0u, 0u);
-          if (r[n] && k + 16 * h < end)
-            v = *reinterpret_cast<const uint2*>(r[n] + p * src.half + k + 16 * h);
+          const uint2 v = *reinterpret_cast<const uint2*>(r[n] + p * src.half + 16 * h);
           b[h][n][p] = (lane & 2) ? make_uint2(v.y, v.x) : v;
         }
+    }
+    template <int G>
+    __device__ __forceinline__ void advance(int rows) {
+#pragma unroll
+      for (int n = 0; n < G; ++n) r[n] += rows;
     }
   };
   // One half of a step for the first G groups of vectors and P of their parts.
   template <int G, int P, int NG, typename Src>
   static __device__ __forceinline__ void half(int h, float (&acc)[4][NG][4], const Lane& l,
-                                              const Matrix&, int end, int k, uint32_t stage, int,
+                                              const Matrix&, int left, uint32_t stage, int,
                                               const Vectors<NG, Src>& v) {
-    if (h && k + 16 >= end) return;  // rows beyond are another expert's
+    if (16 * h >= left) return;  // rows beyond are another expert's
     uint32_t a[4][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) ldsm_trans(a[i], stage + h * l.half + l.off[i]);
@@ -373,11 +358,11 @@ struct Dense16 {
         for (int i = 0; i < 4; ++i) mma<T>(acc[i][n], a[i], v.b[h][n][p].x, v.b[h][n][p].y);
   }
   // The lane's sums to (ADD: added to) red[token][64 columns], row stride LD.
-  template <int NG, int LD, bool ADD>
+  template <int G, int NG, int LD, bool ADD>
   static __device__ __forceinline__ void store(const float (&acc)[4][NG][4], int lane, float* red) {
     const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int n = 0; n < NG; ++n)
+    for (int n = 0; n < G; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -409,9 +394,10 @@ template <typename T>
 struct Int4 {
   using Elem = T;
   static constexpr int kStep = 64;
+  static constexpr bool kGroups = true;
   static constexpr int kStage = 2048 + 2 * 128;  // weights, then scales of two groups
   template <int NG>
-  static constexpr int kDepth = 4;
+  static constexpr int kDepth = NG == 1 ? 4 : 3;
   template <int NG>
   static constexpr int kTokens = 8 * NG;
   struct Lane {
@@ -465,26 +451,33 @@ struct Int4 {
   // The vectors' elements of half h (32 rows) of a step.
   template <int NG, typename Src>
   struct Vectors {
-    const T* r[NG];
+    const T* r[NG];  // at the step's first row
     uint4 b[2][NG][Src::kParts];
-    __device__ __forceinline__ void rows(const Src& src, int count, int lane) {
+    template <int G, int P>
+    __device__ __forceinline__ void rows(const Src& src, int count, int k, int lane) {
       const int g = lane >> 2;
 #pragma unroll
-      for (int n = 0; n < NG; ++n)
-        r[n] = 8 * n + g < count ? src.row(8 * n + g) + 8 * (lane & 3) : nullptr;
-      if (Src::kParts == 2 && count <= 4)
-        r[0] = (g & 3) < count ? src.row(g & 3) + (g & 4 ? src.half : 0) + 8 * (lane & 3) : nullptr;
+      for (int n = 0; n < G; ++n) r[n] = src.row(min(8 * n + g, count - 1)) + 8 * (lane & 3) + k;
+      if (Src::kParts == 2 && P == 1)
+        r[0] = src.row(min(g & 3, count - 1)) + (g & 4 ? src.half : 0) + 8 * (lane & 3) + k;
     }
     template <int G, int P>
-    __device__ __forceinline__ void load(int h, const Src& src, int end, int k, int lane) {
+    __device__ __forceinline__ void load(int h, const Src& src, int left, int lane) {
+      const bool whole = 32 * h + 32 <= left;  // else the weights end inside: 16 rows
+      if (32 * h >= left) return;
 #pragma unroll
       for (int n = 0; n < G; ++n)
 #pragma unroll
         for (int p = 0; p < P; ++p) {
           b[h][n][p] = make_uint4(0, 0, 0, 0);
-          if (r[n] && k + 32 * h + 8 * (lane & 3) < end)
-            b[h][n][p] = *reinterpret_cast<const uint4*>(r[n] + p * src.half + k + 32 * h);
+          if (whole || 32 * h + 8 * (lane & 3) < left)
+            b[h][n][p] = *reinterpret_cast<const uint4*>(r[n] + p * src.half + 32 * h);
         }
+    }
+    template <int G>
+    __device__ __forceinline__ void advance(int rows) {
+#pragma unroll
+      for (int n = 0; n < G; ++n) r[n] += rows;
     }
   };
   // codes j of w as B + 8 q, and the operand of -(B + 64)
@@ -498,9 +491,9 @@ struct Int4 {
   // One half of a step for the first G groups of vectors and P of their parts.
   template <int G, int P, int NG, typename Src>
   static __device__ __forceinline__ void half(int h, float (&acc)[4][NG][4], const Lane&,
-                                              const Matrix& m, int end, int k, uint32_t stage,
+                                              const Matrix& m, int left, uint32_t stage,
                                               int lane, const Vectors<NG, Src>& v) {
-    if (h && k + 32 >= end) return;
+    if (32 * h >= left) return;
     float minus[G][4] = {};
     const uint32_t minus_op[4] = {kMinus, kMinus, kMinus, kMinus};
     const uint32_t scales = stage + 2048 + 4 * (lane >> 2) + (h && m.shift == 5 ? 128 : 0);
@@ -550,11 +543,11 @@ struct Int4 {
       }
     }
   }
-  template <int NG, int LD, bool ADD>
+  template <int G, int NG, int LD, bool ADD>
   static __device__ __forceinline__ void store(const float (&acc)[4][NG][4], int lane, float* red) {
     const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int n = 0; n < NG; ++n)
+    for (int n = 0; n < G; ++n)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         float* p = red + (8 * n + 2 * t + j) * LD + 2 * g;
@@ -580,6 +573,7 @@ struct Int4 {
 struct Dense32 {
   using Elem = float;
   static constexpr int kStep = 16;
+  static constexpr bool kGroups = false;
   static constexpr int kStage = 4096;
   template <int NG>
   static constexpr int kDepth = 2;
@@ -613,21 +607,27 @@ struct Dense32 {
   };
   template <int NG, typename Src>
   struct Vectors {
-    const float* r[4 * NG];
-    __device__ __forceinline__ void rows(const Src& src, int count, int) {
+    const float* r[4 * NG];  // at this half-warp's first row
+    template <int G, int P>
+    __device__ __forceinline__ void rows(const Src& src, int count, int k, int lane) {
 #pragma unroll
-      for (int t = 0; t < 4 * NG; ++t) r[t] = t < count ? src.row(t) : nullptr;
+      for (int t = 0; t < 4 * NG; ++t) r[t] = t < count ? src.row(t) + k + 8 * (lane >> 4) : nullptr;
     }
     template <int G, int P>
-    __device__ __forceinline__ void load(int, const Src&, int, int, int) {}
+    __device__ __forceinline__ void load(int, const Src&, int, int) {}
+    template <int G>
+    __device__ __forceinline__ void advance(int rows) {
+#pragma unroll
+      for (int t = 0; t < 4 * NG; ++t)
+        if (r[t]) r[t] += rows;
+    }
   };
   // One half of a step for the first G groups of vectors and P of their parts.
   template <int G, int P, int NG, typename Src>
   static __device__ __forceinline__ void half(int h, float (&acc)[4][NG][4], const Lane& l,
-                                              const Matrix&, int end, int k0, uint32_t stage,
+                                              const Matrix&, int left, uint32_t stage,
                                               int lane, const Vectors<NG, Src>& v) {
-    const int k = k0 + 8 * (lane >> 4);
-    if (h || k >= end) return;  // (one part: all 16 rows)
+    if (h || 8 * (lane >> 4) >= left) return;  // (one part: all 16 rows)
     float4 w[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -637,7 +637,7 @@ struct Dense32 {
 #pragma unroll
     for (int t = 0; t < 4 * NG; ++t) {
       if (v.r[t]) {
-        const float* x = v.r[t] + k;
+        const float* x = v.r[t];
         const float4 x0 = *reinterpret_cast<const float4*>(x);
         const float4 x1 = *reinterpret_cast<const float4*>(x + 4);
         const float xs[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
@@ -652,7 +652,7 @@ struct Dense32 {
       }
     }
   }
-  template <int NG, int LD, bool ADD>
+  template <int G, int NG, int LD, bool ADD>
   static __device__ __forceinline__ void store(const float (&acc)[4][NG][4], int lane, float* red) {
 #pragma unroll
     for (int t = 0; t < 4 * NG; ++t) {
