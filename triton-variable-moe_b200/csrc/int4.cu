@@ -15,13 +15,14 @@
 // product loads its fragments as they lie, 512 contiguous bytes a warp, and gets the
 // codes to the top of 16-bit mantissas by rotating (few_tokens.cuh).
 //
-// All three are one pass over memory (2.5 bytes a weight at 16 bits) and HBM
-// bound: a CTA takes 128 rows x 64 columns, 16 KB in flight in four vectors a
-// thread, transposes through shared memory (row stride 33 words: conflict free)
-// and writes one 16-byte vector a thread.
+// All three are one pass over memory (2.5 bytes a weight at 16 bits) and HBM bound.
+// A CTA takes 128 rows x 64 columns.  Quantising, a thread holds 4 rows x 8 columns
+// (four 16-byte loads, 16 KB in flight a CTA), which are exactly four words of the
+// packed layout; only the group maxima and the finished words go through shared memory.
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "few_tokens.cuh"
 #include "moe_internal.h"
@@ -70,15 +71,29 @@ __device__ __forceinline__ uint32_t place(uint32_t code, int i, int c) {
   return __funnelshift_l(code, code, bit(i, c));
 }
 
-// The integer nearest to w / s, ties to even, exactly: the quotient's own
-// rounding is undone by the remainder, which fp32 holds without error.
-__device__ __forceinline__ int nearest(float w, float s) {
-  float q = rintf(w / s);
-  const float r = fmaf(-q, s, w), half = 0.5f * s;
-  const bool odd = (static_cast<int>(q) & 1) != 0;
-  if (r > half || (r == half && odd)) q += 1.f;
-  if (r < -half || (r == -half && odd)) q -= 1.f;
-  return static_cast<int>(fminf(fmaxf(q, -8.f), 7.f));
+// The integer nearest to w / s, ties to even, exactly: the quotient's own rounding (w / s,
+// or w times the rounded reciprocal: off by less than one either way) is undone by the
+// remainder, which fp32 holds without error.
+__device__ __forceinline__ uint32_t exact_code(float w, float s, float quotient) {
+  const float magic = 12582912.f;  // 1.5 x 2^23: adding it rounds to integers
+  float q = (quotient + magic) - magic;
+  const float r = fabsf(fmaf(-q, s, w)), half = 0.5f * s;
+  const float sign = fmaf(-q, s, w) < 0.f ? -1.f : 1.f;
+  const bool odd = (__float_as_uint(q + magic) & 1u) != 0;
+  if (r > half || (r == half && odd)) q += sign;
+  return __float_as_uint(fminf(fmaxf(q, -8.f), 7.f) + (magic + 8.f)) & 15u;
+}
+
+// The same for weights and scales of 16 bits, from the reciprocal of the scale.  Both
+// have at most 11 significant bits, so a quotient is either halfway between integers
+// or at least 2^-12 from it; w * inv is within 2^-19 of the quotient; rounding it to
+// steps of 2^-13 first therefore gives halfway exactly when it is, and the second
+// rounding sends that to even.  Returns the clamped q - 8 as the low bits' code.
+__device__ __forceinline__ uint32_t nearest_code(float w, float inv) {
+  const float step = 1536.f;  // 1.5 x 2^10: the sum's last place is 2^-13
+  float t = fmaf(w, inv, step) - step;
+  t = fminf(fmaxf(t, -8.f), 7.f);
+  return __float_as_uint(t + 12582920.f) & 15u;  // 1.5 x 2^23 + 8
 }
 
 // rows x 64 columns of a row-major matrix into shared memory, zeros beyond.
@@ -103,60 +118,112 @@ __device__ __forceinline__ void load_tile(const T* w, long long ld, int row, int
   }
 }
 
+// 8 values of a row as floats.
+template <typename T>
+struct Eight {
+  uint4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p, bool ok) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
+      v[i] = ok ? few::ld_stream(p + 16 / sizeof(T) * i) : make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ float get(int i) const {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+    const float2 f = few::unpack2<std::conditional_t<sizeof(T) == 4, __half, T>>(w[i / 2]);
+    return i & 1 ? f.y : f.x;
+  }
+};
+
 // T: type of the weights, S: type of the scales.
 template <typename T, typename S>
 __global__ void __launch_bounds__(kThreadsQ)
     quantize_kernel(const T* __restrict__ w, long long ld, int N, const Segments seg, int shift,
                     uint4* __restrict__ packed, S* __restrict__ scales) {
-  __shared__ __align__(16) T tile[kRows * kLd];
+  __shared__ __align__(16) uint32_t words[2 * 4 * 32 * 4];
   __shared__ unsigned amax[4][kCols];  // of 32 rows each
-  __shared__ float sc[4][kCols];
-  const int tid = threadIdx.x;
+  __shared__ __align__(16) float scale[4][kCols], inverse[4][kCols];
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const Where at = locate(seg, blockIdx.x, shift);
   const int col = blockIdx.y * kCols, cols = min(kCols, N - col);
-  load_tile(w, ld, at.row, at.rows, col, cols, tile);
-  __syncthreads();
-  {
-    const int c = tid % kCols, part = tid / kCols;
-    unsigned m = 0;  // order of the bits of |w|: a NaN above all
-    for (int r = 0; r < 32; ++r)
-      m = max(m, __float_as_uint(to_f<T>(tile[(32 * part + r) * kLd + c])) & 0x7fffffffu);
-    amax[part][c] = m;
-  }
-  __syncthreads();
-  {
-    const int c = tid % kCols, part = tid / kCols, per = 1 << (shift - 5);
-    const int first = part / per * per;
-    unsigned m = amax[first][c];
-    for (int i = 1; i < per; ++i) m = max(m, amax[first + i][c]);
-    const S s = from_f<S>(__uint_as_float(m) / 7.f);
-    sc[part][c] = to_f<S>(s);
-    if (part == first && 32 * first < at.rows && c < cols)
-      scales[static_cast<long long>(at.group + part / per) * N + col + c] = s;
-  }
-  __syncthreads();
-  // thread = (block row, block column, lane)
-  const int lane = tid & 31, nb = (tid >> 5) & 3, kb = tid >> 7;
-  const int g = lane >> 2, t = lane & 3;
-  if (16 * nb >= cols || 64 * kb >= at.rows) return;
-  uint4 out;
-  uint32_t* word = reinterpret_cast<uint32_t*>(&out);
+  // warp: 32 rows (part) x 32 columns; lane: rows 4 r .. + 3, columns c .. c + 7
+  const int part = wid & 3, r = lane >> 2, c = 32 * (wid >> 2) + 8 * (lane & 3);
+  Eight<T> v[4];
 #pragma unroll
-  for (int s = 0; s < 4; ++s) {
-    const int r0 = 64 * kb + 32 * (s >> 1) + 8 * t + 4 * (s & 1);
-    uint32_t v = 0;
+  for (int i = 0; i < 4; ++i) {
+    const int row = 32 * part + 4 * r + i;
+    v[i].load(w + static_cast<long long>(at.row + row) * ld + col + c, row < at.rows && c < cols);
+  }
+  {
+    unsigned m[8];  // order of the bits of |w|: a NaN above all
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      m[j] = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m[j] = max(m[j], __float_as_uint(v[i].get(j)) & 0x7fffffffu);
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) m[j] = max(m[j], __shfl_xor_sync(0xffffffffu, m[j], o));
+    }
+    unsigned mine = m[0];  // lane r keeps column c + r
+#pragma unroll
+    for (int j = 1; j < 8; ++j) mine = r == j ? m[j] : mine;
+    amax[part][c + r] = mine;
+  }
+  __syncthreads();
+  {
+    const int cc = tid % kCols, pt = tid / kCols, per = 1 << (shift - 5);
+    const int first = pt / per * per;
+    unsigned m = amax[first][cc];
+    for (int i = 1; i < per; ++i) m = max(m, amax[first + i][cc]);
+    const S s = from_f<S>(__uint_as_float(m) / 7.f);
+    const float f = to_f<S>(s);
+    scale[pt][cc] = f;
+    // 0: not finite, zero, or below 2^-100
+    inverse[pt][cc] = f >= 7.8886091e-31f && f <= 3.4028234e38f ? 1.f / f : 0.f;
+    if (pt == first && 32 * first < at.rows && cc < cols)
+      scales[static_cast<long long>(at.group + pt / per) * N + col + cc] = s;
+  }
+  __syncthreads();
+  float inv[8];
+  *reinterpret_cast<float4*>(inv) = *reinterpret_cast<const float4*>(&inverse[part][c]);
+  *reinterpret_cast<float4*>(inv + 4) = *reinterpret_cast<const float4*>(&inverse[part][c + 4]);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {  // columns c + 2 j, + 1: lane (g, t) of a block
+    uint32_t word = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int cc = 16 * nb + 2 * g + c;
-        const float x = to_f<T>(tile[(r0 + i) * kLd + cc]), q = sc[(r0 + i) >> 5][cc];
-        const int code = q > 0.f && q <= 3.4028234e38f ? nearest(x, q) + 8 : 8;
-        v |= place(code, i, c);
+      for (int x = 0; x < 2; ++x) {
+        uint32_t code;
+        const float value = v[i].get(2 * j + x), f = inv[2 * j + x];
+        if constexpr (sizeof(T) == 4)
+          code = exact_code(value, scale[part][c + 2 * j + x], value * f);
+        else
+          code = nearest_code(value, f);
+        word |= place(code, i, x);
       }
-    word[s] = v;
+    if (inv[2 * j] == 0.f || inv[2 * j + 1] == 0.f) {  // a scale without its reciprocal
+      word = 0;
+#pragma unroll 1
+      for (int k = 0; k < 8; ++k) {
+        const float f = scale[part][c + 2 * j + (k & 1)];
+        float value = 0.f;
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
+          if (n == k) value = v[n >> 1].get(2 * j + (n & 1));
+        const uint32_t code = f > 0.f && f <= 3.4028234e38f ? exact_code(value, f, value / f) : 8u;
+        word |= place(code, k >> 1, k & 1);
+      }
+    }
+    const int nb = c / 16, g = c % 16 / 2 + j, t = r >> 1, h = part & 1, kb = part >> 1;
+    words[((kb * 4 + nb) * 32 + 4 * g + t) * 4 + 2 * h + (r & 1)] = word;
   }
-  packed[(static_cast<long long>(at.block + kb) * (N / 16) + col / 16 + nb) * 32 + lane] = out;
+  __syncthreads();
+  // thread = (block row, block column, lane)
+  const int nb = wid & 3, kb = wid >> 2;
+  if (16 * nb >= cols || 64 * kb >= at.rows) return;
+  packed[(static_cast<long long>(at.block + kb) * (N / 16) + col / 16 + nb) * 32 + lane] =
+      reinterpret_cast<const uint4*>(words)[tid];
 }
 
 // Codes 0..15, one a byte, to the packed layout (rows beyond a segment: 8).
@@ -194,51 +261,53 @@ template <typename S>
 __global__ void __launch_bounds__(kThreadsQ)
     dequantize_kernel(const uint4* __restrict__ packed, const S* __restrict__ scales, int N,
                       const Segments seg, int shift, S* __restrict__ out, long long ld) {
-  __shared__ __align__(16) S tile[kRows * kLd];
+  // rows of 128 bytes, 16-byte chunks exchanged by row so that neither side conflicts
+  __shared__ __align__(16) uint32_t tile[kRows * kCols / 2];
   const int tid = threadIdx.x;
   const Where at = locate(seg, blockIdx.x, shift);
   const int col = blockIdx.y * kCols, cols = min(kCols, N - col);
   const int lane = tid & 31, nb = (tid >> 5) & 3, kb = tid >> 7;
   const int g = lane >> 2, t = lane & 3;
+  auto chunk = [](int row, int c) { return c ^ ((row >> 3 & 3) << 1); };
   if (16 * nb < cols && 64 * kb < at.rows) {
     const uint4 v = few::ld_stream(
         packed + (static_cast<long long>(at.block + kb) * (N / 16) + col / 16 + nb) * 32 + lane);
     const uint32_t* word = reinterpret_cast<const uint32_t*>(&v);
-    float s2[2][2];  // of each 32-row half, each column
+    float2 s2[2];  // of each 32-row half
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int r = 64 * kb + 32 * h;
-        s2[h][c] = r < at.rows ? to_f<S>(scales[static_cast<long long>(at.group + (r >> shift)) * N +
-                                               col + 16 * nb + 2 * g + c])
-                               : 0.f;
-      }
+    for (int h = 0; h < 2; ++h) {
+      const int r = 64 * kb + 32 * h;
+      const uint32_t two =
+          r < at.rows ? *reinterpret_cast<const uint32_t*>(
+                            scales + static_cast<long long>(at.group + (r >> shift)) * N + col +
+                            16 * nb + 2 * g)
+                      : 0u;
+      s2[h] = few::unpack2<S>(two);
+    }
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const int r0 = 64 * kb + 32 * (s >> 1) + 8 * t + 4 * (s & 1);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i) {
+        float q[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const int q = static_cast<int>(__funnelshift_r(word[s], word[s], bit(i, c)) & 15u) - 8;
-          tile[(r0 + i) * kLd + 16 * nb + 2 * g + c] =
-              from_f<S>(static_cast<float>(q) * s2[s >> 1][c]);
+          const uint32_t code = __funnelshift_r(word[s], word[s], bit(i, c)) & 15u;
+          q[c] = __uint_as_float(0x4b000000u | code) - 8388616.f;  // 2^23 + code, - 8
         }
+        tile[(r0 + i) * 32 + 4 * chunk(r0 + i, 2 * nb + (g >> 2)) + (g & 3)] =
+            few::pack2<S>(q[0] * s2[s >> 1].x, q[1] * s2[s >> 1].y);
+      }
     }
   }
   __syncthreads();
-  constexpr int V = 8, PER = kCols / V;
+  constexpr int PER = kCols / 8;
 #pragma unroll
   for (int j = 0; j < kRows * PER / kThreadsQ; ++j) {
-    const int i = tid + j * kThreadsQ, r = i / PER, c = V * (i % PER);
-    if (r < at.rows && c < cols) {
-      uint4 v;
-      S* e = reinterpret_cast<S*>(&v);
-#pragma unroll
-      for (int x = 0; x < V; ++x) e[x] = tile[r * kLd + c + x];
-      *reinterpret_cast<uint4*>(out + static_cast<long long>(at.row + r) * ld + col + c) = v;
-    }
+    const int i = tid + j * kThreadsQ, r = i / PER, c = i % PER;
+    if (r < at.rows && 8 * c < cols)
+      *reinterpret_cast<uint4*>(out + static_cast<long long>(at.row + r) * ld + col + 8 * c) =
+          reinterpret_cast<const uint4*>(tile)[r * PER + chunk(r, c)];
   }
 }
 
@@ -329,7 +398,8 @@ int int4_dequantize(const void* packed, const void* scales, long long K, long lo
   Segments s;
   const int shift = shift_of(group);
   if (!packed || !scales || !out || shift == 0 || !make_segments(off, n, K, group, s) ||
-      !sizes_ok(s, N) || ld < N || ld % 8 != 0 || !aligned(packed) || !aligned(out))
+      !sizes_ok(s, N) || ld < N || ld % 8 != 0 || !aligned(packed) || !aligned(scales) ||
+      !aligned(out))
     return kStatusBadArg;
   const dim3 grid(static_cast<unsigned>(s.chunk[s.n]), static_cast<unsigned>((N + kCols - 1) / kCols));
   const uint4* in = static_cast<const uint4*>(packed);
