@@ -243,6 +243,7 @@ __device__ __forceinline__ void run_units(int total, const Matrix& m,
   auto nth = [&](int n) { return n < kTable ? c.table[team][n] : unit(n); };
 
   int copied = 0, used = 0;  // steps
+  uint32_t copy_slot = 0, use_slot = 0, phase = 0;
   // the copying side: the team's cn-th unit, next step at row ck
   int cn = -1, ck = 0, cend = 0;
   bool more = true;
@@ -258,8 +259,8 @@ __device__ __forceinline__ void run_units(int total, const Matrix& m,
           if (ck < cend) cursor.set(m, cu.strip, ck);
         }
       } else {
-        const int slot = copied % D;
-        if (lane == 0) cursor.issue(m, ring + slot * L::kStage, bars + 8 * slot);
+        if (lane == 0) cursor.issue(m, ring + copy_slot * L::kStage, bars + 8 * copy_slot);
+        copy_slot = copy_slot + 1 == D ? 0 : copy_slot + 1;
         ++copied;
         ck += kRows;
         cursor.template next<kRows>(m);
@@ -288,16 +289,19 @@ __device__ __forceinline__ void run_units(int total, const Matrix& m,
         v.template load<G, P>(0, src, left, lane);
       }
       for (; left > 0; left -= kRows) {  // the vectors of each half load during the half before
-        const int slot = used % D;
-        const uint32_t stage = ring + slot * L::kStage;
+        const uint32_t stage = ring + use_slot * L::kStage;
         v.template load<G, P>(1, src, left, lane);
-        if (used < copied) ring_wait(bars + 8 * slot, (used / D) & 1, &c.abort);
+        if (used < copied) ring_wait(bars + 8 * use_slot, phase, &c.abort);
         L::template half<G, P, NG, Src>(0, acc, at, m, left, stage, lane, v);
         v.template advance<G>(kRows);
         v.template load<G, P>(0, src, left - kRows, lane);
         L::template half<G, P, NG, Src>(1, acc, at, m, left, stage, lane, v);
         __syncwarp();  // the step has been read by every lane: its place is free
         ++used;
+        if (++use_slot == D) {
+          use_slot = 0;
+          phase ^= 1;
+        }
         top_up();
       }
       // warps 2 and 3 leave their sums, 0 and 1 add theirs to them
@@ -725,7 +729,7 @@ __device__ __forceinline__ void plan_down(const LayerParams& p, const Active& ac
   int widest = 0;
   for (int j = lane; j < active; j += 32) widest = max(widest, act.width[j]);
   widest = __reduce_max_sync(0xffffffffu, widest);
-  const int len = plan_length(max(1, ceil_div(widest, ROUND)), p.down_teams, p.max_slices, 4,
+  const int len = plan_length(max(1, ceil_div(widest, ROUND)), p.down_teams, p.max_slices, 2,
                               [&](int length) {
     int n = 0;
     for (int j = lane; j < active; j += 32)
@@ -1590,9 +1594,11 @@ int launch_layer(LayerParams& p, cudaStream_t st) {
   return cudaPeekAtLastError() == cudaSuccess ? kStatusOk : kStatusCuda;
 }
 
+// 8 or 16 columns of vectors a unit: 16 when an expert has more than about 6 rows on
+// average (each further pass over an expert's weights reads them again, from L2).
 template <typename L>
 int layer_for_tokens(LayerParams& p, cudaStream_t st) {
-  return p.T <= 8 ? launch_layer<L, 1>(p, st) : launch_layer<L, 2>(p, st);
+  return p.T <= 8 || p.T * p.k <= 6 * p.E ? launch_layer<L, 1>(p, st) : launch_layer<L, 2>(p, st);
 }
 
 template <typename L, int NG>
@@ -1735,11 +1741,12 @@ int grouped_int4(const void* x, long long rows, long long ldx, const void* w, co
   p.ldp = padded_columns(down ? H : max_width, act);
   p.max_slices = slice_limit(rows * p.ldp);
   p.out = out; p.ldo = ldo; p.status = status;
+  const bool narrow = rows <= 8 || rows <= 6ll * E;  // as layer_for_tokens
   if (dtype == 0)
-    return rows <= 8 ? launch_group<Int4<__nv_bfloat16>, 1>(p, st)
-                     : launch_group<Int4<__nv_bfloat16>, 2>(p, st);
+    return narrow ? launch_group<Int4<__nv_bfloat16>, 1>(p, st)
+                  : launch_group<Int4<__nv_bfloat16>, 2>(p, st);
   if (dtype == 1)
-    return rows <= 8 ? launch_group<Int4<__half>, 1>(p, st) : launch_group<Int4<__half>, 2>(p, st);
+    return narrow ? launch_group<Int4<__half>, 1>(p, st) : launch_group<Int4<__half>, 2>(p, st);
   return kStatusUnsupported;
 }
 
