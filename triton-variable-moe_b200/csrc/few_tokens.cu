@@ -145,6 +145,19 @@ __device__ __forceinline__ int find_item(const int* item, int n, int i) {
   return lo;
 }
 
+// Counts up; releases what the thread has seen written and acquires what others
+// released, within the cluster (a counter in shared memory) or the GPU.
+__device__ __forceinline__ int count_cluster(int* counter) {
+  int old;
+  asm volatile("atom.acq_rel.cluster.add.u32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
+  return old;
+}
+__device__ __forceinline__ int count_gpu(int* counter) {
+  int old;
+  asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
+  return old;
+}
+
 __device__ __forceinline__ void team_sync(int team) {
   asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(kTeamThreads) : "memory");
 }
@@ -729,7 +742,7 @@ __device__ __forceinline__ void plan_down(const LayerParams& p, const Active& ac
   int widest = 0;
   for (int j = lane; j < active; j += 32) widest = max(widest, act.width[j]);
   widest = __reduce_max_sync(0xffffffffu, widest);
-  const int len = plan_length(max(1, ceil_div(widest, ROUND)), p.down_teams, p.max_slices, 2,
+  const int len = plan_length(max(1, ceil_div(widest, ROUND)), p.down_teams, p.max_slices, p.T <= kAddTokens ? 9 : 4,
                               [&](int length) {
     int n = 0;
     for (int j = lane; j < active; j += 32)
@@ -826,15 +839,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     // Whole items, a wave of them over all teams at a time; the rest whole too, or in
     // slices of a cluster's items over its teams.  Lane l weighs l + 1 slices, in
-    // quarter rounds: a unit's own cost is half a round, a slice's with the joining
-    // another three quarters.
+    // quarter rounds: a unit's own cost is a round, a slice's, with the joining, two.
     const int rest = s.c.plan[1] % teams;
     const int local = ceil_div(rest, clusters), cut = lane + 1;
     int cost = 0x7fffffff;
     if (cut == 1)
-      cost = 4 * rounds + 2;
+      cost = 4 * rounds + 4;
     else if (cut <= min(p.max_slices, rounds))
-      cost = ceil_div(local * cut, p.cluster * kTeams) * (4 * ceil_div(rounds, cut) + 5) + 3;
+      cost = ceil_div(local * cut, p.cluster * kTeams) * (4 * ceil_div(rounds, cut) + 9);
     const int best = __reduce_min_sync(0xffffffffu, cost);
     const int at = __ffs(__ballot_sync(0xffffffffu, cost == best));
     if (lane == 0) s.c.plan[2] = ceil_div(rounds, at);
@@ -945,10 +957,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     team_sync(team);
     if (tt == 0) {
-      __threadfence();  // the team's sums, before the count
+      // (after the team's sums, and before reading the other teams')
       s.c.last[team] =
-          atomicAdd(cluster.map_shared_rank(s.ticket, 0) + u.local, 1) == slices - 1;
-      __threadfence();  // and the other teams' sums, after it
+          count_cluster(cluster.map_shared_rank(s.ticket, 0) + u.local) == slices - 1;
     }
     team_sync(team);
     if (s.c.last[team]) {
@@ -1068,9 +1079,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!add) return;
         team_sync(team);
         if (tt == 0) {
-          __threadfence();  // the team's sums, before the count
-          s.last[team] = atomicAdd(&p.ticket[u.tile], 1) == items - 1;
-          __threadfence();  // and the other teams' sums, after it
+          // (after the team's sums, and before reading the other teams')
+          s.last[team] = count_gpu(&p.ticket[u.tile]) == items - 1;
         }
         team_sync(team);
         if (!s.last[team]) return;
@@ -1273,7 +1283,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int j = lane; j < active; j += 32) widest = max(widest, s.c.act.width[j]);
     widest = __reduce_max_sync(0xffffffffu, widest);
     const int most = max(1, ceil_div(p.down ? widest : p.H, kRound));
-    const int len = plan_length(most, teams, p.max_slices, 2, [&](int length) {
+    const int len = plan_length(most, teams, p.max_slices, 4, [&](int length) {
       int n = 0;
       for (int j = lane; j < active; j += 32) n += units(j, length);
       return static_cast<long long>(__reduce_add_sync(0xffffffffu, n));
