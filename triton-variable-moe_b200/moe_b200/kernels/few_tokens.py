@@ -18,46 +18,64 @@ from __future__ import annotations
 import torch
 
 from .._lib import ACT_CODE, DTYPE_CODE, check, lib
-from ._ops import _count, _ev_begin, _ev_end, _meta, status_buffer
+from . import _ops
+from ._ops import _meta, status_buffer
 from .int4 import Int4Weight, eager_only, on_device, refuse_grad, row_view, stream_of
 
 FEW_TOKENS_MAX = 64
 
-_workspace_bytes: dict[tuple, int] = {}
+# What the sizes and types of a call come to, worked out and checked at the first call
+# with them: (group, blocks, groups, columns of w1, workspace bytes, codes).
+_signatures: dict[tuple, tuple] = {}
 
 
-def _check_weights(x, router, w1, w2, num_experts, hidden, max_width, gated):
-    """(w1 tensor, its scales, w2 tensor, its scales, group, blocks, groups, columns of w1)."""
-    if isinstance(w1, Int4Weight) != isinstance(w2, Int4Weight):
+def _signature(x_shape, dt, router_shape, w1, w2, offsets, max_width, top_k, activation):
+    if len(x_shape) != 2:
+        raise ValueError(f"moe_few_tokens: x must be [tokens, hidden], got {tuple(x_shape)}")
+    T, H = x_shape
+    if T > FEW_TOKENS_MAX:
+        raise ValueError(f"moe_few_tokens: at most {FEW_TOKENS_MAX} tokens, got {T} (use the "
+                         "layer's forward)")
+    if dt not in DTYPE_CODE:
+        raise TypeError(f"moe_few_tokens: bf16, fp16 or fp32, got {dt}")
+    if activation not in ACT_CODE:
+        raise NotImplementedError(f"activation {activation!r} is not supported "
+                                  f"(supported: {tuple(ACT_CODE)})")
+    if len(router_shape) != 2 or router_shape[1] != H:
+        raise ValueError(f"moe_few_tokens: router_weight must be [experts, {H}], got "
+                         f"{tuple(router_shape)}")
+    E = router_shape[0]
+    if not 1 <= E <= 256 or not 1 <= top_k <= min(E, 32):
+        raise ValueError(f"moe_few_tokens: 1 to 256 experts and top_k up to 32 of them, got {E} and "
+                         f"{top_k}")
+    if H % 16 or not 16 <= H <= 32768 or max_width % 16 or not 16 <= max_width <= 32768:
+        raise ValueError("moe_few_tokens: hidden size and expert widths must be multiples of 16 up "
+                         f"to 32768, got {H} and {max_width}")
+    if offsets != E + 1:
+        raise ValueError(f"moe_few_tokens: expert_weight_offsets needs {E + 1} entries, got {offsets}")
+    gated = 2 if activation == "swiglu" else 1
+    packed = isinstance(w1, Int4Weight)
+    if packed != isinstance(w2, Int4Weight):
         raise TypeError("moe_few_tokens: w1 and w2 must both be tensors or both be Int4Weight")
-    dt, dev = x.dtype, x.device
-    if router.dtype != dt or w1.dtype != dt or w2.dtype != dt:
-        raise TypeError(f"moe_few_tokens: x, router_weight, w1 and w2 must share a dtype, got {dt}, "
-                        f"{router.dtype}, {w1.dtype} and {w2.dtype}")
-    if router.device != dev or w1.device != dev or w2.device != dev:
-        raise ValueError("moe_few_tokens: all tensors must be on one device")
-    if len(w1.shape) != 2 or w1.shape[0] != hidden or w1.shape[1] % (16 * gated) or w1.shape[1] < 16:
-        raise ValueError(f"moe_few_tokens: w1 must be [{hidden}, total width in multiples of "
+    if len(w1.shape) != 2 or w1.shape[0] != H or w1.shape[1] % (16 * gated) or w1.shape[1] < 16:
+        raise ValueError(f"moe_few_tokens: w1 must be [{H}, total width in multiples of "
                          f"{16 * gated}], got {tuple(w1.shape)}")
     total = w1.shape[1]
-    if tuple(w2.shape) != (total // gated, hidden):
-        raise ValueError(f"moe_few_tokens: w2 must be {(total // gated, hidden)}, got "
-                         f"{tuple(w2.shape)}")
-    if isinstance(w1, Int4Weight):
+    if tuple(w2.shape) != (total // gated, H):
+        raise ValueError(f"moe_few_tokens: w2 must be {(total // gated, H)}, got {tuple(w2.shape)}")
+    group = blocks = groups = 0
+    if packed:
         if w1.group_size != w2.group_size:
             raise ValueError("moe_few_tokens: w1 and w2 must have one group size, got "
                              f"{w1.group_size} and {w2.group_size}")
         if w1.row_offsets is not None and len(w1.row_offsets) > 2:
             raise ValueError("moe_few_tokens: a 4-bit w1 is one segment (no row_offsets)")
-        offs = w2.row_offsets if w2.row_offsets is not None else (0, w2.rows)
-        if len(offs) != num_experts + 1:
-            raise ValueError(f"moe_few_tokens: a 4-bit w2 needs row_offsets of its {num_experts} "
-                             "experts")
-        return (w1.packed, w1.scales.data_ptr(), w2.packed, w2.scales.data_ptr(), w1.group_size,
-                w2.packed.shape[0], w2.scales.shape[0], total)
-    if not (w1.is_contiguous() and w2.is_contiguous()):
-        raise ValueError("moe_few_tokens: w1 and w2 must be contiguous")
-    return w1, None, w2, None, 0, 0, 0, total
+        if len(w2.row_offsets or (0, 0)) != E + 1:
+            raise ValueError(f"moe_few_tokens: a 4-bit w2 needs row_offsets of its {E} experts")
+        group, blocks, groups = w1.group_size, w2.packed.shape[0], w2.scales.shape[0]
+    act = ACT_CODE[activation]
+    ws_bytes = int(lib.moe_few_tokens_workspace_bytes(T, H, E, top_k, max_width, act))
+    return T, H, E, group, blocks, groups, total, ws_bytes, act, DTYPE_CODE[dt]
 
 
 @eager_only
@@ -83,65 +101,60 @@ def moe_few_tokens(
     of 16; an expert whose offsets do not fit adds nothing and sets the device
     status word.  In fp16 an intermediate above 65504 is infinite, as in the
     training forward.  Inference only."""
-    if x.dim() != 2:
-        raise ValueError(f"moe_few_tokens: x must be [tokens, hidden], got {tuple(x.shape)}")
-    T, H = x.shape
-    if T > FEW_TOKENS_MAX:
-        raise ValueError(f"moe_few_tokens: at most {FEW_TOKENS_MAX} tokens, got {T} (use the "
-                         "layer's forward)")
-    if not (x.is_cuda and expert_weight_offsets.is_cuda):
-        raise ValueError("moe_b200 kernels need CUDA tensors (no CPU fallback)")
-    if x.dtype not in DTYPE_CODE:
-        raise TypeError(f"moe_few_tokens: bf16, fp16 or fp32, got {x.dtype}")
-    if activation not in ACT_CODE:
-        raise NotImplementedError(f"activation {activation!r} is not supported "
-                                  f"(supported: {tuple(ACT_CODE)})")
-    E = router_weight.shape[0]
-    if router_weight.dim() != 2 or router_weight.shape[1] != H or not router_weight.is_contiguous():
-        raise ValueError(f"moe_few_tokens: router_weight must be contiguous [experts, {H}], got "
-                         f"{tuple(router_weight.shape)}")
-    if not 1 <= E <= 256 or not 1 <= top_k <= min(E, 32):
-        raise ValueError(f"moe_few_tokens: 1 to 256 experts and top_k up to 32 of them, got {E} and "
-                         f"{top_k}")
-    if (H % 16 or not 16 <= H <= 32768 or max_expert_width % 16
-            or not 16 <= max_expert_width <= 32768):
-        raise ValueError("moe_few_tokens: hidden size and expert widths must be multiples of 16 up "
-                         f"to 32768, got {H} and {max_expert_width}")
-    if expert_weight_offsets.numel() != E + 1 or expert_weight_offsets.device != x.device:
-        raise ValueError(f"moe_few_tokens: expert_weight_offsets needs {E + 1} entries on x's device")
-    gated = 2 if activation == "swiglu" else 1
-    w1t, s1, w2t, s2, group, blocks, groups, total = _check_weights(
-        x, router_weight, w1, w2, E, H, max_expert_width, gated)
-    if group:
-        refuse_grad("moe_few_tokens", x, router_weight)
+    dt, dev = x.dtype, x.device
+    packed = w1.__class__ is Int4Weight and w2.__class__ is Int4Weight
+    if packed:
+        t1, t2 = w1.packed, w2.packed
+        key = (x.shape, dt, router_weight.shape, w1.shape, w2.shape, w1.group_size, w2.group_size,
+               w1.row_offsets is None or len(w1.row_offsets), w2.row_offsets is None or
+               len(w2.row_offsets), t2.shape, w2.scales.shape, expert_weight_offsets.numel(),
+               max_expert_width, top_k, activation)
     else:
-        refuse_grad("moe_few_tokens", x, router_weight, w1, w2)
-    dev = x.device
-    out = torch.empty(T, H, dtype=x.dtype, device=dev)
+        t1, t2 = w1, w2
+        key = (x.shape, dt, router_weight.shape, w1.shape, w2.shape, w1.__class__ is Int4Weight,
+               w2.__class__ is Int4Weight, expert_weight_offsets.numel(), max_expert_width, top_k,
+               activation)
+    sig = _signatures.get(key)
+    if sig is None:
+        sig = _signature(x.shape, dt, router_weight.shape, w1, w2, expert_weight_offsets.numel(),
+                         max_expert_width, top_k, activation)
+        if len(_signatures) >= 4096:
+            _signatures.clear()
+        _signatures[key] = sig
+    T, H, E, group, blocks, groups, total, ws_bytes, act, dt_code = sig
+    if not x.is_cuda:
+        raise ValueError("moe_b200 kernels need CUDA tensors (no CPU fallback)")
+    if router_weight.dtype is not dt or w1.dtype is not dt or w2.dtype is not dt:
+        raise TypeError(f"moe_few_tokens: x, router_weight, w1 and w2 must share a dtype, got {dt}, "
+                        f"{router_weight.dtype}, {w1.dtype} and {w2.dtype}")
+    idx = x.get_device()
+    if (router_weight.get_device() != idx or t1.get_device() != idx or t2.get_device() != idx
+            or expert_weight_offsets.get_device() != idx):
+        raise ValueError("moe_few_tokens: all tensors must be on one device")
+    if not (t1.is_contiguous() and t2.is_contiguous() and router_weight.is_contiguous()):
+        raise ValueError("moe_few_tokens: router_weight, w1 and w2 must be contiguous")
+    if torch.is_grad_enabled():
+        refuse_grad("moe_few_tokens", x, router_weight, t1, t2)
+    out = torch.empty((T, H), dtype=dt, device=dev)
     if T == 0:
         return out
     x = row_view(x)
     off = _meta(expert_weight_offsets)
-    p1, p2, pr = w1t.data_ptr(), w2t.data_ptr(), router_weight.data_ptr()
+    p1, p2, pr = t1.data_ptr(), t2.data_ptr(), router_weight.data_ptr()
     if (p1 | p2 | pr) & 15:
         raise ValueError("moe_few_tokens: weights must be 16-byte aligned")
-    act = ACT_CODE[activation]
-    key = (T, H, E, top_k, max_expert_width, act)
-    ws_bytes = _workspace_bytes.get(key)
-    if ws_bytes is None:
-        ws_bytes = int(lib.moe_few_tokens_workspace_bytes(*key))
-        if len(_workspace_bytes) > 4096:
-            _workspace_bytes.clear()
-        _workspace_bytes[key] = ws_bytes
+    s1 = w1.scales.data_ptr() if packed else None
+    s2 = w2.scales.data_ptr() if packed else None
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     with on_device(dev):
-        ev = _ev_begin()
+        ev = _ops._ev_begin()
         rc = lib.moe_few_tokens(
             x.data_ptr(), T, x.stride(0) if T > 1 else H, H, pr, E, p1, s1, p2, s2, group, blocks,
             groups, total, off.data_ptr(), max_expert_width, top_k, 1 if norm_topk_prob else 0, act,
-            out.data_ptr(), H, ws.data_ptr(), ws_bytes, DTYPE_CODE[x.dtype],
-            status_buffer(dev).data_ptr(), stream_of(dev))
-        _ev_end(ev, "few_tokens")
-    check(rc, "moe_few_tokens")
-    _count(2)
+            out.data_ptr(), H, ws.data_ptr(), ws_bytes, dt_code, status_buffer(dev).data_ptr(),
+            stream_of(dev))
+        _ops._ev_end(ev, "few_tokens")
+    if rc:
+        check(rc, "moe_few_tokens")
+    _ops._count(2 if T <= 8 else 4)
     return out

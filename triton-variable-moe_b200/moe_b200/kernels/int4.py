@@ -139,7 +139,8 @@ class Int4Weight:
         return self._host_offsets, n
 
 
-def _layout(rows: int, cols: int, group_size: int, row_offsets):
+@functools.lru_cache(maxsize=256)
+def _layout(rows: int, cols: int, group_size: int, row_offsets: tuple[int, ...] | None):
     """(block rows, groups, host offset array) of a weight; ValueError if it cannot be packed."""
     if group_size not in GROUP_SIZES:
         raise ValueError(f"group_size must be one of {GROUP_SIZES}, got {group_size}")
@@ -169,7 +170,7 @@ def _offsets_tuple(row_offsets: Sequence[int] | None) -> tuple[int, ...] | None:
         if row_offsets.is_cuda:
             raise TypeError("row_offsets are read on the host: pass a list, not a CUDA tensor")
         row_offsets = row_offsets.tolist()
-    return tuple(int(o) for o in row_offsets)
+    return tuple(row_offsets)
 
 
 @eager_only
