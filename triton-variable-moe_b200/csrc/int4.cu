@@ -74,26 +74,41 @@ __device__ __forceinline__ uint32_t place(uint32_t code, int i, int c) {
 // The integer nearest to w / s, ties to even, exactly: the quotient's own rounding (w / s,
 // or w times the rounded reciprocal: off by less than one either way) is undone by the
 // remainder, which fp32 holds without error.
-__device__ __forceinline__ uint32_t exact_code(float w, float s, float quotient) {
-  const float magic = 12582912.f;  // 1.5 x 2^23: adding it rounds to integers
-  float q = (quotient + magic) - magic;
-  const float r = fabsf(fmaf(-q, s, w)), half = 0.5f * s;
-  const float sign = fmaf(-q, s, w) < 0.f ? -1.f : 1.f;
-  const bool odd = (__float_as_uint(q + magic) & 1u) != 0;
-  if (r > half || (r == half && odd)) q += sign;
-  return __float_as_uint(fminf(fmaxf(q, -8.f), 7.f) + (magic + 8.f)) & 15u;
+constexpr float kMagic = 12582912.f;  // 1.5 x 2^23: adding it rounds to integers
+__device__ __forceinline__ float exact_nearest(float w, float s, float quotient) {
+  const float q = (quotient + kMagic) - kMagic;
+  const float r = fmaf(-q, s, w), half = 0.5f * s;
+  const bool odd = (__float_as_uint(q + kMagic) & 1u) != 0;
+  const bool move = fabsf(r) > half || (fabsf(r) == half && odd);
+  return move ? q + (r < 0.f ? -1.f : 1.f) : q;
 }
 
 // The same for weights and scales of 16 bits, from the reciprocal of the scale.  Both
 // have at most 11 significant bits, so a quotient is either halfway between integers
 // or at least 2^-12 from it; w * inv is within 2^-19 of the quotient; rounding it to
 // steps of 2^-13 first therefore gives halfway exactly when it is, and the second
-// rounding sends that to even.  Returns the clamped q - 8 as the low bits' code.
-__device__ __forceinline__ uint32_t nearest_code(float w, float inv) {
+// rounding sends that to even.
+__device__ __forceinline__ float nearest(float w, float inv) {
   const float step = 1536.f;  // 1.5 x 2^10: the sum's last place is 2^-13
-  float t = fmaf(w, inv, step) - step;
-  t = fminf(fmaxf(t, -8.f), 7.f);
-  return __float_as_uint(t + 12582920.f) & 15u;  // 1.5 x 2^23 + 8
+  return ((fmaf(w, inv, step) - step) + kMagic) - kMagic;
+}
+
+// |w| and maxima of two 16-bit weights, a NaN above all.
+template <typename T>
+__device__ __forceinline__ uint32_t abs_max(uint32_t a, uint32_t b);
+template <>
+__device__ __forceinline__ uint32_t abs_max<__nv_bfloat16>(uint32_t a, uint32_t b) {
+  b &= 0x7fff7fffu;
+  const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a),
+                                       *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+template <>
+__device__ __forceinline__ uint32_t abs_max<__half>(uint32_t a, uint32_t b) {
+  b &= 0x7fff7fffu;
+  const __half2 m =
+      __hmax2_nan(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
 }
 
 // rows x 64 columns of a row-major matrix into shared memory, zeros beyond.
@@ -133,6 +148,9 @@ struct Eight {
     const float2 f = few::unpack2<std::conditional_t<sizeof(T) == 4, __half, T>>(w[i / 2]);
     return i & 1 ? f.y : f.x;
   }
+  __device__ __forceinline__ uint32_t pair(int j) const {  // 16-bit types
+    return reinterpret_cast<const uint32_t*>(v)[j];
+  }
 };
 
 // T: type of the weights, S: type of the scales.
@@ -154,7 +172,7 @@ __global__ void __launch_bounds__(kThreadsQ)
     const int row = 32 * part + 4 * r + i;
     v[i].load(w + static_cast<long long>(at.row + row) * ld + col + c, row < at.rows && c < cols);
   }
-  {
+  if constexpr (sizeof(T) == 4) {
     unsigned m[8];  // order of the bits of |w|: a NaN above all
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -168,6 +186,22 @@ __global__ void __launch_bounds__(kThreadsQ)
 #pragma unroll
     for (int j = 1; j < 8; ++j) mine = r == j ? m[j] : mine;
     amax[part][c + r] = mine;
+  } else {
+    uint32_t m[4];  // pairs of columns
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      m[j] = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m[j] = abs_max<T>(m[j], v[i].pair(j));
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1)
+        m[j] = abs_max<T>(m[j], __shfl_xor_sync(0xffffffffu, m[j], o));
+    }
+    uint32_t two = m[0];
+#pragma unroll
+    for (int j = 1; j < 4; ++j) two = r >> 1 == j ? m[j] : two;
+    const float2 f = few::unpack2<T>(two);
+    amax[part][c + r] = __float_as_uint(r & 1 ? f.y : f.x);
   }
   __syncthreads();
   {
@@ -178,8 +212,10 @@ __global__ void __launch_bounds__(kThreadsQ)
     const S s = from_f<S>(__uint_as_float(m) / 7.f);
     const float f = to_f<S>(s);
     scale[pt][cc] = f;
-    // 0: not finite, zero, or below 2^-100
-    inverse[pt][cc] = f >= 7.8886091e-31f && f <= 3.4028234e38f ? 1.f / f : 0.f;
+    // 0: not finite, zero, below 2^-100, or so small in S that its rounding lets a
+    // quotient past 7
+    constexpr float kLeast = few::kIsBf16<S> ? 7.8886091e-31f : 6.1035156e-05f;
+    inverse[pt][cc] = f >= kLeast && f <= 3.4028234e38f ? 1.f / f : 0.f;
     if (pt == first && 32 * first < at.rows && cc < cols)
       scales[static_cast<long long>(at.group + pt / per) * N + col + cc] = s;
   }
@@ -189,19 +225,28 @@ __global__ void __launch_bounds__(kThreadsQ)
   *reinterpret_cast<float4*>(inv + 4) = *reinterpret_cast<const float4*>(&inverse[part][c + 4]);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {  // columns c + 2 j, + 1: lane (g, t) of a block
-    uint32_t word = 0;
+    // Rows 0 and 2 (of both columns) make the low 16 bits, rows 1 and 3 the high ones:
+    // four numbers -7..7 with weights 1, 16, 256, 4096, and 8 of each, as one integer.
+    uint32_t half[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int o = 0; o < 2; ++o) {
+      float sum = 0.f, weight = 1.f;
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        uint32_t code;
+      for (int n = 0; n < 4; ++n) {
+        const int i = o + 2 * (n >> 1), x = n & 1;
         const float value = v[i].get(2 * j + x), f = inv[2 * j + x];
+        float q;
         if constexpr (sizeof(T) == 4)
-          code = exact_code(value, scale[part][c + 2 * j + x], value * f);
+          q = exact_nearest(value, scale[part][c + 2 * j + x], value * f);
         else
-          code = nearest_code(value, f);
-        word |= place(code, i, x);
+          q = nearest(value, f);
+        sum = fmaf(q, weight, sum);
+        weight *= 16.f;
       }
+      half[o] = __float_as_uint(sum + (kMagic + 34952.f));
+    }
+    uint32_t word = __byte_perm(half[0], half[1], 0x5410);
+    word = __funnelshift_l(word, word, 3);
     if (inv[2 * j] == 0.f || inv[2 * j + 1] == 0.f) {  // a scale without its reciprocal
       word = 0;
 #pragma unroll 1
@@ -211,8 +256,10 @@ __global__ void __launch_bounds__(kThreadsQ)
 #pragma unroll
         for (int n = 0; n < 8; ++n)
           if (n == k) value = v[n >> 1].get(2 * j + (n & 1));
-        const uint32_t code = f > 0.f && f <= 3.4028234e38f ? exact_code(value, f, value / f) : 8u;
-        word |= place(code, k >> 1, k & 1);
+        float q = 0.f;
+        if (f > 0.f && f <= 3.4028234e38f)
+          q = fminf(fmaxf(exact_nearest(value, f, value / f), -8.f), 7.f);
+        word |= place(__float_as_uint(q + (kMagic + 8.f)) & 15u, k >> 1, k & 1);
       }
     }
     const int nb = c / 16, g = c % 16 / 2 + j, t = r >> 1, h = part & 1, kb = part >> 1;
