@@ -50,7 +50,7 @@ namespace cg = cooperative_groups;
 using namespace few;
 
 constexpr int kMaxTokens = 64;    // one 64-bit mask of tokens an expert
-constexpr int kMaxExperts = 256;
+constexpr int kMaxExperts = 256;  // (a byte names one)
 constexpr int kMaxTopK = 32;
 constexpr int kMaxCluster = 8;
 constexpr int kThreads = 512;     // 16 warps: at 128 registers a thread the SM is full
@@ -59,16 +59,23 @@ constexpr int kTeam = 4;          // warps that share a unit (they split its red
 constexpr int kTeams = kWarps / kTeam;
 constexpr int kTeamThreads = kTeam * 32;
 constexpr int kMaxLocal = kMaxCluster * kTeams;  // sliced items of a cluster: under a wave
-constexpr int kTile = 64;         // columns of a unit
-constexpr int kRedLd = kTile + 4;
+constexpr int kMinTile = 64;      // columns of a unit: L::kTile, 64 or 128
+constexpr int kMaxTile = 128;
+template <typename L>
+constexpr int kRedLd = L::kTile + 4;
 constexpr int kMaxSlices = 16;
-constexpr int kMaxDepth = 4;
+constexpr int kMaxDepth = 2;
 constexpr int kAddTokens = 8;     // up to this many, the down kernel writes the output
 constexpr int kMaxWidth = 32768;  // hidden size and expert width: item counts stay 32-bit
 
 __host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
-// Outputs of a 64-column tile: a gated activation's tile is 32 gate and 32 up columns.
-__host__ __device__ inline int tile_outputs(int act) { return act == ACT_SWIGLU ? 32 : 64; }
+// log2 of the outputs of a tile: a gated activation's is half gate and half up columns.
+template <typename L>
+__device__ __forceinline__ int outputs_log2(int act) {
+  constexpr int n = L::kTile == 128 ? 7 : 6;
+  static_assert(1 << n == L::kTile, "tiles of 64 or 128 columns");
+  return act == ACT_SWIGLU ? n - 1 : n;
+}
 __host__ __device__ inline int group_count(int rows, int shift) {
   return (rows + (1 << shift) - 1) >> shift;
 }
@@ -186,30 +193,34 @@ struct alignas(16) Common {
   Unit table[kTeams][kTable];
 };
 
-// The strip of an up product's tile: 64 columns, or 32 gate and their 32 up columns.
+// The strip of an up product's tile.
+template <typename L>
 __device__ __forceinline__ void up_strip(Strip& s, int first, int width, int act, int tile, int H,
                                          int shift) {
+  constexpr int half = L::kTile / 2;
   s.row = 0;
   s.kb = s.sg = 0;
   s.groups = group_count(H, shift);
   if (act == ACT_SWIGLU) {
-    s.col = first + tile * 32;
-    s.lo = s.hi = min(32, width - tile * 32);
+    s.col = first + tile * half;
+    s.lo = s.hi = min(half, width - tile * half);
     s.jump = width;
   } else {
-    s.col = first + tile * 64;
-    s.lo = min(32, width - tile * 64);
-    s.hi = min(32, max(0, width - tile * 64 - 32));
-    s.jump = 32;
+    s.col = first + tile * L::kTile;
+    s.lo = min(half, width - tile * L::kTile);
+    s.hi = min(half, max(0, width - tile * L::kTile - half));
+    s.jump = half;
   }
 }
+template <typename L>
 __device__ __forceinline__ void down_strip(Strip& s, const Active& a, int e, int row, int tile,
                                            int H, int shift) {
   s.row = row;
-  s.col = tile * kTile;
-  s.lo = min(32, H - s.col);
-  s.hi = min(32, max(0, H - s.col - 32));
-  s.jump = 32;
+  constexpr int half = L::kTile / 2;
+  s.col = tile * L::kTile;
+  s.lo = min(half, H - s.col);
+  s.hi = min(half, max(0, H - s.col - half));
+  s.jump = half;
   s.kb = a.kb[e];
   s.sg = a.sg[e];
   s.groups = group_count(a.width[e], shift);
@@ -281,7 +292,7 @@ __device__ __forceinline__ void run_units(int total, const Matrix& m,
     }
   };
   top_up();
-  float acc[4][NG][4];
+  float acc[L::kSums][NG][4];
   for (int n = 0; n < total; ++n) {
     const Unit u = nth(n);
     const Src src = source(u);
@@ -289,7 +300,7 @@ __device__ __forceinline__ void run_units(int total, const Matrix& m,
     auto sums = [&](auto groups, auto parts) {
       constexpr int G = decltype(groups)::value, P = decltype(parts)::value;
 #pragma unroll
-      for (int a = 0; a < 4; ++a)
+      for (int a = 0; a < L::kSums; ++a)
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
@@ -305,10 +316,10 @@ __device__ __forceinline__ void run_units(int total, const Matrix& m,
         const uint32_t stage = ring + use_slot * L::kStage;
         v.template load<G, P>(1, src, left, lane);
         if (used < copied) ring_wait(bars + 8 * use_slot, phase, &c.abort);
-        L::template half<G, P, NG, Src>(0, acc, at, m, left, stage, lane, v);
+        L::template half<G, P, NG, Src>(0, acc, at, m, u.strip, left, stage, lane, v);
         v.template advance<G>(kRows);
         v.template load<G, P>(0, src, left - kRows, lane);
-        L::template half<G, P, NG, Src>(1, acc, at, m, left, stage, lane, v);
+        L::template half<G, P, NG, Src>(1, acc, at, m, u.strip, left, stage, lane, v);
         __syncwarp();  // the step has been read by every lane: its place is free
         ++used;
         if (++use_slot == D) {
@@ -318,10 +329,10 @@ __device__ __forceinline__ void run_units(int total, const Matrix& m,
         top_up();
       }
       // warps 2 and 3 leave their sums, 0 and 1 add theirs to them
-      float* mine = red + (wr & 1) * TOK * kRedLd;
-      if (wr >= 2) L::template store<G, NG, kRedLd, false>(acc, lane, mine);
+      float* mine = red + (wr & 1) * TOK * kRedLd<L>;
+      if (wr >= 2) L::template store<G, NG, kRedLd<L>, false>(acc, lane, mine);
       team_sync(team);
-      if (wr < 2) L::template store<G, NG, kRedLd, true>(acc, lane, mine);
+      if (wr < 2) L::template store<G, NG, kRedLd<L>, true>(acc, lane, mine);
       team_sync(team);
     };
     if constexpr (!L::kGroups)
@@ -358,10 +369,11 @@ __device__ __forceinline__ void ring_init(Common& c) {
 }
 
 // The unit's sums of vector `tok`, columns c .. c + 3.
-template <int TOK>
+template <typename L, int NG>
 __device__ __forceinline__ float4 unit_sum(const float* red, int tok, int c) {
-  const float4 a = *reinterpret_cast<const float4*>(red + tok * kRedLd + c);
-  const float4 b = *reinterpret_cast<const float4*>(red + (TOK + tok) * kRedLd + c);
+  constexpr int TOK = L::template kTokens<NG>, LD = kRedLd<L>;
+  const float4 a = *reinterpret_cast<const float4*>(red + tok * LD + c);
+  const float4 b = *reinterpret_cast<const float4*>(red + (TOK + tok) * LD + c);
   return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
 }
 __device__ __forceinline__ void add4(float4& a, const float4& b) {
@@ -387,7 +399,7 @@ __device__ __forceinline__ void store4(T* d, float4 v, bool vec) {
 template <typename L, int NG>
 constexpr int kRingBytes = kWarps * L::template kDepth<NG> * L::kStage;
 template <typename L, int NG>
-constexpr int kRedFloats = 2 * L::template kTokens<NG> * kRedLd;  // a team
+constexpr int kRedFloats = 2 * L::template kTokens<NG> * kRedLd<L>;  // a team
 template <typename L, int NG>
 constexpr int kWorkBytes = kRingBytes<L, NG> + 4 * kTeams * kRedFloats<L, NG>;
 
@@ -662,9 +674,9 @@ __device__ __forceinline__ bool expert_width(int a, int b, int total, int max_wi
 // One warp: from the token masks and the offsets, the experts that have rows and
 // columns, and their (pass, tile) items.  Offsets that leave the matrices, or are
 // not in steps of 16, empty the expert and set the status word.
-template <int TOK>
+template <typename L, int TOK>
 __device__ __forceinline__ void find_active(const LayerParams& p, UpSmem& s) {
-  const int lane = threadIdx.x & 31, outputs = p.act == ACT_SWIGLU ? 5 : 6;  // log2
+  const int lane = threadIdx.x & 31, outputs = outputs_log2<L>(p.act);
   static_assert((kMaxTokens / 8 * kMaxTopK + kMaxExperts) * (kMaxWidth / 32) <= 1 << 20,
                 "20 bits of items, 12 of rows");
   unsigned sums = 0;
@@ -736,13 +748,13 @@ __device__ __forceinline__ void find_packed(const LayerParams& p, UpSmem& s) {
 }
 
 // One warp: the down kernel's slice length and items, into the workspace.
-template <int TOK, int ROUND>
+template <typename L, int TOK, int ROUND>
 __device__ __forceinline__ void plan_down(const LayerParams& p, const Active& act, int active) {
-  const int lane = threadIdx.x & 31, tiles = ceil_div(p.H, kTile);
+  const int lane = threadIdx.x & 31, tiles = ceil_div(p.H, L::kTile);
   int widest = 0;
   for (int j = lane; j < active; j += 32) widest = max(widest, act.width[j]);
   widest = __reduce_max_sync(0xffffffffu, widest);
-  const int len = plan_length(max(1, ceil_div(widest, ROUND)), p.down_teams, p.max_slices, p.T <= kAddTokens ? 9 : 4,
+  const int len = plan_length(max(1, ceil_div(widest, ROUND)), p.down_teams, p.max_slices, p.T <= kAddTokens ? 9 : 8,
                               [&](int length) {
     int n = 0;
     for (int j = lane; j < active; j += 32)
@@ -777,9 +789,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   float* log = reinterpret_cast<float*>(work);  // the routing's sums, before the rings
   float* part = log + p.T * lde;
   UpSmem& s = *reinterpret_cast<UpSmem*>(raw + p.smem_work);
-  int* sel_s = reinterpret_cast<int*>(raw + p.smem_work + sizeof(UpSmem));
-  float* wgt_s = reinterpret_cast<float*>(sel_s + A);
-  int* list = sel_s + 2 * A;  // token of each expert-sorted row
+  float* wgt_s = reinterpret_cast<float*>(raw + p.smem_work + sizeof(UpSmem));
+  uint8_t* sel_s = reinterpret_cast<uint8_t*>(wgt_s + A);
+  uint8_t* list = sel_s + A;  // token of each expert-sorted row
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = static_cast<int>(cluster.block_rank());
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
@@ -804,7 +816,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     for (int a = tid; a < A; a += kThreads) {
       const int sel = p.sel[a], t = a / p.k;
-      sel_s[a] = sel;
+      sel_s[a] = static_cast<uint8_t>(sel);
       wgt_s[a] = p.wgt[a];
       atomicOr(mask32 + 2 * sel + (t >> 5), 1u << (t & 31));
     }
@@ -822,7 +834,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       choose(p, cluster, log, lde, t, &sel, &wgt);
       if (lane < p.k) {
         for (int c = 0; c < p.cluster; ++c) {
-          cluster.map_shared_rank(sel_s, c)[t * p.k + lane] = sel;
+          cluster.map_shared_rank(sel_s, c)[t * p.k + lane] = static_cast<uint8_t>(sel);
           cluster.map_shared_rank(wgt_s, c)[t * p.k + lane] = wgt;
           // (32-bit words: 64-bit atomics of several CTAs on one shared word lose bits)
           atomicOr(cluster.map_shared_rank(mask32, c) + 2 * sel + (t >> 5), 1u << (t & 31));
@@ -835,7 +847,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int clusters = gridDim.x / p.cluster, teams = gridDim.x * kTeams;
   const int rounds = ceil_div(p.H, kRound);
   if (wid == 0) {
-    find_active<TOK>(p, s);
+    find_active<L, TOK>(p, s);
     __syncwarp();
     // Whole items, a wave of them over all teams at a time; the rest whole too, or in
     // slices of a cluster's items over its teams.  Lane l weighs l + 1 slices, in
@@ -858,7 +870,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   for (int a = tid; a < A; a += kThreads) {
     const int e = sel_s[a], t = a / p.k;
-    list[s.base[e] + __popcll(s.mask[e] & ((1ull << t) - 1))] = t;
+    list[s.base[e] + __popcll(s.mask[e] & ((1ull << t) - 1))] = static_cast<uint8_t>(t);
   }
   __syncthreads();
   if (blockIdx.x == gridDim.x - 1) {  // (the block that units come to last)
@@ -868,7 +880,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       p.row[a] = s.base[e] + __popcll(s.mask[e] & ((1ull << t) - 1));
       if (!p.sel) p.wgt[a] = wgt_s[a];
     }
-    for (int i = tid; i < ceil_div(p.H, kTile); i += kThreads) p.ticket[i] = 0;
+    for (int i = tid; i < ceil_div(p.H, L::kTile); i += kThreads) p.ticket[i] = 0;
     for (int j = tid; j < active; j += kThreads) {
       int* d = p.plan + PLAN_WORDS + j;
       d[0 * kMaxExperts] = s.c.act.n[j];
@@ -878,7 +890,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       d[4 * kMaxExperts] = s.c.act.kb[j];
       d[5 * kMaxExperts] = s.c.act.sg[j];
     }
-    if (wid == kWarps - 1) plan_down<TOK, kRound>(p, s.c.act, active);
+    if (wid == kWarps - 1) plan_down<L, TOK, kRound>(p, s.c.act, active);
   }
 
   // the team's units: its items of the whole waves, then its slices of the cluster's
@@ -907,7 +919,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       item = waves * teams + mine + clusters * u.local;
     }
     u.e = find_item(act.item, active, item);
-    const int width = act.width[u.e], outputs = tile_outputs(p.act) == 32 ? 5 : 6;
+    const int width = act.width[u.e], outputs = outputs_log2<L>(p.act);
     const int tiles = (width + (1 << outputs) - 1) >> outputs, r = item - act.item[u.e];
     const int pass = r / tiles;
     u.tile = r - pass * tiles;
@@ -915,7 +927,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     u.row = act.base[u.e] + pass * TOK;
     u.begin = u.slice * q * kRound;
     u.strip.end = u.local < 0 ? p.H : min(p.H, u.begin + q * kRound);
-    up_strip(u.strip, act.first[u.e], width, p.act, u.tile, p.H, p.shift);
+    up_strip<L>(u.strip, act.first[u.e], width, p.act, u.tile, p.H, p.shift);
     return u;
   };
   auto source = [&](const Unit& u) {
@@ -926,10 +938,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto emit = [&](const Unit& u, int tok, int c, auto get) {
     const float4 a = get(tok, c);
     float v[4];
-    int col = u.tile * 64 + c;
+    const int col = (u.tile << outputs_log2<L>(p.act)) + c;
     if (p.act == ACT_SWIGLU) {
-      const float4 b = get(tok, c + 32);
-      col = u.tile * 32 + c;
+      const float4 b = get(tok, c + L::kTile / 2);
       v[0] = act_gated(a.x, b.x); v[1] = act_gated(a.y, b.y);
       v[2] = act_gated(a.z, b.z); v[3] = act_gated(a.w, b.w);
     } else {
@@ -939,21 +950,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (col < act.width[u.e])
       hidden_store4<T>(static_cast<T*>(p.h) + (u.row + tok) * p.ldh, p.max_width, col, v);
   };
-  const int vecs = tile_outputs(p.act) / 4;
+  const int vecs = 1 << (outputs_log2<L>(p.act) - 2);
   const Matrix m{&p.map1, p.w1, p.s1, p.total, p.shift, p.act == ACT_SWIGLU};
   run_units<L, NG>(total, m, work, red, s.c, unit, source, [&](const Unit& u) {
     if (u.local < 0) {
       for (int j = tt; j < u.count * vecs; j += kTeamThreads)
         emit(u, j / vecs, 4 * (j % vecs),
-             [&](int tok, int c) { return unit_sum<TOK>(red, tok, c); });
+             [&](int tok, int c) { return unit_sum<L, NG>(red, tok, c); });
       return;
     }
-    float* dst = p.u + u.row * p.ldu + u.tile * kTile;
+    float* dst = p.u + u.row * p.ldu + u.tile * L::kTile;
     const long long slice = static_cast<long long>(A) * p.ldu;
-    for (int j = tt; j < u.count * (kTile / 4); j += kTeamThreads) {
-      const int tok = j / (kTile / 4), c = 4 * (j % (kTile / 4));
+    for (int j = tt; j < u.count * (L::kTile / 4); j += kTeamThreads) {
+      const int tok = j / (L::kTile / 4), c = 4 * (j % (L::kTile / 4));
       *reinterpret_cast<float4*>(dst + u.slice * slice + tok * p.ldu + c) =
-          unit_sum<TOK>(red, tok, c);
+          unit_sum<L, NG>(red, tok, c);
     }
     team_sync(team);
     if (tt == 0) {
@@ -1011,7 +1022,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncthreads();
   const int active = s.plan[PLAN_ACTIVE], q = s.plan[PLAN_LENGTH], items = s.plan[PLAN_ITEMS];
-  const int tiles = ceil_div(p.H, kTile);
+  const int tiles = ceil_div(p.H, L::kTile);
   const Active& act = s.act;
 
   T* out = static_cast<T*>(p.out);
@@ -1045,7 +1056,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     u.row = act.base[u.e] + pass * TOK;
     u.begin = u.slice * q * kRound;
     u.strip.end = min(width, u.begin + q * kRound);
-    down_strip(u.strip, act, u.e, act.first[u.e] / gated, u.tile, p.H, p.shift);
+    down_strip<L>(u.strip, act, u.e, act.first[u.e] / gated, u.tile, p.H, p.shift);
     return u;
   };
   auto source = [&](const Unit& u) {
@@ -1055,22 +1066,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   const long long slice = static_cast<long long>(A) * p.H;
   const bool vec = (p.ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
   // threads that share a (token, column vector) of the final sum
-  const int share = p.T == 1 ? 8 : p.T == 2 ? 4 : p.T <= 4 ? 2 : 1;
+  // (one pass over them then: they meet in shared memory)
+  constexpr int kVecs = L::kTile / 4;
+  const int share = p.T * kVecs > kTeamThreads / 2 ? 1
+                    : kTeamThreads / (kVecs * (p.T == 1 ? 1 : p.T == 2 ? 2 : 4));
   const Matrix m{&p.map2, p.w2, p.s2, p.H, p.shift, 0};
   run_units<L, NG>(
       items * tiles > me ? ceil_div(items * tiles - me, teams) : 0, m, work, red, s, unit, source,
       [&](const Unit& u) {
-        const int cols = p.H - u.tile * kTile;
-        float* y = p.y + u.tile * kTile;
+        const int cols = p.H - u.tile * L::kTile;
+        float* y = p.y + u.tile * L::kTile;
         // (with the remainders' columns, see HiddenSource)
         const bool split = sizeof(T) == 2 && u.count <= 4;
         auto down_sum = [&](int tok, int c) {
-          float4 v = unit_sum<TOK>(red, tok, c);
-          if (split) add4(v, unit_sum<TOK>(red, tok + 4, c));
+          float4 v = unit_sum<L, NG>(red, tok, c);
+          if (split) add4(v, unit_sum<L, NG>(red, tok + 4, c));
           return v;
         };
-        for (int j = tt; j < u.count * (kTile / 4); j += kTeamThreads) {
-          const int tok = j / (kTile / 4), c = 4 * (j % (kTile / 4));
+        for (int j = tt; j < u.count * (L::kTile / 4); j += kTeamThreads) {
+          const int tok = j / (L::kTile / 4), c = 4 * (j % (L::kTile / 4));
           if (c < cols)
             *reinterpret_cast<float4*>(y + u.slice * slice +
                                        static_cast<long long>(u.row + tok) * p.H + c) =
@@ -1086,8 +1100,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!s.last[team]) return;
         // each thread's slots in order, four at a time, their parts in order
         const int lanes = kTeamThreads / share, part = tt / lanes;
-        for (int j0 = 0; j0 < p.T * (kTile / 4); j0 += lanes) {  // (barriers inside)
-          const int j = j0 + tt % lanes, t = j / (kTile / 4), c = 4 * (j % (kTile / 4));
+        for (int j0 = 0; j0 < p.T * (L::kTile / 4); j0 += lanes) {  // (barriers inside)
+          const int j = j0 + tt % lanes, t = j / (L::kTile / 4), c = 4 * (j % (L::kTile / 4));
           const bool in = t < p.T && c < cols;
           float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
           if (in) {
@@ -1132,7 +1146,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (part == 0)
               for (int g = 1; g < share; ++g) add4(o, sums[tt + g * lanes]);
           }
-          if (part == 0 && in) store4<T>(out + t * p.ldo + u.tile * kTile + c, o, vec);
+          if (part == 0 && in) store4<T>(out + t * p.ldo + u.tile * L::kTile + c, o, vec);
         }
       });
   if (s.abort && lane == 0 && p.status) *p.status = kStatusTimeout;
@@ -1231,7 +1245,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   ring_init<L::template kDepth<NG>>(s.c);
   __syncthreads();
-  const int outputs = tile_outputs(p.act), teams = gridDim.x * kTeams;
+  const int outputs = 1 << outputs_log2<L>(p.act), teams = gridDim.x * kTeams;
   if (wid == 0) {  // as find_active
     const int gated = p.act == ACT_SWIGLU ? 2 : 1;
     int active = 0, kb = 0, sg = 0;
@@ -1276,7 +1290,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     auto units = [&](int j, int len) {
       return ceil_div(s.c.act.n[j], TOK) *
-             (p.down ? ceil_div(p.H, kTile) * ceil_div(ceil_div(s.c.act.width[j], kRound), len)
+             (p.down ? ceil_div(p.H, L::kTile) * ceil_div(ceil_div(s.c.act.width[j], kRound), len)
                      : ceil_div(s.c.act.width[j], outputs) * ceil_div(ceil_div(p.H, kRound), len));
     };
     int widest = 0;
@@ -1325,7 +1339,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     Unit u;
     u.e = find_item(act.item, active, i);
     const int width = act.width[u.e], k_rows = p.down ? width : p.H;
-    const int tiles = p.down ? ceil_div(p.H, kTile) : ceil_div(width, outputs);
+    const int tiles = p.down ? ceil_div(p.H, L::kTile) : ceil_div(width, outputs);
     const int ns = ceil_div(ceil_div(k_rows, kRound), q), r = i - act.item[u.e];
     const int j = r / tiles, pass = j / ns;
     u.tile = r - j * tiles;
@@ -1336,9 +1350,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     u.begin = u.slice * q * kRound;
     u.strip.end = min(k_rows, u.begin + q * kRound);
     if (p.down)
-      down_strip(u.strip, act, u.e, act.first[u.e], u.tile, p.H, p.shift);
+      down_strip<L>(u.strip, act, u.e, act.first[u.e], u.tile, p.H, p.shift);
     else
-      up_strip(u.strip, act.first[u.e], width, p.act, u.tile, p.H, p.shift);
+      up_strip<L>(u.strip, act.first[u.e], width, p.act, u.tile, p.H, p.shift);
     return u;
   };
   auto source = [&](const Unit& u) {
@@ -1350,13 +1364,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                    [&](const Unit& u) {
                      float* dst = p.part +
                                   (static_cast<long long>(u.slice) * p.rows + u.row) * p.ldp +
-                                  u.tile * kTile;
-                     const int cols = p.act == ACT_SWIGLU ? kTile : static_cast<int>(p.ldp) - u.tile * kTile;
-                     for (int j = tt; j < u.count * (kTile / 4); j += kTeamThreads) {
-                       const int tok = j / (kTile / 4), c = 4 * (j % (kTile / 4));
+                                  u.tile * L::kTile;
+                     const int cols = static_cast<int>(p.ldp) - u.tile * L::kTile;
+                     for (int j = tt; j < u.count * (L::kTile / 4); j += kTeamThreads) {
+                       const int tok = j / (L::kTile / 4), c = 4 * (j % (L::kTile / 4));
                        if (c < cols)
                          *reinterpret_cast<float4*>(dst + tok * p.ldp + c) =
-                             unit_sum<TOK>(red, tok, c);
+                             unit_sum<L, NG>(red, tok, c);
                      }
                    });
   if (s.c.abort && lane == 0 && p.status) *p.status = kStatusTimeout;
@@ -1392,12 +1406,12 @@ __global__ void __launch_bounds__(kThreads)
       const int e = find_item(base_s, active, row);
       if (row >= base_s[e] && row - base_s[e] < n_s[e] && (p.down || c < width_s[e])) {
         const int ns = ceil_div(ceil_div(p.down ? width_s[e] : p.H, kRound), q);
-        const float* src = p.part + row * p.ldp + (gated ? c / 32 * kTile + c % 32 : c);
+        const float* src = p.part + row * p.ldp + (gated ? c / (L::kTile / 2) * L::kTile + c % (L::kTile / 2) : c);
         float4 b = v;
 #pragma unroll 4
         for (int z = 0; z < ns; ++z) {
           add4(v, __ldcg(reinterpret_cast<const float4*>(src + z * slice)));
-          if (gated) add4(b, __ldcg(reinterpret_cast<const float4*>(src + z * slice + 32)));
+          if (gated) add4(b, __ldcg(reinterpret_cast<const float4*>(src + z * slice + L::kTile / 2)));
         }
         if (gated)
           v = make_float4(act_gated(v.x, b.x), act_gated(v.y, b.y), act_gated(v.z, b.z),
@@ -1420,10 +1434,10 @@ struct LayerPlan {
   int slices;
 };
 
-// Columns of a product's partial sums: whole tiles.
+// Columns of a product's partial sums: whole tiles of either size.
 long long padded_columns(long long width, int act) {
-  const int n = tile_outputs(act);
-  return (width + n - 1) / n * kTile;
+  const int n = act == ACT_SWIGLU ? kMaxTile / 2 : kMaxTile;
+  return (width + n - 1) / n * kMaxTile;
 }
 
 // Slices of a reduction the workspace holds: 64 MB of partial sums, or one slice.
@@ -1447,7 +1461,7 @@ LayerPlan layer_plan(int T, int H, int k, int max_width, int act) {
   p.slot = take(4 * A);
   p.row = take(4 * A);
   p.wgt = take(4 * A);
-  p.ticket = take(4ll * ceil_div(H, kTile));
+  p.ticket = take(4ll * ceil_div(H, kMinTile));
   p.sel = take(4 * A);
   p.u = take(4 * p.slices * A * p.ldu);
   p.h = take(4 * A * max_width);  // two 16-bit values or one fp32
@@ -1552,7 +1566,7 @@ int launch_layer(LayerParams& p, cudaStream_t st) {
   const size_t route = p.T > kAddTokens ? 0 : sizeof(float) * (1 + ksub) * p.T * lde;
   const size_t work = kWorkBytes<L, NG>;
   p.smem_work = static_cast<int>(route > work ? route : work);
-  const size_t up_smem = p.smem_work + sizeof(UpSmem) + 12 * A;
+  const size_t up_smem = p.smem_work + sizeof(UpSmem) + 6 * A;
   const size_t down_smem = work + sizeof(Common) + 12 * A;
   if (up_smem > kSmemMax || down_smem > kSmemMax) return kStatusUnsupported;
   using T = typename L::Elem;
@@ -1605,7 +1619,8 @@ int launch_layer(LayerParams& p, cudaStream_t st) {
 }
 
 // 8 or 16 columns of vectors a unit: 16 when an expert has more than about 6 rows on
-// average (each further pass over an expert's weights reads them again, from L2).
+// average (each further pass over an expert's weights reads them again, from L2).  The
+// 4-bit products, 128 columns wide, have registers for 8.
 template <typename L>
 int layer_for_tokens(LayerParams& p, cudaStream_t st) {
   return p.T <= 8 || p.T * p.k <= 6 * p.E ? launch_layer<L, 1>(p, st) : launch_layer<L, 2>(p, st);
@@ -1702,8 +1717,8 @@ int few_tokens(const void* x, long long T, long long ldx, long long H, const voi
   p.max_slices = plan.slices;
   p.status = status;
   if (shift) {
-    if (dtype == 0) return layer_for_tokens<Int4<__nv_bfloat16>>(p, st);
-    if (dtype == 1) return layer_for_tokens<Int4<__half>>(p, st);
+    if (dtype == 0) return launch_layer<Int4<__nv_bfloat16>, 1>(p, st);
+    if (dtype == 1) return launch_layer<Int4<__half>, 1>(p, st);
     return kStatusUnsupported;
   }
   if (dtype < 0 || dtype > 2) return kStatusUnsupported;
@@ -1751,12 +1766,8 @@ int grouped_int4(const void* x, long long rows, long long ldx, const void* w, co
   p.ldp = padded_columns(down ? H : max_width, act);
   p.max_slices = slice_limit(rows * p.ldp);
   p.out = out; p.ldo = ldo; p.status = status;
-  const bool narrow = rows <= 8 || rows <= 6ll * E;  // as layer_for_tokens
-  if (dtype == 0)
-    return narrow ? launch_group<Int4<__nv_bfloat16>, 1>(p, st)
-                  : launch_group<Int4<__nv_bfloat16>, 2>(p, st);
-  if (dtype == 1)
-    return narrow ? launch_group<Int4<__half>, 1>(p, st) : launch_group<Int4<__half>, 2>(p, st);
+  if (dtype == 0) return launch_group<Int4<__nv_bfloat16>, 1>(p, st);
+  if (dtype == 1) return launch_group<Int4<__half>, 1>(p, st);
   return kStatusUnsupported;
 }
 

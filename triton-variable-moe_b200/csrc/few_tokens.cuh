@@ -189,7 +189,7 @@ struct RowSource {
   static constexpr int half = 0;
   const T* x;
   long long ld;
-  const int* list;  // null: rows first, first + 1, ..
+  const uint8_t* list;  // null: rows first, first + 1, ..
   int first;
   __device__ __forceinline__ const T* row(int i) const {
     return x + static_cast<long long>(list ? list[first + i] : first + i) * ld;
@@ -237,11 +237,10 @@ __device__ __forceinline__ void hidden_store4<float>(float* row, int, int c, con
 }
 
 // ------------------------------------------------------------------ weights
-// A strip: reduction rows up to `end` of one expert's weights and 64 of its
-// columns, in two halves of 32: side by side, or (a gated activation) 32 gate
-// columns and the 32 up columns they go with, `jump` further right.  `lo` and `hi`
-// of each half's columns exist, in multiples of 16; the sums of others are
-// meaningless and nobody reads them.
+// A strip: reduction rows up to `end` of one expert's weights and a tile of its
+// columns, in two halves: side by side, or (a gated activation) gate columns and the
+// up columns they go with, `jump` further right.  `lo` and `hi` of each half's columns
+// exist, in multiples of 16; the sums of others are meaningless and nobody reads them.
 struct Strip {
   int row, col;        // matrix row of reduction row 0; first column
   int end;             // reduction rows
@@ -269,6 +268,8 @@ struct Matrix {
 template <typename T>
 struct Dense16 {
   using Elem = T;
+  static constexpr int kTile = 64;  // columns of a strip
+  static constexpr int kSums = 4;   // a lane's multiplies of 16 columns
   static constexpr int kStep = 32;
   static constexpr bool kGroups = true;  // vectors in groups of 8 columns, of which a unit
                                          // may have fewer
@@ -344,7 +345,8 @@ struct Dense16 {
   // One half of a step for the first G groups of vectors and P of their parts.
   template <int G, int P, int NG, typename Src>
   static __device__ __forceinline__ void half(int h, float (&acc)[4][NG][4], const Lane& l,
-                                              const Matrix&, int left, uint32_t stage, int,
+                                              const Matrix&, const Strip&, int left,
+                                              uint32_t stage, int,
                                               const Vectors<NG, Src>& v) {
     if (16 * h >= left) return;  // rows beyond are another expert's
     uint32_t a[4][4];
@@ -389,15 +391,18 @@ struct Dense16 {
 // leave 4 or 5.)  The fp32 sums carry terms of up to 31 + 24 (fp16: 143 + 136) steps
 // for a weight of up to 8: 2^-19 of the sum of magnitudes at worst.  The sums of each
 // group are scaled as they are added up, so the scales are never rounded into the
-// weights.  One step is 64 rows.
+// weights.  One step is 64 rows of 128 columns: the work beside the codes themselves
+// (copies, vectors, the constant product) is that of 64 columns, and was half of all.
 template <typename T>
 struct Int4 {
   using Elem = T;
+  static constexpr int kTile = 128;
+  static constexpr int kSums = 8;
   static constexpr int kStep = 64;
   static constexpr bool kGroups = true;
-  static constexpr int kStage = 2048 + 2 * 128;  // weights, then scales of two groups
+  static constexpr int kStage = 4096 + 2 * 256;  // weights, then scales of two groups
   template <int NG>
-  static constexpr int kDepth = NG == 1 ? 4 : 3;
+  static constexpr int kDepth = 2;
   template <int NG>
   static constexpr int kTokens = 8 * NG;
   struct Lane {
@@ -434,17 +439,17 @@ struct Int4 {
       expect_bytes(bar, (two ? 36 : 34) * n);
       if (m.gated) {
         bulk_load(stage, w, 32 * lo, bar);
-        bulk_load(stage + 1024, w + 32ll * jump, 32 * hi, bar);
-        bulk_load(stage + 2048, sc, 2 * lo, bar);
-        bulk_load(stage + 2048 + 64, sc + jump, 2 * hi, bar);
+        bulk_load(stage + 2048, w + 32ll * jump, 32 * hi, bar);
+        bulk_load(stage + 4096, sc, 2 * lo, bar);
+        bulk_load(stage + 4096 + 128, sc + jump, 2 * hi, bar);
         if (two) {
-          bulk_load(stage + 2176, sd, 2 * lo, bar);
-          bulk_load(stage + 2176 + 64, sd + jump, 2 * hi, bar);
+          bulk_load(stage + 4352, sd, 2 * lo, bar);
+          bulk_load(stage + 4352 + 128, sd + jump, 2 * hi, bar);
         }
       } else {
         bulk_load(stage, w, 32 * n, bar);
-        bulk_load(stage + 2048, sc, 2 * n, bar);
-        if (two) bulk_load(stage + 2176, sd, 2 * n, bar);
+        bulk_load(stage + 4096, sc, 2 * n, bar);
+        if (two) bulk_load(stage + 4352, sd, 2 * n, bar);
       }
     }
   };
@@ -490,13 +495,14 @@ struct Int4 {
   }
   // One half of a step for the first G groups of vectors and P of their parts.
   template <int G, int P, int NG, typename Src>
-  static __device__ __forceinline__ void half(int h, float (&acc)[4][NG][4], const Lane&,
-                                              const Matrix& m, int left, uint32_t stage,
-                                              int lane, const Vectors<NG, Src>& v) {
+  static __device__ __forceinline__ void half(int h, float (&acc)[kSums][NG][4], const Lane&,
+                                              const Matrix& m, const Strip& s, int left,
+                                              uint32_t stage, int lane,
+                                              const Vectors<NG, Src>& v) {
     if (32 * h >= left) return;
     float minus[G][4] = {};
     const uint32_t minus_op[4] = {kMinus, kMinus, kMinus, kMinus};
-    const uint32_t scales = stage + 2048 + 4 * (lane >> 2) + (h && m.shift == 5 ? 128 : 0);
+    const uint32_t scales = stage + 4096 + 4 * (lane >> 2) + (h && m.shift == 5 ? 256 : 0);
 #pragma unroll
     for (int q = 0; q < 2; ++q)
 #pragma unroll
@@ -505,17 +511,17 @@ struct Int4 {
         for (int n = 0; n < G; ++n)
           mma<T>(minus[n], minus_op, q ? v.b[h][n][p].z : v.b[h][n][p].x,
                  q ? v.b[h][n][p].w : v.b[h][n][p].y);
-    constexpr int kBlocks = G == 1 ? 4 : 2;  // interleaved, as registers allow
 #pragma unroll
-    for (int i0 = 0; i0 < 4; i0 += kBlocks) {
-      uint2 w[kBlocks];
-      float part[kBlocks][G][4];
+    for (int i0 = 0; i0 < kSums; i0 += 4) {  // four blocks interleaved
+      if (i0 >= kSums / 2 && s.hi == 0) break;
+      uint2 w[4];
+      float part[4][G][4];
 #pragma unroll
-      for (int i = 0; i < kBlocks; ++i) w[i] = lds8(stage + 512 * (i0 + i) + 16 * lane + 8 * h);
+      for (int i = 0; i < 4; ++i) w[i] = lds8(stage + 512 * (i0 + i) + 16 * lane + 8 * h);
 #pragma unroll
       for (int q = 0; q < 2; ++q)
 #pragma unroll
-        for (int i = 0; i < kBlocks; ++i) {
+        for (int i = 0; i < 4; ++i) {
           uint32_t a[4];
           operands(a, q ? w[i].y : w[i].x);
 #pragma unroll
@@ -530,7 +536,7 @@ struct Int4 {
             }
         }
 #pragma unroll
-      for (int i = 0; i < kBlocks; ++i) {
+      for (int i = 0; i < 4; ++i) {
         const float2 sc = unpack2<T>(lds4(scales + 32 * (i0 + i)));
 #pragma unroll
         for (int n = 0; n < G; ++n) {
@@ -544,7 +550,7 @@ struct Int4 {
     }
   }
   template <int G, int NG, int LD, bool ADD>
-  static __device__ __forceinline__ void store(const float (&acc)[4][NG][4], int lane, float* red) {
+  static __device__ __forceinline__ void store(const float (&acc)[kSums][NG][4], int lane, float* red) {
     const int g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int n = 0; n < G; ++n)
@@ -552,7 +558,7 @@ struct Int4 {
       for (int j = 0; j < 2; ++j) {
         float* p = red + (8 * n + 2 * t + j) * LD + 2 * g;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kSums; ++i) {
           float2* d = reinterpret_cast<float2*>(p + 16 * i);
           float2 a = make_float2(0.125f * acc[i][n][j], 0.125f * acc[i][n][j + 2]);
           if (ADD) {
@@ -572,6 +578,8 @@ struct Int4 {
 // at the end.
 struct Dense32 {
   using Elem = float;
+  static constexpr int kTile = 64;
+  static constexpr int kSums = 4;
   static constexpr int kStep = 16;
   static constexpr bool kGroups = false;
   static constexpr int kStage = 4096;
@@ -625,8 +633,9 @@ struct Dense32 {
   // One half of a step for the first G groups of vectors and P of their parts.
   template <int G, int P, int NG, typename Src>
   static __device__ __forceinline__ void half(int h, float (&acc)[4][NG][4], const Lane& l,
-                                              const Matrix&, int left, uint32_t stage,
-                                              int lane, const Vectors<NG, Src>& v) {
+                                              const Matrix&, const Strip&, int left,
+                                              uint32_t stage, int lane,
+                                              const Vectors<NG, Src>& v) {
     if (h || 8 * (lane >> 4) >= left) return;  // (one part: all 16 rows)
     float4 w[8];
 #pragma unroll
