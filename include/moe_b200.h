@@ -490,7 +490,7 @@ MOE_API int moe_ep_combine(void* const* peers, int64_t ld_peer, const int32_t* o
 /*
  * Few tokens (decode).  No counterpart in the reference, whose layer pads every
  * expert's rows to a tile; the result is triton_moe/moe.py:148-249's for up to 64
- * tokens, in two launches: router logits (fp32), sigmoid, the top_k largest
+ * tokens, in two launches (four above 8): router logits (fp32), sigmoid, the top_k largest
  * logits (equal ones: lower index; NaN above all, as torch.topk), weights
  * p / (sum p + 1e-20) or p, up product, activation, down product, weighted sum.
  * Sums are fp32 and nothing is rounded before the output, so near-equal logits
@@ -507,6 +507,8 @@ MOE_API int moe_ep_combine(void* const* peers, int64_t ld_peer, const int32_t* o
  *   max_expert_width multiples of 16 up to 32768.  An expert whose offsets leave
  *   the matrices, are no multiples of 16, or exceed max_expert_width adds
  *   nothing and sets MOE_ERR_BAD_ARG in status.
+ *   In fp16 an intermediate above 65504 is infinite; 4-bit products make a NaN of an
+ *   infinite x or intermediate.
  *   workspace: moe_few_tokens_workspace_bytes(...) bytes, 16-byte aligned, any
  *   contents; one per call that may run at the same time.
  * num_tokens = 0 launches nothing.  moe_few_tokens_workspace_bytes returns -1
@@ -554,7 +556,7 @@ MOE_API int moe_int4_dequantize(const void* packed, const void* scales, int64_t 
 
 /*
  * moe_grouped_gemm_up / _down with 4-bit weights, for a few rows an expert (the
- * weights are read once for every 16 rows): down = 0: out [rows, max_expert_width]
+ * weights are read once for every 8 rows): down = 0: out [rows, max_expert_width]
  * = act(x @ w1_e) over x [rows, hidden], total_width columns; down = 1: out [rows,
  * hidden] = x[:, :w_e] @ w2_e over x [rows, max_expert_width], total_width rows,
  * activation NONE.  Every element of out is written; rows of no expert (or beyond

@@ -74,6 +74,10 @@ CASES = [
     (11, 80, [(3, 48), (2, 144)], 2, False, "relu_squared", F32),
     (64, 272, [(33, 16)], 5, True, "none", F32),
     (64, 1024, [(2, 1040)], 2, True, "relu_squared", F32),
+    (64, 64, [(256, 16)], 32, True, "relu_squared", BF),
+    (64, 32, [(256, 16)], 32, True, "relu_squared", F32),
+    # more units a team than its table holds
+    (64, 16, [(80, 32768)], 8, True, "relu_squared", BF),
 ]
 
 

@@ -1,13 +1,15 @@
 """Argument checks of the few-token and 4-bit entry points that need no GPU: the
 C functions refuse before they touch a device."""
 
+import copy
 import ctypes
+import pickle
 
 import pytest
 import torch
 
 from moe_b200._lib import lib
-from moe_b200.kernels import moe_few_tokens, quantize_int4
+from moe_b200.kernels import Int4Weight, moe_few_tokens, quantize_int4
 
 BAD = -1
 
@@ -91,6 +93,7 @@ def gemv(**kw):
     dict(mw=40), dict(act=3), dict(down=1, ldo=64), dict(group=0), dict(group=16), dict(x=None),
     dict(w=None), dict(s=None), dict(tok=None), dict(off=None), dict(out=None), dict(ws=None),
     dict(wsb=100), dict(ldx=48), dict(ldx=65), dict(ldo=16), dict(x=P + 2), dict(blocks=-1),
+    dict(blocks=0), dict(groups=0), dict(group=32),
 ])
 def test_gemv_refuses(kw):
     assert gemv(**kw) == BAD
@@ -112,6 +115,22 @@ def test_quantize_refuses():
     assert lib.moe_int4_pack(P, 64, 64, 40, 64, None, 1, P, None) == BAD
     assert lib.moe_int4_dequantize(P, P, 64, 64, 64, None, 1, P, 64, 2, None) == -2
     assert lib.moe_int4_dequantize(P, None, 64, 64, 64, None, 1, P, 64, 0, None) == BAD
+
+
+def test_weights_copy_and_pickle():
+    rows = (0, 48, 64, 144)  # 1 + 1 + 2 block rows, 2 + 1 + 3 groups of 32
+    q = Int4Weight(torch.randint(0, 256, (4, 2, 512), dtype=torch.uint8),
+                   torch.randn(6, 32).bfloat16(), 144, 32, 32, rows)
+    for c in (copy.deepcopy(q), pickle.loads(pickle.dumps(q)), q.to("cpu")):
+        assert c.shape == (144, 32) and c.group_size == 32 and c.row_offsets == rows
+        assert torch.equal(c.packed, q.packed) and torch.equal(c.scales, q.scales)
+        assert list(c._segments()[0]) == list(rows) and c._segments()[1] == 3
+    with pytest.raises(ValueError, match="packed"):
+        Int4Weight(q.packed[:3], q.scales, 144, 32, 32, rows)
+    with pytest.raises(ValueError, match="scales"):
+        Int4Weight(q.packed, q.scales[:5], 144, 32, 32, rows)
+    with pytest.raises(TypeError, match="bf16"):
+        Int4Weight(q.packed, q.scales.float(), 144, 32, 32, rows)
 
 
 def test_cpu_tensors_are_refused():

@@ -143,6 +143,22 @@ LAYERS = [
     (33, 528, [(5, 80), (2, 272)], 4, True, "relu_squared", BF, 32),
     (64, 64, [(256, 16)], 9, True, "relu_squared", BF, 128),
     (12, 2048, [(16, 320)], 8, True, "swiglu", BF, 128),
+    # final sums shared by several threads, with 64-column tiles
+    (2, 272, [(5, 80), (2, 272)], 4, True, "relu_squared", HF, 64),
+    (3, 528, [(11, 96)], 5, False, "swiglu", BF, 32),
+    (4, 144, [(7, 208)], 3, True, "none", BF, 128),
+    (64, 32, [(256, 16)], 32, True, "relu_squared", BF, 32),
+    # 128-column tiles: 12800 columns or more
+    (1, 256, [(4, 2048), (4, 1616)], 8, True, "relu_squared", BF, 64),
+    (2, 528, [(10, 1360)], 5, True, "relu_squared", HF, 32),
+    (3, 272, [(5, 2720)], 4, False, "swiglu", HF, 32),
+    (4, 1040, [(8, 1616)], 6, True, "swiglu", BF, 128),
+    (6, 1104, [(7, 2016)], 3, False, "none", BF, 128),
+    (8, 2048, [(20, 1024)], 8, True, "relu_squared", BF, 64),
+    (9, 96, [(40, 336)], 5, True, "relu_squared", BF, 64),
+    (33, 336, [(7, 2080), (30, 48)], 6, True, "swiglu", HF, 32),
+    (64, 528, [(3, 4096), (2, 1040), (1, 16)], 2, True, "relu_squared", BF, 64),
+    (64, 64, [(256, 64)], 32, True, "relu_squared", BF, 32),
 ]
 
 
@@ -169,6 +185,13 @@ GROUPED = [
     ([9, 8, 16, 1], 2, 272, [(4, 144)], "swiglu", BF, 128),
     ([2] * 64, 0, 2048, [(64, 64)], "relu_squared", BF, 128),
     ([300, 0, 1], 5, 96, [(3, 48)], "relu_squared", HF, 64),
+    # 128-column tiles in one direction or both
+    ([3] * 20, 0, 768, [(20, 688)], "relu_squared", BF, 64),
+    ([0, 1, 11, 2, 30], 3, 2640, [(2, 2608), (3, 1328)], "swiglu", HF, 32),
+    ([2, 9] * 8, 0, 1040, [(16, 80)], "none", BF, 128),
+    # more units a team than its table holds
+    ([32767], 1, 32, [(1, 640)], "none", BF, 32),
+    ([3100], 0, 32, [(1, 12800)], "relu_squared", BF, 64),
 ]
 
 

@@ -1,5 +1,5 @@
-// The MoE layer for a few tokens (decode), in two kernels, and the products of
-// 4-bit expert weights with rows grouped by expert.
+// The MoE layer for a few tokens (decode), in two kernels (four above 8 tokens), and
+// the products of 4-bit expert weights with rows grouped by expert, in two.
 //
 // Mathematics, for token t and its k experts S(t):
 //   l[t,e] = sum_h x[t,h] Wr[e,h]     S(t) = the k largest l[t,:]
@@ -11,22 +11,23 @@
 // What bounds it: the weights of the experts that the tokens reach are read
 // once from HBM; nothing else is large.  At one token of a small layer the
 // bytes take about a microsecond and the chain launch -> router -> up -> down
-// -> sum is what costs, so there are two launches, no host step and no memset:
+// -> sum is what costs, so there are two launches up to 8 tokens, each able to start
+// while the one before it ends, no host step and no memset:
 //   up kernel    Every cluster of 2 to 8 CTAs computes the routing for itself (each
 //                CTA its part of the hidden size, the sums exchanged over
 //                distributed shared memory): it costs one or two microseconds of
 //                L2 reads and needs no launch and no grid-wide wait of its own.
-//                Then the grid's teams of four warps share the items (expert,
-//                64-column tile, up to 8 NG of its tokens).  Items that do not make
+//                Then the grid's teams of four warps share the items (expert, tile of
+//                64 or 128 columns, 8 or 16 of its tokens).  Items that do not make
 //                a whole wave are cut into slices of the reduction, all in one
 //                cluster; the team that finishes an item's last slice (a counter in
 //                shared memory) adds them in order.  Then the activation, and h.
 //                (More than 8 tokens: a router kernel runs first.)
-//   down kernel  The units (slice of an expert's width, 64-column tile of the
-//                hidden size).  The team that finishes a column tile's last unit
+//   down kernel  The units (slice of an expert's width, tile of the hidden size).  The team that finishes a column tile's last unit
 //                (a counter per tile, zeroed by the up kernel) adds the tile's
 //                partial sums in a fixed order, weights them and writes the
-//                output: results do not depend on timing.
+//                output: results do not depend on timing.  (More than 8 tokens: a
+//                sum kernel after it.)
 // No block waits for another but at hardware barriers and the grid dependency
 // between the two launches; a warp's wait for its own copies is bounded.
 #include <cooperative_groups.h>
@@ -64,7 +65,7 @@ constexpr int kMaxTile = 128;
 template <typename L>
 constexpr int kRedLd = L::kTile + 4;
 constexpr int kMaxSlices = 16;
-constexpr int kMaxDepth = 2;
+constexpr int kMaxDepth = 4;
 constexpr int kAddTokens = 8;     // up to this many, the down kernel writes the output
 constexpr int kMaxWidth = 32768;  // hidden size and expert width: item counts stay 32-bit
 
@@ -315,7 +316,8 @@ __device__ __forceinline__ void run_units(int total, const Matrix& m,
       for (; left > 0; left -= kRows) {  // the vectors of each half load during the half before
         const uint32_t stage = ring + use_slot * L::kStage;
         v.template load<G, P>(1, src, left, lane);
-        if (used < copied) ring_wait(bars + 8 * use_slot, phase, &c.abort);
+        if (used < copied && !ring_wait(bars + 8 * use_slot, phase, &c.abort))
+          more = false;  // (its place may still be written: no further copies)
         L::template half<G, P, NG, Src>(0, acc, at, m, u.strip, left, stage, lane, v);
         v.template advance<G>(kRows);
         v.template load<G, P>(0, src, left - kRows, lane);
@@ -754,7 +756,10 @@ __device__ __forceinline__ void plan_down(const LayerParams& p, const Active& ac
   int widest = 0;
   for (int j = lane; j < active; j += 32) widest = max(widest, act.width[j]);
   widest = __reduce_max_sync(0xffffffffu, widest);
-  const int len = plan_length(max(1, ceil_div(widest, ROUND)), p.down_teams, p.max_slices, p.T <= kAddTokens ? 9 : 8,
+  // a unit's own cost in quarter rounds (4, 8, 12 where no final sum follows: 64 tokens,
+  // 435, 426, 427 us; 9 for 5, 9, 14 with it: 69.5, 68.9, 69.4 at 5 tokens)
+  const int own = p.T <= kAddTokens ? 9 : 8;
+  const int len = plan_length(max(1, ceil_div(widest, ROUND)), p.down_teams, p.max_slices, own,
                               [&](int length) {
     int n = 0;
     for (int j = lane; j < active; j += 32)
@@ -1211,7 +1216,7 @@ struct GroupParams {
   int E, H, total, max_width, act, down;
   int shift, blocks, groups;
   int* plan;           // [PLAN_WORDS], then n, base, width [E] of the active experts
-  float* part;         // [slices][rows][ldp]: 64 columns a tile
+  float* part;         // [slices][rows][ldp]: whole tiles
   long long ldp;
   int max_slices;
   void* out;
@@ -1406,7 +1411,8 @@ __global__ void __launch_bounds__(kThreads)
       const int e = find_item(base_s, active, row);
       if (row >= base_s[e] && row - base_s[e] < n_s[e] && (p.down || c < width_s[e])) {
         const int ns = ceil_div(ceil_div(p.down ? width_s[e] : p.H, kRound), q);
-        const float* src = p.part + row * p.ldp + (gated ? c / (L::kTile / 2) * L::kTile + c % (L::kTile / 2) : c);
+        const float* src = p.part + row * p.ldp +
+                           (gated ? c / (L::kTile / 2) * L::kTile + c % (L::kTile / 2) : c);
         float4 b = v;
 #pragma unroll 4
         for (int z = 0; z < ns; ++z) {
@@ -1514,6 +1520,8 @@ int resident_ctas(K* kernel, std::atomic<int>* known, int size) {
 // larger clusters read less of it; but 8 CTAs fit together on only 120 of 148 SMs
 // (4: 132, 2: all).
 int cluster_size(long long router_bytes) {
+  // (5 tokens, 256 KB: 68.8, 71.4, 71.5 us with 2, 4, 8; one token on 4-bit experts, 1 MB:
+  // 52.3, 44.2, 42.7)
   return router_bytes <= (256 << 10) ? 2 : router_bytes <= (512 << 10) ? 4 : 8;
 }
 
@@ -1550,6 +1558,14 @@ bool weight_map(CUtensorMap* map, const void* w, int dtype, long long rows, long
             : gated    ? CU_TENSOR_MAP_SWIZZLE_64B
                        : CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// 4-bit products in tiles of 128 columns rather than 64: cheaper a weight, but a step
+// takes twice as long, which shows where every team has one or two.  (64 / 128 columns:
+// 33 tokens, 64 experts of 1024, 94 / 85 us; one token, 8 of up to 2048, 42.7 / 41.1; 6
+// tokens, 11 of up to 336, 22.8 / 26.5.)
+bool wide_tiles(long long experts, long long rows, long long cols) {
+  return (rows < experts ? rows : experts) * cols >= 100 * 128;
 }
 
 template <typename L, int NG>
@@ -1618,9 +1634,9 @@ int launch_layer(LayerParams& p, cudaStream_t st) {
   return cudaPeekAtLastError() == cudaSuccess ? kStatusOk : kStatusCuda;
 }
 
-// 8 or 16 columns of vectors a unit: 16 when an expert has more than about 6 rows on
-// average (each further pass over an expert's weights reads them again, from L2).  The
-// 4-bit products, 128 columns wide, have registers for 8.
+// 8 or 16 vectors a unit: 16 when an expert has more than about 6 rows on average (each
+// further pass over an expert's weights reads them again, from L2).  4-bit products have 8:
+// 128 columns of 16 vectors do not fit the registers.
 template <typename L>
 int layer_for_tokens(LayerParams& p, cudaStream_t st) {
   return p.T <= 8 || p.T * p.k <= 6 * p.E ? launch_layer<L, 1>(p, st) : launch_layer<L, 2>(p, st);
@@ -1717,8 +1733,13 @@ int few_tokens(const void* x, long long T, long long ldx, long long H, const voi
   p.max_slices = plan.slices;
   p.status = status;
   if (shift) {
-    if (dtype == 0) return launch_layer<Int4<__nv_bfloat16>, 1>(p, st);
-    if (dtype == 1) return launch_layer<Int4<__half>, 1>(p, st);
+    const bool wide = wide_tiles(E, T * k, act == ACT_SWIGLU ? 2 * max_width : max_width);
+    if (dtype == 0)
+      return wide ? launch_layer<Int4<__nv_bfloat16, 128>, 1>(p, st)
+                  : launch_layer<Int4<__nv_bfloat16, 64>, 1>(p, st);
+    if (dtype == 1)
+      return wide ? launch_layer<Int4<__half, 128>, 1>(p, st)
+                  : launch_layer<Int4<__half, 64>, 1>(p, st);
     return kStatusUnsupported;
   }
   if (dtype < 0 || dtype > 2) return kStatusUnsupported;
@@ -1748,13 +1769,15 @@ int grouped_int4(const void* x, long long rows, long long ldx, const void* w, co
   const int shift = group_shift(group);
   const long long need = grouped_int4_workspace(rows, H, max_width, act, down);
   if (need < 0 || total < 16 || total % 16 != 0 || total > (1ll << 30) || E < 1 ||
-      E > kMaxExperts || shift == 0 || blocks < 0 || groups < 0 || blocks > (1 << 30) || groups > (1 << 30))
+      E > kMaxExperts || shift == 0 || blocks < 0 || groups < 0 || blocks > (1 << 30) ||
+      groups > (1 << 30))
     return kStatusBadArg;
   if (rows == 0) return kStatusOk;
-  if (!x || !w || !s || !tok_off || !off || !out || !ws || ldx < (down ? max_width : H) || ldx % 8 != 0 ||
-      ldo < (down ? H : max_width) || !aligned16(x) || !aligned16(w) || !aligned16(s) ||
+  if (!x || !w || !s || !tok_off || !off || !out || !ws || ldx < (down ? max_width : H) ||
+      ldx % 8 != 0 || ldo < (down ? H : max_width) || !aligned16(x) || !aligned16(w) || !aligned16(s) ||
       !aligned16(ws) || ws_bytes < need)
     return kStatusBadArg;
+  if (!down && (blocks < (H + 63) / 64 || groups < (H + group - 1) / group)) return kStatusBadArg;
   GroupParams p{};
   p.x = x; p.ldx = ldx; p.rows = rows; p.w = w; p.s = s;
   p.tok_off = tok_off; p.tok_cnt = tok_cnt; p.off = off;
@@ -1766,8 +1789,13 @@ int grouped_int4(const void* x, long long rows, long long ldx, const void* w, co
   p.ldp = padded_columns(down ? H : max_width, act);
   p.max_slices = slice_limit(rows * p.ldp);
   p.out = out; p.ldo = ldo; p.status = status;
-  if (dtype == 0) return launch_group<Int4<__nv_bfloat16>, 1>(p, st);
-  if (dtype == 1) return launch_group<Int4<__half>, 1>(p, st);
+  const bool wide = wide_tiles(E, rows, down ? H : act == ACT_SWIGLU ? 2 * max_width : max_width);
+  if (dtype == 0)
+    return wide ? launch_group<Int4<__nv_bfloat16, 128>, 1>(p, st)
+                : launch_group<Int4<__nv_bfloat16, 64>, 1>(p, st);
+  if (dtype == 1)
+    return wide ? launch_group<Int4<__half, 128>, 1>(p, st)
+                : launch_group<Int4<__half, 64>, 1>(p, st);
   return kStatusUnsupported;
 }
 

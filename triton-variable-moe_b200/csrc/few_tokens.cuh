@@ -1,5 +1,5 @@
-// Device pieces of the few-token kernels: a warp's product of a 64-column
-// strip of weights with up to 8 * NG token vectors.
+// Device pieces of the few-token kernels: a warp's product of a strip of weights (64 or
+// 128 columns) with up to 8 * NG token vectors.
 //
 // With few rows per expert the products are bound by reading the weights once
 // (at 8 tokens: 16 flops per 2-byte weight against the ~250 that would balance
@@ -201,7 +201,8 @@ struct RowSource {
 // bf16, 2^-22 in fp16), multiplied one after the other: the intermediate is not
 // rounded to the storage type, and the second multiply is free beside the weight
 // loads.  In fp16 a value above 65504 is infinite, as it is in the layer's
-// forward, which stores it.  A row: [values | remainders].
+// forward, which stores it (and times 4-bit weights a NaN: see Int4).  A row:
+// [values | remainders].
 //
 // A unit of up to 4 vectors holds their remainders in the instruction's other four
 // columns (one multiply for both; `split`), and the sums of columns j and j + 4 are
@@ -389,20 +390,24 @@ struct Dense16 {
 // (Subtracting in the operands instead is exact to the bit but costs another
 // instruction for two codes, where the 1.7 codes a cycle and lane that HBM delivers
 // leave 4 or 5.)  The fp32 sums carry terms of up to 31 + 24 (fp16: 143 + 136) steps
-// for a weight of up to 8: 2^-19 of the sum of magnitudes at worst.  The sums of each
+// for a weight of up to 8: 2^-19 of the sum of magnitudes at worst, and an infinite
+// vector element makes a NaN of every column it meets.  The sums of each
 // group are scaled as they are added up, so the scales are never rounded into the
 // weights.  One step is 64 rows of 128 columns: the work beside the codes themselves
-// (copies, vectors, the constant product) is that of 64 columns, and was half of all.
-template <typename T>
+// (copies, vectors, the constant product) is that of 64 columns, and was half of all;
+// 64 columns where there are few units (see wide_tiles in few_tokens.cu).  Bound by
+// instructions, not bytes: 33 tokens on 64 experts of 2048 x 1024 take 84 us, 1.7 TB/s.
+template <typename T, int TILE>
 struct Int4 {
   using Elem = T;
-  static constexpr int kTile = 128;
-  static constexpr int kSums = 8;
+  static constexpr int kTile = TILE;
+  static constexpr int kSums = TILE / 16;
   static constexpr int kStep = 64;
   static constexpr bool kGroups = true;
-  static constexpr int kStage = 4096 + 2 * 256;  // weights, then scales of two groups
+  static constexpr int kScales = 32 * TILE;  // a step in the ring: weights, then the
+  static constexpr int kStage = kScales + 4 * TILE;  // scales of two groups
   template <int NG>
-  static constexpr int kDepth = 2;
+  static constexpr int kDepth = 256 / TILE;
   template <int NG>
   static constexpr int kTokens = 8 * NG;
   struct Lane {
@@ -439,17 +444,17 @@ struct Int4 {
       expect_bytes(bar, (two ? 36 : 34) * n);
       if (m.gated) {
         bulk_load(stage, w, 32 * lo, bar);
-        bulk_load(stage + 2048, w + 32ll * jump, 32 * hi, bar);
-        bulk_load(stage + 4096, sc, 2 * lo, bar);
-        bulk_load(stage + 4096 + 128, sc + jump, 2 * hi, bar);
+        bulk_load(stage + kScales / 2, w + 32ll * jump, 32 * hi, bar);
+        bulk_load(stage + kScales, sc, 2 * lo, bar);
+        bulk_load(stage + kScales + TILE, sc + jump, 2 * hi, bar);
         if (two) {
-          bulk_load(stage + 4352, sd, 2 * lo, bar);
-          bulk_load(stage + 4352 + 128, sd + jump, 2 * hi, bar);
+          bulk_load(stage + kScales + 2 * TILE, sd, 2 * lo, bar);
+          bulk_load(stage + kScales + 3 * TILE, sd + jump, 2 * hi, bar);
         }
       } else {
         bulk_load(stage, w, 32 * n, bar);
-        bulk_load(stage + 4096, sc, 2 * n, bar);
-        if (two) bulk_load(stage + 4352, sd, 2 * n, bar);
+        bulk_load(stage + kScales, sc, 2 * n, bar);
+        if (two) bulk_load(stage + kScales + 2 * TILE, sd, 2 * n, bar);
       }
     }
   };
@@ -502,7 +507,8 @@ struct Int4 {
     if (32 * h >= left) return;
     float minus[G][4] = {};
     const uint32_t minus_op[4] = {kMinus, kMinus, kMinus, kMinus};
-    const uint32_t scales = stage + 4096 + 4 * (lane >> 2) + (h && m.shift == 5 ? 256 : 0);
+    const uint32_t scales =
+        stage + kScales + 4 * (lane >> 2) + (h && m.shift == 5 ? 2 * TILE : 0);
 #pragma unroll
     for (int q = 0; q < 2; ++q)
 #pragma unroll
@@ -513,7 +519,7 @@ struct Int4 {
                  q ? v.b[h][n][p].w : v.b[h][n][p].y);
 #pragma unroll
     for (int i0 = 0; i0 < kSums; i0 += 4) {  // four blocks interleaved
-      if (i0 >= kSums / 2 && s.hi == 0) break;
+      if (TILE > 64 && i0 >= kSums / 2 && s.hi == 0) break;
       uint2 w[4];
       float part[4][G][4];
 #pragma unroll
@@ -571,6 +577,7 @@ struct Int4 {
       }
   }
 };
+
 // fp32 weights: plain FMAs (the tensor pipe's tf32 would drop 13 bits of both
 // operands).  One step is a box of 16 rows x 64 columns (gated: two of 32): half-warp
 // p takes columns 4c..4c+3 (c = lane % 16) of rows 8p..8p+7; the token values are

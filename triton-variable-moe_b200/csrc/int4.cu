@@ -15,10 +15,12 @@
 // product loads its fragments as they lie, 512 contiguous bytes a warp, and gets the
 // codes to the top of 16-bit mantissas by rotating (few_tokens.cuh).
 //
-// All three are one pass over memory (2.5 bytes a weight at 16 bits) and HBM bound.
+// All three are one pass over memory (2.5 bytes a weight at 16 bits).
 // A CTA takes 128 rows x 64 columns.  Quantising, a thread holds 4 rows x 8 columns
 // (four 16-byte loads, 16 KB in flight a CTA), which are exactly four words of the
 // packed layout; only the group maxima and the finished words go through shared memory.
+// A 2048 x 65536 bf16 weight: quantising 92 us (3.7 TB/s, held by its instructions: the
+// maxima and one rounding a weight), back 65 us (5.2 TB/s), codes packed in 59 us.
 #include <cuda_runtime.h>
 
 #include <cstdint>

@@ -1,4 +1,5 @@
-"""The whole MoE layer for a few tokens (decode), in two launches.
+"""The whole MoE layer for a few tokens (decode), in two launches (four above 8
+tokens).
 
 No counterpart in the reference: its layer (triton_moe/moe.py:148-249) sorts the
 tokens and pads every expert's rows to a tile, which at a few tokens is mostly
@@ -95,12 +96,13 @@ def moe_few_tokens(
     router_weight [E, H]; w1 [H, total width] and w2 [total width, H] with the
     experts side by side at expert_weight_offsets (device, [E + 1]), in bf16, fp16
     or fp32 (fp32 products are fp32, not tf32), or both Int4Weight (x in the
-    scales' bf16 or fp16).  activation "relu_squared", "none" or "swiglu" (then w1
+    scales' bf16 or fp16; w2 quantised with the experts' row offsets).  activation "relu_squared", "none" or "swiglu" (then w1
     holds each expert's gate columns and up columns, the offsets step by 2 w_e and
     w2 has half as many rows as w1 columns).  Hidden size and widths are multiples
     of 16; an expert whose offsets do not fit adds nothing and sets the device
     status word.  In fp16 an intermediate above 65504 is infinite, as in the
-    training forward.  Inference only."""
+    training forward; 4-bit products make a NaN of an infinite x or intermediate.
+    Inference only."""
     dt, dev = x.dtype, x.device
     packed = w1.__class__ is Int4Weight and w2.__class__ is Int4Weight
     if packed:

@@ -10,7 +10,7 @@ scales from elsewhere (a checkpoint quantised by another program), and
 `grouped_gemv_up_int4` / `grouped_gemv_down_int4` stand beside `grouped_gemm_up`
 / `grouped_gemm_down` (same arguments, an Int4Weight in place of the weight) for
 a few rows an expert, as a decode step has: the weights are read once for every
-16 rows of an expert.  The whole layer on 4-bit experts is `moe_few_tokens`.
+8 rows of an expert.  The whole layer on 4-bit experts is `moe_few_tokens`.
 All of it is for inference: nothing here is differentiable.
 """
 
@@ -77,7 +77,7 @@ def row_view(x: torch.Tensor) -> torch.Tensor:
     return x.clone(memory_format=torch.contiguous_format)
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class Int4Weight:
     """A [rows, cols] weight in 4 bits.
 
@@ -116,6 +116,10 @@ class Int4Weight:
         self.__dict__.update(packed=packed, scales=scales, rows=rows, cols=cols,
                              group_size=group_size, row_offsets=row_offsets, _host_offsets=host)
         return self
+
+    def __reduce__(self):  # copies and pickles: all but the host offsets, made again
+        return (Int4Weight, (self.packed, self.scales, self.rows, self.cols, self.group_size,
+                             self.row_offsets))
 
     @property
     def dtype(self) -> torch.dtype:

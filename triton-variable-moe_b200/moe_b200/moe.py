@@ -379,8 +379,8 @@ class TritonMoEMLP(nn.Module):
     def decode(self, x: torch.Tensor,
                experts: tuple[Int4Weight, Int4Weight] | None = None) -> torch.Tensor:
         """The layer's output for a few tokens, for serving: x [..., n_embd] with at
-        most kernels.FEW_TOKENS_MAX (64) tokens in all -> output of x's shape, in two
-        launches (`forward` takes any number of tokens, and gradients and the
+        most kernels.FEW_TOKENS_MAX (64) tokens in all -> output of x's shape, in two to
+        four launches (`forward` takes any number of tokens, and gradients and the
         auxiliary losses, which this does not).  experts: `quantize_experts()`, to
         run on 4-bit expert weights.  Logits, routing weights and the intermediate
         stay fp32, so the result differs from `forward` by that rounding.  Call it
