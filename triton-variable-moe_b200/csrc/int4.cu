@@ -90,24 +90,25 @@ __device__ __forceinline__ float exact_nearest(float w, float s, float quotient)
 // or at least 2^-12 from it; w * inv is within 2^-19 of the quotient; rounding it to
 // steps of 2^-13 first therefore gives halfway exactly when it is, and the second
 // rounding sends that to even.
-__device__ __forceinline__ float nearest(float w, float inv) {
+//
+// The result is the bits of kMagic + the integer: its low bits are the integer's, in two's
+// complement.
+__device__ __forceinline__ uint32_t nearest(float w, float inv) {
   const float step = 1536.f;  // 1.5 x 2^10: the sum's last place is 2^-13
-  return ((fmaf(w, inv, step) - step) + kMagic) - kMagic;
+  return __float_as_uint(fmaf(w, inv, step) + (kMagic - step));
 }
 
-// |w| and maxima of two 16-bit weights, a NaN above all.
+// Maxima of two pairs of magnitudes of 16 bits, a NaN above all.
 template <typename T>
-__device__ __forceinline__ uint32_t abs_max(uint32_t a, uint32_t b);
+__device__ __forceinline__ uint32_t pair_max(uint32_t a, uint32_t b);
 template <>
-__device__ __forceinline__ uint32_t abs_max<__nv_bfloat16>(uint32_t a, uint32_t b) {
-  b &= 0x7fff7fffu;
+__device__ __forceinline__ uint32_t pair_max<__nv_bfloat16>(uint32_t a, uint32_t b) {
   const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a),
                                        *reinterpret_cast<const __nv_bfloat162*>(&b));
   return *reinterpret_cast<const uint32_t*>(&m);
 }
 template <>
-__device__ __forceinline__ uint32_t abs_max<__half>(uint32_t a, uint32_t b) {
-  b &= 0x7fff7fffu;
+__device__ __forceinline__ uint32_t pair_max<__half>(uint32_t a, uint32_t b) {
   const __half2 m =
       __hmax2_nan(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&m);
@@ -192,17 +193,23 @@ __global__ void __launch_bounds__(kThreadsQ)
     uint32_t m[4];  // pairs of columns
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      m[j] = 0;
+      m[j] = v[0].pair(j) & 0x7fff7fffu;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) m[j] = abs_max<T>(m[j], v[i].pair(j));
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1)
-        m[j] = abs_max<T>(m[j], __shfl_xor_sync(0xffffffffu, m[j], o));
+      for (int i = 1; i < 4; ++i) m[j] = pair_max<T>(m[j], v[i].pair(j) & 0x7fff7fffu);
     }
-    uint32_t two = m[0];
+    // each exchange halves the columns that a lane keeps: in the end 2 (r / 2) and the
+    // next, of which it writes column r
+    const bool up = r & 4, right = r & 2;
+    uint32_t keep[2], one;
 #pragma unroll
-    for (int j = 1; j < 4; ++j) two = r >> 1 == j ? m[j] : two;
-    const float2 f = few::unpack2<T>(two);
+    for (int j = 0; j < 2; ++j) {
+      keep[j] = up ? m[j + 2] : m[j];
+      keep[j] = pair_max<T>(keep[j], __shfl_xor_sync(0xffffffffu, up ? m[j] : m[j + 2], 16));
+    }
+    one = right ? keep[1] : keep[0];
+    one = pair_max<T>(one, __shfl_xor_sync(0xffffffffu, right ? keep[0] : keep[1], 8));
+    one = pair_max<T>(one, __shfl_xor_sync(0xffffffffu, one, 4));
+    const float2 f = few::unpack2<T>(one);
     amax[part][c + r] = __float_as_uint(r & 1 ? f.y : f.x);
   }
   __syncthreads();
@@ -228,24 +235,23 @@ __global__ void __launch_bounds__(kThreadsQ)
 #pragma unroll
   for (int j = 0; j < 4; ++j) {  // columns c + 2 j, + 1: lane (g, t) of a block
     // Rows 0 and 2 (of both columns) make the low 16 bits, rows 1 and 3 the high ones:
-    // four numbers -7..7 with weights 1, 16, 256, 4096, and 8 of each, as one integer.
+    // four numbers -7..7 with weights 1, 16, 256, 4096, and 8 of each, modulo 2^16.
     uint32_t half[2];
 #pragma unroll
     for (int o = 0; o < 2; ++o) {
-      float sum = 0.f, weight = 1.f;
+      uint32_t sum = 0x8888u;
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         const int i = o + 2 * (n >> 1), x = n & 1;
         const float value = v[i].get(2 * j + x), f = inv[2 * j + x];
-        float q;
+        uint32_t q;
         if constexpr (sizeof(T) == 4)
-          q = exact_nearest(value, scale[part][c + 2 * j + x], value * f);
+          q = __float_as_uint(exact_nearest(value, scale[part][c + 2 * j + x], value * f) + kMagic);
         else
           q = nearest(value, f);
-        sum = fmaf(q, weight, sum);
-        weight *= 16.f;
+        sum += q << 4 * n;
       }
-      half[o] = __float_as_uint(sum + (kMagic + 34952.f));
+      half[o] = sum;
     }
     uint32_t word = __byte_perm(half[0], half[1], 0x5410);
     word = __funnelshift_l(word, word, 3);
@@ -306,6 +312,29 @@ __global__ void __launch_bounds__(kThreadsQ)
   packed[(static_cast<long long>(at.block + kb) * (N / 16) + col / 16 + nb) * 32 + lane] = out;
 }
 
+// (q - 8) s of two codes, `shift` bits up from bits 3..6 and 19..22 of the word, and two
+// scales.  The codes become the mantissas of B + 8 q (B = 128 in bf16, 1024 in fp16); an
+// eighth of that less B / 8 + 8 is q - 8 exactly, and the product with the scale is
+// rounded once.
+template <typename S>
+__device__ __forceinline__ uint32_t two_values(uint32_t word, int shift, uint32_t s) {
+  const uint32_t codes = __funnelshift_r(word, word, shift) & 0x00780078u;
+  if constexpr (few::kIsBf16<S>) {
+    const uint32_t b = codes | 0x43004300u;
+    const __nv_bfloat162 q =
+        __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&b), __float2bfloat162_rn(0.125f),
+                __float2bfloat162_rn(-24.f));
+    const __nv_bfloat162 r = __hmul2_rn(q, *reinterpret_cast<const __nv_bfloat162*>(&s));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  } else {
+    const uint32_t b = codes | 0x64006400u;
+    const __half2 q = __hfma2(*reinterpret_cast<const __half2*>(&b), __float2half2_rn(0.125f),
+                              __float2half2_rn(-136.f));
+    const __half2 r = __hmul2_rn(q, *reinterpret_cast<const __half2*>(&s));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+}
+
 template <typename S>
 __global__ void __launch_bounds__(kThreadsQ)
     dequantize_kernel(const uint4* __restrict__ packed, const S* __restrict__ scales, int N,
@@ -322,7 +351,7 @@ __global__ void __launch_bounds__(kThreadsQ)
     const uint4 v = few::ld_stream(
         packed + (static_cast<long long>(at.block + kb) * (N / 16) + col / 16 + nb) * 32 + lane);
     const uint32_t* word = reinterpret_cast<const uint32_t*>(&v);
-    float2 s2[2];  // of each 32-row half
+    uint32_t s2[2];  // two columns' scales of each 32-row half
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int r = 64 * kb + 32 * h;
@@ -331,21 +360,22 @@ __global__ void __launch_bounds__(kThreadsQ)
                             scales + static_cast<long long>(at.group + (r >> shift)) * N + col +
                             16 * nb + 2 * g)
                       : 0u;
-      s2[h] = few::unpack2<S>(two);
+      s2[h] = two;
     }
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       const int r0 = 64 * kb + 32 * (s >> 1) + 8 * t + 4 * (s & 1);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float q[2];
+      for (int i = 0; i < 4; i += 2) {  // two rows of two columns
+        uint32_t v[2];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const uint32_t code = __funnelshift_r(word[s], word[s], bit(i, c)) & 15u;
-          q[c] = __uint_as_float(0x4b000000u | code) - 8388616.f;  // 2^23 + code, - 8
-        }
-        tile[(r0 + i) * 32 + 4 * chunk(r0 + i, 2 * nb + (g >> 2)) + (g & 3)] =
-            few::pack2<S>(q[0] * s2[s >> 1].x, q[1] * s2[s >> 1].y);
+        for (int c = 0; c < 2; ++c)
+          v[c] = two_values<S>(word[s], 4 * (i + c),
+                               __byte_perm(s2[s >> 1], 0, c ? 0x3232 : 0x1010));
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+          tile[(r0 + i + n) * 32 + 4 * chunk(r0 + i + n, 2 * nb + (g >> 2)) + (g & 3)] =
+              __byte_perm(v[0], v[1], n ? 0x7632 : 0x5410);
       }
     }
   }
