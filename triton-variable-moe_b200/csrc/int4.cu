@@ -385,8 +385,8 @@ __global__ void __launch_bounds__(kThreadsQ)
   for (int j = 0; j < kRows * PER / kThreadsQ; ++j) {
     const int i = tid + j * kThreadsQ, r = i / PER, c = i % PER;
     if (r < at.rows && 8 * c < cols)
-      *reinterpret_cast<uint4*>(out + static_cast<long long>(at.row + r) * ld + col + 8 * c) =
-          reinterpret_cast<const uint4*>(tile)[r * PER + chunk(r, c)];
+      __stcs(reinterpret_cast<uint4*>(out + static_cast<long long>(at.row + r) * ld + col + 8 * c),
+             reinterpret_cast<const uint4*>(tile)[r * PER + chunk(r, c)]);
   }
 }
 
