@@ -28,6 +28,11 @@
 //                partial sums in a fixed order, weights them and writes the
 //                output: results do not depend on timing.  (More than 8 tokens: a
 //                sum kernel after it.)
+// Measured: one token of 768 on 16 experts 19 us, all latency; 5 tokens on 64 experts of
+// 2048 x 1024 69 us (3.8 TB/s over the call, 5.2 while it streams); 64 tokens of 4096 on
+// 128 experts 424 us, 5.6 TB/s where a copy reaches 6.6.  (Prefetching the down weights to
+// L2 as the up kernel ends: 69.3 to 69.9 us at 16 MB, 73 at 64 MB, as other teams still
+// stream theirs.)
 // No block waits for another but at hardware barriers and the grid dependency
 // between the two launches; a warp's wait for its own copies is bounded.
 #include <cooperative_groups.h>
@@ -1204,6 +1209,10 @@ __global__ void __launch_bounds__(kSumThreads) few_sum_kernel(const __grid_const
 }
 
 // ---- 4-bit products of rows grouped by expert --------------------------------
+// The up or down product by itself: its units are (expert, 8 rows, tile, slice), the
+// slices meet in the sum kernel, which also applies the activation and writes the zeros.
+// Bound by the instructions a code, as the layer's 4-bit products: 192 rows on 64 experts
+// of 1024 x 2048 take 37 us (1.8 TB/s); 6 rows on 16 small experts 10.5, two launches.
 struct GroupParams {
   const void* x;
   long long ldx;
