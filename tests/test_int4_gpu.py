@@ -294,6 +294,61 @@ def test_grouped_offsets_that_do_not_fit(device):
     assert good.shape == (4, 32)
 
 
+def test_layer_offsets_that_do_not_fit_the_packed_weight(device):
+    """w2 packed for other experts than the offsets name: those beyond its blocks add
+    nothing and set the status word."""
+    from moe_b200._lib import MoEKernelError
+    from moe_b200.kernels import check_device_status, moe_few_tokens, quantize_int4
+
+    p = make(5, 64, [(4, 32)], BF)
+    q1, q2, *_ = quantized(p, "relu_squared", 32)
+    off = torch.tensor(p["off"], dtype=torch.int32, device=device)
+    whole = moe_few_tokens(p["x"], p["router"], q1, q2, off, 32, 4)
+    check_device_status(device)
+    # two block rows where the offsets need four
+    other = quantize_int4(p["w2"], 32, row_offsets=[0, 64, 128, 128, 128])
+    out = moe_few_tokens(p["x"], p["router"], q1, other, off, 32, 4)
+    with pytest.raises(MoEKernelError):
+        check_device_status(device)
+    assert bool(torch.isfinite(out).all())
+    assert torch.equal(whole, moe_few_tokens(p["x"], p["router"], q1, q2, off, 32, 4))
+    check_device_status(device)
+
+
+@pytest.mark.parametrize("T", [5, 12])
+def test_not_finite_tokens_reach_no_other(T, device):
+    from moe_b200.kernels import moe_few_tokens
+
+    p = make(T, 128, [(8, 64)], BF, seed=2)
+    q1, q2, *_ = quantized(p, "relu_squared", 64)
+    off = torch.tensor(p["off"], dtype=torch.int32, device=device)
+    clean = moe_few_tokens(p["x"], p["router"], q1, q2, off, 64, 3)
+    x = p["x"].clone()
+    x[1, 7], x[3, 100] = float("nan"), float("inf")
+    out = moe_few_tokens(x, p["router"], q1, q2, off, 64, 3)
+    assert bool(torch.isnan(out[1]).all())
+    # (the others' experts may share passes otherwise than before: within a rounding)
+    keep = [t for t in range(T) if t not in (1, 3)]
+    d = (out[keep].float() - clean[keep].float()).abs()
+    assert bool((d <= 2 * 2.0**-8 * clean[keep].float().abs().amax()).all())
+
+
+def test_offsets_of_other_types_and_strides(device):
+    from moe_b200.kernels import grouped_gemv_up_int4, moe_few_tokens
+
+    p = make(6, 64, [(4, 32)], BF)
+    q1, q2, *_ = quantized(p, "relu_squared", 32)
+    i32 = dict(dtype=torch.int32, device=device)
+    off, tok = torch.tensor(p["off"], **i32), torch.tensor([0, 2, 2, 5, 6], **i32)
+    wid = torch.tensor([32] * 4, **i32)
+    apart = torch.stack([off, off], 1)[:, 0]
+    layer = moe_few_tokens(p["x"], p["router"], q1, q2, off, 32, 2)
+    up = grouped_gemv_up_int4(p["x"], q1, tok, off, wid, None, 32)
+    for o in (off.long(), apart):
+        assert torch.equal(layer, moe_few_tokens(p["x"], p["router"], q1, q2, o, 32, 2))
+        assert torch.equal(up, grouped_gemv_up_int4(p["x"], q1, tok.long(), o, wid, None, 32))
+
+
 def test_graph_capture_of_products(device):
     from moe_b200.kernels import grouped_gemv_up_int4
 
