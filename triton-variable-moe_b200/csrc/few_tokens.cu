@@ -28,7 +28,7 @@
 //                partial sums in a fixed order, weights them and writes the
 //                output: results do not depend on timing.  (More than 8 tokens: a
 //                sum kernel after it.)
-// Measured: one token of 768 on 16 experts 19 us, all latency; 5 tokens on 64 experts of
+// Measured: one token of 768 on 16 experts 18.3 us, all latency; 5 tokens on 64 experts of
 // 2048 x 1024 69 us (3.8 TB/s over the call, 5.2 while it streams); 64 tokens of 4096 on
 // 128 experts 424 us, 5.6 TB/s where a copy reaches 6.6.  (Prefetching the down weights to
 // L2 as the up kernel ends: 69.3 to 69.9 us at 16 MB, 73 at 64 MB, as other teams still
@@ -1108,20 +1108,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         team_sync(team);
         if (!s.last[team]) return;
-        // each thread's slots in order, four at a time, their parts in order
+        // each thread's slots in order, two at a time, their parts in order (four or eight,
+        // or several parts at once, are more loads in flight but more code to fetch: one token
+        // 18.4 us with two, 18.9, 20.1; 5 tokens 69.2, 68.8, 72.2)
         const int lanes = kTeamThreads / share, part = tt / lanes;
         for (int j0 = 0; j0 < p.T * (L::kTile / 4); j0 += lanes) {  // (barriers inside)
           const int j = j0 + tt % lanes, t = j / (L::kTile / 4), c = 4 * (j % (L::kTile / 4));
           const bool in = t < p.T && c < cols;
           float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
           if (in) {
-            for (int a0 = part; a0 < p.k; a0 += 4 * share) {
-              const float* src[4];
-              int parts[4];
-              float4 v[4];
+            for (int a0 = part; a0 < p.k; a0 += 2 * share) {
+              const float* src[2];
+              int parts[2];
+              float4 v[2];
               int longest = 0;
 #pragma unroll
-              for (int n = 0; n < 4; ++n) {
+              for (int n = 0; n < 2; ++n) {
                 const int a = t * p.k + a0 + n * share;
                 v[n] = make_float4(0.f, 0.f, 0.f, 0.f);
                 parts[n] = 0;
@@ -1132,14 +1134,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 longest = max(longest, parts[n]);
               }
-#pragma unroll 2
+#pragma unroll 1
               for (int z = 0; z < longest; ++z)
 #pragma unroll
-                for (int n = 0; n < 4; ++n)
+                for (int n = 0; n < 2; ++n)
                   if (z < parts[n])
                     add4(v[n], __ldcg(reinterpret_cast<const float4*>(src[n] + z * slice)));
 #pragma unroll
-              for (int n = 0; n < 4; ++n) {
+              for (int n = 0; n < 2; ++n) {
                 // (an expert without columns adds nothing, whatever its weight)
                 const float g = parts[n] ? wgt_s[t * p.k + a0 + n * share] : 0.f;
                 o.x = fmaf(g, v[n].x, o.x);
