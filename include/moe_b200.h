@@ -502,11 +502,18 @@ MOE_API int moe_ep_combine(void* const* peers, int64_t ld_peer, const int32_t* o
  *   group = 0: w1, w2 as above; scales NULL.  group = 32, 64 or 128: w1 and w2
  *   packed by moe_int4_quantize / _pack with that group (w1 as one segment, w2
  *   with one segment an expert), scales in dtype (bf16 or fp16); w2_blocks and
- *   w2_groups are moe_int4_rows' of w2.
+ *   w2_groups are moe_int4_rows' of w2, whose segments are taken to be the
+ *   experts' rows as expert_weight_offsets name them.
  *   expert_weight_offsets [E+1], num_experts <= 256, top_k <= 32, hidden and
  *   max_expert_width multiples of 16 up to 32768.  An expert whose offsets leave
  *   the matrices, are no multiples of 16, or exceed max_expert_width adds
- *   nothing and sets MOE_ERR_BAD_ARG in status.
+ *   nothing and sets MOE_ERR_BAD_ARG in status.  With 4-bit weights so does every
+ *   expert after one whose offsets leave w1 or are no multiples of 16, as nothing
+ *   says where its rows of w2 start.
+ * moe_few_tokens_int4 is moe_few_tokens on 4-bit weights with w2's row_offsets
+ * (HOST, num_experts + 1; NULL for a single expert) in place of w2_blocks and
+ * w2_groups: an expert whose offsets are not its rows of w2 adds nothing and sets
+ * the status, and the others are right.
  *   In fp16 an intermediate above 65504 is infinite; 4-bit products make a NaN of an
  *   infinite x or intermediate.
  *   workspace: moe_few_tokens_workspace_bytes(...) bytes, 16-byte aligned, any
@@ -525,6 +532,15 @@ MOE_API int moe_few_tokens(const void* x, int64_t num_tokens, int64_t ld_x, int6
                            int top_k, int normalize, int activation, void* out, int64_t ld_out,
                            void* workspace, int64_t workspace_bytes, int dtype, int* status,
                            void* stream);
+
+MOE_API int moe_few_tokens_int4(const void* x, int64_t num_tokens, int64_t ld_x, int64_t hidden,
+                                const void* router, int num_experts, const void* w1,
+                                const void* w1_scales, const void* w2, const void* w2_scales,
+                                int group, const int32_t* w2_row_offsets, int64_t total_width,
+                                const int32_t* expert_weight_offsets, int64_t max_expert_width,
+                                int top_k, int normalize, int activation, void* out,
+                                int64_t ld_out, void* workspace, int64_t workspace_bytes,
+                                int dtype, int* status, void* stream);
 
 /*
  * 4-bit weights with group scales (no counterpart in the reference).  A weight
@@ -562,7 +578,13 @@ MOE_API int moe_int4_dequantize(const void* packed, const void* scales, int64_t 
  * activation NONE.  Every element of out is written; rows of no expert (or beyond
  * tokens_per_expert, when given) and columns >= w_e are zero.  rows <= 65536,
  * dtype bf16 or fp16 (the scales').  For SwiGLU expert_weight_offsets step by
- * 2 w_e.  blocks and groups: moe_int4_rows' of the weight.  workspace:
+ * 2 w_e.  blocks and groups: moe_int4_rows' of the weight.  An expert whose offsets,
+ * rows or count do not fit gets zeros and sets the status; so does, with down = 1,
+ * every expert after one whose weight offsets do not.
+ * moe_grouped_gemv_down_int4 is down = 1 with the weight's row_offsets (HOST,
+ * num_experts + 1; NULL for a single expert) in place of blocks and groups: each
+ * expert's weight offsets have to be its rows, and no expert depends on another's.
+ * workspace:
  * moe_grouped_gemv_int4_workspace_bytes(...) bytes, as moe_few_tokens' (-1 for
  * sizes out of range).
  */
@@ -578,6 +600,15 @@ MOE_API int moe_grouped_gemv_int4(const void* x, int64_t rows, int64_t ld_x, con
                                   int64_t max_expert_width, int activation, int down, void* out,
                                   int64_t ld_out, void* workspace, int64_t workspace_bytes,
                                   int dtype, int* status, void* stream);
+MOE_API int moe_grouped_gemv_down_int4(const void* x, int64_t rows, int64_t ld_x, const void* w,
+                                       const void* scales, int group, const int32_t* row_offsets,
+                                       int64_t hidden, int64_t total_width,
+                                       const int32_t* expert_token_offsets,
+                                       const int32_t* expert_weight_offsets,
+                                       const int32_t* tokens_per_expert, int num_experts,
+                                       int64_t max_expert_width, void* out, int64_t ld_out,
+                                       void* workspace, int64_t workspace_bytes, int dtype,
+                                       int* status, void* stream);
 
 #ifdef __cplusplus
 }

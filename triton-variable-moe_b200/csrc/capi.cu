@@ -60,8 +60,16 @@ int grouped_int4(const void* x, long long rows, long long ldx, const void* w, co
                  const int* tok_off, const int* off, const int* tok_cnt, int E,
                  long long max_width, int act, int down, void* out, long long ldo, void* ws,
                  long long ws_bytes, int dtype, int* status, cudaStream_t st);
-int int4_rows(long long K, int group, const int32_t* off, int n, long long* blocks,
-              long long* groups);
+int few_tokens_int4(const void* x, long long T, long long ldx, long long H, const void* router,
+                    int E, const void* w1, const void* s1, const void* w2, const void* s2,
+                    int group, const int32_t* rows2, long long total, const int* off,
+                    long long max_width, int k, int norm, int act, void* out, long long ldo,
+                    void* ws, long long ws_bytes, int dtype, int* status, cudaStream_t st);
+int grouped_down_int4(const void* x, long long rows, long long ldx, const void* w, const void* s,
+                      int group, const int32_t* rows_w, long long H, long long total,
+                      const int* tok_off, const int* off, const int* tok_cnt, int E,
+                      long long max_width, void* out, long long ldo, void* ws, long long ws_bytes,
+                      int dtype, int* status, cudaStream_t st);
 int int4_quantize(const void* w, long long K, long long N, long long ld, int w_dtype, int group,
                   const int32_t* off, int n, void* packed, void* scales, int s_dtype,
                   cudaStream_t st);
@@ -276,6 +284,21 @@ int moe_few_tokens(const void* x, int64_t num_tokens, int64_t ld_x, int64_t hidd
                          out, ld_out, workspace, workspace_bytes, dtype, status, S(stream));
 }
 
+int moe_few_tokens_int4(const void* x, int64_t num_tokens, int64_t ld_x, int64_t hidden,
+                        const void* router, int num_experts, const void* w1,
+                        const void* w1_scales, const void* w2, const void* w2_scales, int group,
+                        const int32_t* w2_row_offsets, int64_t total_width,
+                        const int32_t* expert_weight_offsets, int64_t max_expert_width,
+                        int top_k, int normalize, int activation, void* out, int64_t ld_out,
+                        void* workspace, int64_t workspace_bytes, int dtype, int* status,
+                        void* stream) {
+  return moe::few_tokens_int4(x, num_tokens, ld_x, hidden, router, num_experts, w1, w1_scales, w2,
+                              w2_scales, group, w2_row_offsets, total_width,
+                              expert_weight_offsets, max_expert_width, top_k, normalize,
+                              activation, out, ld_out, workspace, workspace_bytes, dtype, status,
+                              S(stream));
+}
+
 int moe_int4_rows(int64_t rows, int group, const int32_t* row_offsets, int num_segments,
                   int64_t* blocks, int64_t* groups) {
   if (!blocks || !groups) return MOE_ERR_BAD_ARG;
@@ -324,6 +347,21 @@ int moe_grouped_gemv_int4(const void* x, int64_t rows, int64_t ld_x, const void*
                            expert_token_offsets, expert_weight_offsets, tokens_per_expert,
                            num_experts, max_expert_width, activation, down, out, ld_out,
                            workspace, workspace_bytes, dtype, status, S(stream));
+}
+
+int moe_grouped_gemv_down_int4(const void* x, int64_t rows, int64_t ld_x, const void* w,
+                               const void* scales, int group, const int32_t* row_offsets,
+                               int64_t hidden, int64_t total_width,
+                               const int32_t* expert_token_offsets,
+                               const int32_t* expert_weight_offsets,
+                               const int32_t* tokens_per_expert, int num_experts,
+                               int64_t max_expert_width, void* out, int64_t ld_out,
+                               void* workspace, int64_t workspace_bytes, int dtype, int* status,
+                               void* stream) {
+  return moe::grouped_down_int4(x, rows, ld_x, w, scales, group, row_offsets, hidden, total_width,
+                                expert_token_offsets, expert_weight_offsets, tokens_per_expert,
+                                num_experts, max_expert_width, out, ld_out, workspace,
+                                workspace_bytes, dtype, status, S(stream));
 }
 
 }  // extern "C"

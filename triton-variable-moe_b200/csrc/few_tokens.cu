@@ -135,6 +135,16 @@ struct LayerParams {
   int* status;
 };
 
+// The rows of a packed w2's segments, an expert each: segment e is rows row[e] ..
+// row[e + 1] - 1 (n = 0: not known, and taken from the call's offsets).
+struct PackedRows {
+  int n;
+  int row[kMaxExperts + 1];
+};
+struct NoRows {};
+template <typename L>
+using RowsOf = std::conditional_t<L::kPacked, PackedRows, NoRows>;
+
 // Exclusive prefix sum over a warp; `total` gets the sum.
 __device__ __forceinline__ int warp_scan(int v, int* total) {
   const int lane = threadIdx.x & 31;
@@ -667,15 +677,61 @@ struct alignas(16) UpSmem {
 };
 static_assert(sizeof(UpSmem) % 16 == 0, "16-byte vectors follow");
 
-// Whether an expert's offsets [a, b) fit the matrices, and its width.
+// Whether an expert's offsets [a, b) are columns of the matrix, and whether the width
+// that they give is one that the call allows.
+__device__ __forceinline__ bool expert_columns(int a, int b, int total, int act) {
+  const int step = (act == ACT_SWIGLU ? 32 : 16) - 1;
+  return a >= 0 && b >= a && b <= total && ((a | b) & step) == 0;
+}
 __device__ __forceinline__ bool expert_width(int a, int b, int total, int max_width, int act,
                                              int* width) {
   const int gated = act == ACT_SWIGLU ? 1 : 0;  // log2
-  const int step = (16 << gated) - 1;
-  const bool ok = a >= 0 && b >= a && b <= total && ((a | b) & step) == 0 &&
-                  (b - a) >> gated <= max_width;
+  const bool ok = expert_columns(a, b, total, act) && (b - a) >> gated <= max_width;
   *width = ok ? (b - a) >> gated : 0;
   return ok;
+}
+
+// One warp: where each expert's rows of a packed w2 start, and whether they are the
+// call's.  Known rows: the expert's offsets have to be its segment's.  Otherwise the
+// segments are those of the offsets, as far as these are columns of w1: nothing says
+// where the experts after others start, and they are refused.
+__device__ __forceinline__ void find_packed(const PackedRows& rows, const int* off, int E, int total,
+                                            int act, int shift, int blocks2, int groups2, int* kb_s,
+                                            int* sg_s, int* fits) {
+  const int lane = threadIdx.x & 31, gated = act == ACT_SWIGLU ? 1 : 0;
+  int kb = 0, sg = 0;
+  bool lost = false;
+#pragma unroll 1
+  for (int e0 = 0; e0 < E; e0 += 32) {
+    const int e = e0 + lane;
+    int a = 0, b = 0, n;
+    if (e < E) {
+      a = off[e];
+      b = off[e + 1];
+    }
+    bool ok;
+    int w;
+    if (rows.n > 0) {
+      const int lo = e < E ? rows.row[e] : 0, hi = e < E ? rows.row[e + 1] : 0;
+      ok = a == lo << gated && b == hi << gated;
+      w = hi - lo;
+    } else {
+      const unsigned bad = __ballot_sync(0xffffffffu, !expert_columns(a, b, total, act));
+      ok = !lost && (bad & ((2u << lane) - 1)) == 0;
+      w = ok ? (b - a) >> gated : 0;
+      lost = lost || bad != 0;
+    }
+    const int blocks = ceil_div(w, 64), groups = group_count(w, shift);
+    const int my_kb = kb + warp_scan(blocks, &n);
+    kb += n;
+    const int my_sg = sg + warp_scan(groups, &n);
+    sg += n;
+    if (e < E) {
+      kb_s[e] = my_kb;
+      sg_s[e] = my_sg;
+      fits[e] = ok && my_kb + blocks <= blocks2 && my_sg + groups <= groups2;
+    }
+  }
 }
 
 // One warp: from the token masks and the offsets, the experts that have rows and
@@ -731,29 +787,6 @@ __device__ __forceinline__ void find_active(const LayerParams& p, UpSmem& s) {
   }
 }
 
-// One warp, while others route: where each expert's rows of a packed w2 start, and
-// whether they lie in it (not when it was quantised for other offsets).
-__device__ __forceinline__ void find_packed(const LayerParams& p, UpSmem& s) {
-  const int lane = threadIdx.x & 31;
-  int kb = 0, sg = 0;
-#pragma unroll 1
-  for (int e0 = 0; e0 < p.E; e0 += 32) {
-    const int e = e0 + lane;
-    int w = 0, total;
-    if (e < p.E) expert_width(s.off[e], s.off[e + 1], p.total, p.max_width, p.act, &w);
-    const int blocks = ceil_div(w, 64), groups = group_count(w, p.shift);
-    const int my_kb = kb + warp_scan(blocks, &total);
-    kb += total;
-    const int my_sg = sg + warp_scan(groups, &total);
-    sg += total;
-    if (e < p.E) {
-      s.kb[e] = my_kb;
-      s.sg[e] = my_sg;
-      s.fits[e] = my_kb + blocks <= p.blocks2 && my_sg + groups <= p.groups2;
-    }
-  }
-}
-
 // One warp: the down kernel's slice length and items, into the workspace.
 template <typename L, int TOK, int ROUND>
 __device__ __forceinline__ void plan_down(const LayerParams& p, const Active& act, int active) {
@@ -790,7 +823,7 @@ __device__ __forceinline__ void plan_down(const LayerParams& p, const Active& ac
 // ---- up kernel ---------------------------------------------------------------
 template <typename L, int NG>
 __global__ void __launch_bounds__(kThreads, 1)
-    few_up_kernel(const __grid_constant__ LayerParams p) {
+    few_up_kernel(const __grid_constant__ LayerParams p, const __grid_constant__ RowsOf<L> rows2) {
   using T = typename L::Elem;
   constexpr int TOK = L::template kTokens<NG>, kRound = kTeam * L::kStep;
   extern __shared__ __align__(1024) unsigned char raw[];
@@ -820,9 +853,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   ring_init<L::template kDepth<NG>>(s.c);
 
   unsigned* mask32 = reinterpret_cast<unsigned*>(s.mask);
+  auto packed = [&]() {  // (one warp, while others route)
+    if constexpr (L::kPacked)
+      if (wid == kWarps - 1)
+        find_packed(rows2, s.off, p.E, p.total, p.act, p.shift, p.blocks2, p.groups2, s.kb, s.sg,
+                    s.fits);
+  };
   if (p.sel) {
     __syncthreads();
-    if (p.shift && wid == kWarps - 1) find_packed(p, s);
+    packed();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     for (int a = tid; a < A; a += kThreads) {
       const int sel = p.sel[a], t = a / p.k;
@@ -837,7 +876,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     partial_logits<T>(p, static_cast<const T*>(p.x), p.T, min(rank * per, p.H),
                       min((rank + 1) * per, p.H), part, log, lde);
     cluster.sync();
-    if (p.shift && wid == kWarps - 1) find_packed(p, s);
+    packed();
     for (int t = rank + p.cluster * wid; t < p.T; t += p.cluster * kWarps) {
       int sel;
       float wgt;
@@ -1240,12 +1279,15 @@ struct alignas(16) GroupSmem {
   int off[kMaxExperts + 1];
   int tok[kMaxExperts + 1];
   int cnt[kMaxExperts];
+  int kb[kMaxExperts];  // as UpSmem's
+  int sg[kMaxExperts];
+  int fits[kMaxExperts];
 };
 static_assert(sizeof(GroupSmem) % 16 == 0, "16-byte vectors follow");
 
 template <typename L, int NG>
 __global__ void __launch_bounds__(kThreads, 1)
-    few_group_kernel(const __grid_constant__ GroupParams p) {
+    few_group_kernel(const __grid_constant__ GroupParams p, const __grid_constant__ PackedRows rows) {
   using T = typename L::Elem;
   constexpr int TOK = L::template kTokens<NG>, kRound = kTeam * L::kStep;
   extern __shared__ __align__(1024) unsigned char raw[];
@@ -1257,37 +1299,33 @@ __global__ void __launch_bounds__(kThreads, 1)
   for (int e = tid; e <= p.E; e += kThreads) {
     s.off[e] = p.off[e];
     s.tok[e] = p.tok_off[e];
-    if (e < p.E) s.cnt[e] = p.tok_cnt ? p.tok_cnt[e] : 0x7fffffff;
+    if (e < p.E) {
+      s.cnt[e] = p.tok_cnt ? p.tok_cnt[e] : 0x7fffffff;
+      s.kb[e] = s.sg[e] = 0;
+      s.fits[e] = 1;
+    }
   }
   ring_init<L::template kDepth<NG>>(s.c);
   __syncthreads();
   const int outputs = 1 << outputs_log2<L>(p.act), teams = gridDim.x * kTeams;
   if (wid == 0) {  // as find_active
-    const int gated = p.act == ACT_SWIGLU ? 2 : 1;
-    int active = 0, kb = 0, sg = 0;
+    if (p.down) {
+      find_packed(rows, s.off, p.E, p.total, p.act, p.shift, p.blocks, p.groups, s.kb, s.sg, s.fits);
+      __syncwarp();
+    }
+    int active = 0;
 #pragma unroll 1
     for (int e0 = 0; e0 < p.E; e0 += 32) {
       const int e = e0 + lane;
-      int n = 0, a = 0, w = 0, lo = 0, total;
+      int n = 0, a = 0, w = 0, lo = 0;
       bool ok = true;
       if (e < p.E) {
         a = s.off[e];
-        const int b = s.off[e + 1], hi = s.tok[e + 1];
         lo = s.tok[e];
-        ok = a >= 0 && b >= a && b <= p.total && a % (16 * gated) == 0 &&
-             (b - a) % (16 * gated) == 0 && (b - a) / gated <= p.max_width && lo >= 0 &&
+        const int hi = s.tok[e + 1];
+        ok = expert_width(a, s.off[e + 1], p.total, p.max_width, p.act, &w) && s.fits[e] && lo >= 0 &&
              hi >= lo && hi <= p.rows && s.cnt[e] >= 0;
-        w = ok ? (b - a) / gated : 0;
         n = ok ? min(hi - lo, s.cnt[e]) : 0;
-      }
-      int my_kb = 0, my_sg = 0;
-      if (p.down) {
-        const int blocks = ceil_div(w, 64), groups = group_count(w, p.shift);
-        my_kb = kb + warp_scan(blocks, &total);
-        kb += total;
-        my_sg = sg + warp_scan(groups, &total);
-        sg += total;
-        if (my_kb + blocks > p.blocks || my_sg + groups > p.groups) ok = false;
       }
       if (!ok && p.status && blockIdx.x == 0) *p.status = kStatusBadArg;
       const bool here = ok && n > 0 && w > 0;
@@ -1299,8 +1337,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         s.c.act.base[at] = lo;
         s.c.act.first[at] = a;
         s.c.act.width[at] = w;
-        s.c.act.kb[at] = my_kb;
-        s.c.act.sg[at] = my_sg;
+        s.c.act.kb[at] = s.kb[e];
+        s.c.act.sg[at] = s.sg[e];
       }
     }
     __syncwarp();
@@ -1580,7 +1618,7 @@ bool wide_tiles(long long experts, long long rows, long long cols) {
 }
 
 template <typename L, int NG>
-int launch_layer(LayerParams& p, cudaStream_t st) {
+int launch_layer(LayerParams& p, const RowsOf<L>& rows2, cudaStream_t st) {
   static std::atomic<unsigned long long> up_ok{0}, down_ok{0};
   static std::atomic<int> resident[64][kMaxCluster + 1];
   const int dev = current_device();
@@ -1630,7 +1668,7 @@ int launch_layer(LayerParams& p, cudaStream_t st) {
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = up_smem;
   cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, up, p) != cudaSuccess) return kStatusCuda;
+  if (cudaLaunchKernelEx(&cfg, up, p, rows2) != cudaSuccess) return kStatusCuda;
   cfg.numAttrs = 1;
   cfg.gridDim = dim3(static_cast<unsigned>(sms));
   cfg.dynamicSmemBytes = down_smem;
@@ -1651,11 +1689,12 @@ int launch_layer(LayerParams& p, cudaStream_t st) {
 // at one token of 768, 161 instead of 152 at 6 rows each for 16 experts of 2048 x 1024).
 template <typename L>
 int layer_for_tokens(LayerParams& p, cudaStream_t st) {
-  return p.T <= 8 || p.T * p.k <= 6 * p.E ? launch_layer<L, 1>(p, st) : launch_layer<L, 2>(p, st);
+  return p.T <= 8 || p.T * p.k <= 6 * p.E ? launch_layer<L, 1>(p, {}, st)
+                                          : launch_layer<L, 2>(p, {}, st);
 }
 
 template <typename L, int NG>
-int launch_group(const GroupParams& p, cudaStream_t st) {
+int launch_group(const GroupParams& p, const PackedRows& rows, cudaStream_t st) {
   static std::atomic<unsigned long long> ok{0};
   const int dev = current_device();
   if (dev < 0) return kStatusCuda;
@@ -1672,7 +1711,7 @@ int launch_group(const GroupParams& p, cudaStream_t st) {
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) return kStatusCuda;
+  if (cudaLaunchKernelEx(&cfg, kernel, p, rows) != cudaSuccess) return kStatusCuda;
   const long long vecs = p.rows * ((p.down ? p.H : p.max_width) / 4);
   long long blocks = (vecs + kThreads - 1) / kThreads;
   if (blocks > 4ll * num_sms()) blocks = 4ll * num_sms();
@@ -1692,6 +1731,19 @@ bool layer_sizes_ok(long long T, long long H, int E, int k, long long max_width,
          max_width % 16 == 0 && max_width <= kMaxWidth && act >= 0 && act <= 2;
 }
 
+// A packed w2's segments from its row offsets (host; null: one segment of all rows), and
+// its block rows and groups.
+int packed_rows(const int32_t* off, int E, long long rows, int group, PackedRows* r,
+                long long* blocks, long long* groups) {
+  if (off == nullptr && E != 1) return kStatusBadArg;
+  if (E < 1 || E > kMaxExperts) return kStatusBadArg;
+  const int rc = int4_rows(rows, group, off, E, blocks, groups);
+  if (rc != kStatusOk) return rc;
+  r->n = E;
+  for (int e = 0; e <= E; ++e) r->row[e] = off ? off[e] : e * static_cast<int>(rows);
+  return kStatusOk;
+}
+
 constexpr long long kGroupHeader = 4 * (PLAN_WORDS + 3 * kMaxExperts);
 static_assert(kGroupHeader % 128 == 0, "partial sums follow");
 
@@ -1704,11 +1756,14 @@ long long few_tokens_workspace(long long T, long long H, int E, int k, long long
       .bytes;
 }
 
-int few_tokens(const void* x, long long T, long long ldx, long long H, const void* router, int E,
-               const void* w1, const void* s1, const void* w2, const void* s2, int group,
-               long long blocks2, long long groups2, long long total, const int* off,
-               long long max_width, int k, int norm, int act, void* out, long long ldo, void* ws,
-               long long ws_bytes, int dtype, int* status, cudaStream_t st) {
+namespace {
+
+int run_layer(const void* x, long long T, long long ldx, long long H, const void* router, int E,
+              const void* w1, const void* s1, const void* w2, const void* s2, int group,
+              long long blocks2, long long groups2, const PackedRows& rows2, long long total,
+              const int* off, long long max_width, int k, int norm, int act, void* out,
+              long long ldo, void* ws, long long ws_bytes, int dtype, int* status,
+              cudaStream_t st) {
   if (!layer_sizes_ok(T, H, E, k, max_width, act)) return kStatusBadArg;
   if (T == 0) return kStatusOk;
   const int shift = group_shift(group);
@@ -1747,11 +1802,11 @@ int few_tokens(const void* x, long long T, long long ldx, long long H, const voi
   if (shift) {
     const bool wide = wide_tiles(E, T * k, act == ACT_SWIGLU ? 2 * max_width : max_width);
     if (dtype == 0)
-      return wide ? launch_layer<Int4<__nv_bfloat16, 128>, 1>(p, st)
-                  : launch_layer<Int4<__nv_bfloat16, 64>, 1>(p, st);
+      return wide ? launch_layer<Int4<__nv_bfloat16, 128>, 1>(p, rows2, st)
+                  : launch_layer<Int4<__nv_bfloat16, 64>, 1>(p, rows2, st);
     if (dtype == 1)
-      return wide ? launch_layer<Int4<__half, 128>, 1>(p, st)
-                  : launch_layer<Int4<__half, 64>, 1>(p, st);
+      return wide ? launch_layer<Int4<__half, 128>, 1>(p, rows2, st)
+                  : launch_layer<Int4<__half, 64>, 1>(p, rows2, st);
     return kStatusUnsupported;
   }
   if (dtype < 0 || dtype > 2) return kStatusUnsupported;
@@ -1761,7 +1816,35 @@ int few_tokens(const void* x, long long T, long long ldx, long long H, const voi
     return kStatusCuda;
   if (dtype == 0) return layer_for_tokens<Dense16<__nv_bfloat16>>(p, st);
   if (dtype == 1) return layer_for_tokens<Dense16<__half>>(p, st);
-  return launch_layer<Dense32, 1>(p, st);
+  return launch_layer<Dense32, 1>(p, {}, st);
+}
+
+}  // namespace
+
+int few_tokens(const void* x, long long T, long long ldx, long long H, const void* router, int E,
+               const void* w1, const void* s1, const void* w2, const void* s2, int group,
+               long long blocks2, long long groups2, long long total, const int* off,
+               long long max_width, int k, int norm, int act, void* out, long long ldo, void* ws,
+               long long ws_bytes, int dtype, int* status, cudaStream_t st) {
+  PackedRows unknown;
+  unknown.n = 0;
+  return run_layer(x, T, ldx, H, router, E, w1, s1, w2, s2, group, blocks2, groups2, unknown, total,
+                   off, max_width, k, norm, act, out, ldo, ws, ws_bytes, dtype, status, st);
+}
+
+int few_tokens_int4(const void* x, long long T, long long ldx, long long H, const void* router,
+                    int E, const void* w1, const void* s1, const void* w2, const void* s2,
+                    int group, const int32_t* rows2, long long total, const int* off,
+                    long long max_width, int k, int norm, int act, void* out, long long ldo,
+                    void* ws, long long ws_bytes, int dtype, int* status, cudaStream_t st) {
+  PackedRows rows;
+  long long blocks = 0, groups = 0;
+  if (act < 0 || act > 2 || total % (act == ACT_SWIGLU ? 32 : 16) != 0) return kStatusBadArg;
+  const int rc = packed_rows(rows2, E, act == ACT_SWIGLU ? total / 2 : total, group, &rows, &blocks,
+                             &groups);
+  if (rc != kStatusOk) return rc;
+  return run_layer(x, T, ldx, H, router, E, w1, s1, w2, s2, group, blocks, groups, rows, total, off,
+                   max_width, k, norm, act, out, ldo, ws, ws_bytes, dtype, status, st);
 }
 
 long long grouped_int4_workspace(long long rows, long long H, long long max_width, int act,
@@ -1773,11 +1856,13 @@ long long grouped_int4_workspace(long long rows, long long H, long long max_widt
   return kGroupHeader + 4ll * slice_limit(rows * cols) * rows * cols;
 }
 
-int grouped_int4(const void* x, long long rows, long long ldx, const void* w, const void* s,
-                 int group, long long blocks, long long groups, long long H, long long total,
-                 const int* tok_off, const int* off, const int* tok_cnt, int E,
-                 long long max_width, int act, int down, void* out, long long ldo, void* ws,
-                 long long ws_bytes, int dtype, int* status, cudaStream_t st) {
+namespace {
+
+int run_group(const void* x, long long rows, long long ldx, const void* w, const void* s,
+              int group, long long blocks, long long groups, const PackedRows& rows_w, long long H,
+              long long total, const int* tok_off, const int* off, const int* tok_cnt, int E,
+              long long max_width, int act, int down, void* out, long long ldo, void* ws,
+              long long ws_bytes, int dtype, int* status, cudaStream_t st) {
   const int shift = group_shift(group);
   const long long need = grouped_int4_workspace(rows, H, max_width, act, down);
   if (need < 0 || total < 16 || total % 16 != 0 || total > (1ll << 30) || E < 1 ||
@@ -1803,12 +1888,38 @@ int grouped_int4(const void* x, long long rows, long long ldx, const void* w, co
   p.out = out; p.ldo = ldo; p.status = status;
   const bool wide = wide_tiles(E, rows, down ? H : act == ACT_SWIGLU ? 2 * max_width : max_width);
   if (dtype == 0)
-    return wide ? launch_group<Int4<__nv_bfloat16, 128>, 1>(p, st)
-                : launch_group<Int4<__nv_bfloat16, 64>, 1>(p, st);
+    return wide ? launch_group<Int4<__nv_bfloat16, 128>, 1>(p, rows_w, st)
+                : launch_group<Int4<__nv_bfloat16, 64>, 1>(p, rows_w, st);
   if (dtype == 1)
-    return wide ? launch_group<Int4<__half, 128>, 1>(p, st)
-                : launch_group<Int4<__half, 64>, 1>(p, st);
+    return wide ? launch_group<Int4<__half, 128>, 1>(p, rows_w, st)
+                : launch_group<Int4<__half, 64>, 1>(p, rows_w, st);
   return kStatusUnsupported;
+}
+
+}  // namespace
+
+int grouped_int4(const void* x, long long rows, long long ldx, const void* w, const void* s,
+                 int group, long long blocks, long long groups, long long H, long long total,
+                 const int* tok_off, const int* off, const int* tok_cnt, int E,
+                 long long max_width, int act, int down, void* out, long long ldo, void* ws,
+                 long long ws_bytes, int dtype, int* status, cudaStream_t st) {
+  PackedRows unknown;
+  unknown.n = 0;
+  return run_group(x, rows, ldx, w, s, group, blocks, groups, unknown, H, total, tok_off, off,
+                   tok_cnt, E, max_width, act, down, out, ldo, ws, ws_bytes, dtype, status, st);
+}
+
+int grouped_down_int4(const void* x, long long rows, long long ldx, const void* w, const void* s,
+                      int group, const int32_t* rows_w, long long H, long long total,
+                      const int* tok_off, const int* off, const int* tok_cnt, int E,
+                      long long max_width, void* out, long long ldo, void* ws, long long ws_bytes,
+                      int dtype, int* status, cudaStream_t st) {
+  PackedRows r;
+  long long blocks = 0, groups = 0;
+  const int rc = packed_rows(rows_w, E, total, group, &r, &blocks, &groups);
+  if (rc != kStatusOk) return rc;
+  return run_group(x, rows, ldx, w, s, group, blocks, groups, r, H, total, tok_off, off, tok_cnt, E,
+                   max_width, ACT_NONE, 1, out, ldo, ws, ws_bytes, dtype, status, st);
 }
 
 }  // namespace moe

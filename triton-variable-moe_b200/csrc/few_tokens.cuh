@@ -272,6 +272,7 @@ struct Dense16 {
   static constexpr int kTile = 64;  // columns of a strip
   static constexpr int kSums = 4;   // a lane's multiplies of 16 columns
   static constexpr int kStep = 32;
+  static constexpr bool kPacked = false;
   static constexpr bool kGroups = true;  // vectors in groups of 8 columns, of which a unit
                                          // may have fewer
   static constexpr int kStage = 4096;  // bytes of a step in the ring
@@ -403,6 +404,7 @@ struct Int4 {
   static constexpr int kTile = TILE;
   static constexpr int kSums = TILE / 16;
   static constexpr int kStep = 64;
+  static constexpr bool kPacked = true;
   static constexpr bool kGroups = true;
   static constexpr int kScales = 32 * TILE;  // a step in the ring: weights, then the
   static constexpr int kStage = kScales + 4 * TILE;  // scales of two groups
@@ -588,6 +590,7 @@ struct Dense32 {
   static constexpr int kTile = 64;
   static constexpr int kSums = 4;
   static constexpr int kStep = 16;
+  static constexpr bool kPacked = false;
   static constexpr bool kGroups = false;
   static constexpr int kStage = 4096;
   template <int NG>

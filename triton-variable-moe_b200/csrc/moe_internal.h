@@ -40,6 +40,11 @@ int run_grouped_gemms(const GemmOperands* ops, const GroupedGemmDesc* gs, const 
 
 int num_sms();
 
+// Block rows and groups of a 4-bit weight of K rows in n segments at the row offsets `off`
+// (null: one segment).
+int int4_rows(long long K, int group, const int32_t* off, int n, long long* blocks,
+              long long* groups);
+
 // Limit (ns) of the grouped GEMM's device-side waits for launches that follow;
 // 0 restores the default.  Returns the previous limit.
 unsigned long long set_wait_ns(unsigned long long ns);

@@ -26,7 +26,7 @@ from .int4 import Int4Weight, eager_only, on_device, refuse_grad, row_view, stre
 FEW_TOKENS_MAX = 64
 
 # What the sizes and types of a call come to, worked out and checked at the first call
-# with them: (group, blocks, groups, columns of w1, workspace bytes, codes).
+# with them: (tokens, hidden, experts, group, columns of w1, workspace bytes, codes).
 _signatures: dict[tuple, tuple] = {}
 
 
@@ -64,7 +64,7 @@ def _signature(x_shape, dt, router_shape, w1, w2, offsets, max_width, top_k, act
     total = w1.shape[1]
     if tuple(w2.shape) != (total // gated, H):
         raise ValueError(f"moe_few_tokens: w2 must be {(total // gated, H)}, got {tuple(w2.shape)}")
-    group = blocks = groups = 0
+    group = 0
     if packed:
         if w1.group_size != w2.group_size:
             raise ValueError("moe_few_tokens: w1 and w2 must have one group size, got "
@@ -73,10 +73,10 @@ def _signature(x_shape, dt, router_shape, w1, w2, offsets, max_width, top_k, act
             raise ValueError("moe_few_tokens: a 4-bit w1 is one segment (no row_offsets)")
         if len(w2.row_offsets or (0, 0)) != E + 1:
             raise ValueError(f"moe_few_tokens: a 4-bit w2 needs row_offsets of its {E} experts")
-        group, blocks, groups = w1.group_size, w2.packed.shape[0], w2.scales.shape[0]
+        group = w1.group_size
     act = ACT_CODE[activation]
     ws_bytes = int(lib.moe_few_tokens_workspace_bytes(T, H, E, top_k, max_width, act))
-    return T, H, E, group, blocks, groups, total, ws_bytes, act, DTYPE_CODE[dt]
+    return T, H, E, group, total, ws_bytes, act, DTYPE_CODE[dt]
 
 
 @eager_only
@@ -99,8 +99,8 @@ def moe_few_tokens(
     scales' bf16 or fp16; w2 quantised with the experts' row offsets).  activation "relu_squared", "none" or "swiglu" (then w1
     holds each expert's gate columns and up columns, the offsets step by 2 w_e and
     w2 has half as many rows as w1 columns).  Hidden size and widths are multiples
-    of 16; an expert whose offsets do not fit adds nothing and sets the device
-    status word.  In fp16 an intermediate above 65504 is infinite, as in the
+    of 16; an expert whose offsets do not fit (with 4-bit weights: are not those that
+    w2 was quantised with) adds nothing and sets the device status word.  In fp16 an intermediate above 65504 is infinite, as in the
     training forward; 4-bit products make a NaN of an infinite x or intermediate.
     Inference only."""
     dt, dev = x.dtype, x.device
@@ -109,8 +109,8 @@ def moe_few_tokens(
         t1, t2 = w1.packed, w2.packed
         key = (x.shape, dt, router_weight.shape, w1.shape, w2.shape, w1.group_size, w2.group_size,
                w1.row_offsets is None or len(w1.row_offsets), w2.row_offsets is None or
-               len(w2.row_offsets), t2.shape, w2.scales.shape, expert_weight_offsets.numel(),
-               max_expert_width, top_k, activation)
+               len(w2.row_offsets), expert_weight_offsets.numel(), max_expert_width, top_k,
+               activation)
     else:
         t1, t2 = w1, w2
         key = (x.shape, dt, router_weight.shape, w1.shape, w2.shape, w1.__class__ is Int4Weight,
@@ -123,7 +123,7 @@ def moe_few_tokens(
         if len(_signatures) >= 4096:
             _signatures.clear()
         _signatures[key] = sig
-    T, H, E, group, blocks, groups, total, ws_bytes, act, dt_code = sig
+    T, H, E, group, total, ws_bytes, act, dt_code = sig
     if not x.is_cuda:
         raise ValueError("moe_b200 kernels need CUDA tensors (no CPU fallback)")
     if router_weight.dtype is not dt or w1.dtype is not dt or w2.dtype is not dt:
@@ -145,16 +145,19 @@ def moe_few_tokens(
     p1, p2, pr = t1.data_ptr(), t2.data_ptr(), router_weight.data_ptr()
     if (p1 | p2 | pr) & 15:
         raise ValueError("moe_few_tokens: weights must be 16-byte aligned")
-    s1 = w1.scales.data_ptr() if packed else None
-    s2 = w2.scales.data_ptr() if packed else None
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     with on_device(dev):
         ev = _ops._ev_begin()
-        rc = lib.moe_few_tokens(
-            x.data_ptr(), T, x.stride(0) if T > 1 else H, H, pr, E, p1, s1, p2, s2, group, blocks,
-            groups, total, off.data_ptr(), max_expert_width, top_k, 1 if norm_topk_prob else 0, act,
-            out.data_ptr(), H, ws.data_ptr(), ws_bytes, dt_code, status_buffer(dev).data_ptr(),
-            stream_of(dev))
+        tail = (total, off.data_ptr(), max_expert_width, top_k, 1 if norm_topk_prob else 0, act,
+                out.data_ptr(), H, ws.data_ptr(), ws_bytes, dt_code, status_buffer(dev).data_ptr(),
+                stream_of(dev))
+        ldx = x.stride(0) if T > 1 else H
+        if packed:
+            rc = lib.moe_few_tokens_int4(
+                x.data_ptr(), T, ldx, H, pr, E, p1, w1.scales.data_ptr(), p2, w2.scales.data_ptr(),
+                group, w2._host_offsets, *tail)
+        else:
+            rc = lib.moe_few_tokens(x.data_ptr(), T, ldx, H, pr, E, p1, None, p2, None, 0, 0, 0, *tail)
         _ops._ev_end(ev, "few_tokens")
     if rc:
         check(rc, "moe_few_tokens")

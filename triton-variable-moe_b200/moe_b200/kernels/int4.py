@@ -316,14 +316,18 @@ def _gemv(name, x, q, tok_off, w_off, expert_widths, tok_cnt, hidden, max_width,
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     with on_device(dev):
         ev = _ev_begin()
-        rc = lib.moe_grouped_gemv_int4(
-            ptr(x), rows, x.stride(0) if rows > 1 else x.shape[1], ptr(q.packed), ptr(q.scales),
-            q.group_size, q.packed.shape[0], q.scales.shape[0], hidden,
-            q.rows if down else q.cols, ptr(tok_off), ptr(w_off), ptr(tok_cnt), E, max_width,
-            ACT_CODE[activation], 1 if down else 0, ptr(out), out_cols, ptr(ws), ws_bytes,
-            DTYPE_CODE[x.dtype], ptr(status_buffer(dev)), stream_of(dev))
+        head = (ptr(x), rows, x.stride(0) if rows > 1 else x.shape[1], ptr(q.packed), ptr(q.scales),
+                q.group_size)
+        offs = (ptr(tok_off), ptr(w_off), ptr(tok_cnt), E, max_width)
+        tail = (ptr(out), out_cols, ptr(ws), ws_bytes, DTYPE_CODE[x.dtype],
+                ptr(status_buffer(dev)), stream_of(dev))
+        if down:
+            rc = lib.moe_grouped_gemv_down_int4(*head, q._host_offsets, hidden, q.rows, *offs, *tail)
+        else:
+            rc = lib.moe_grouped_gemv_int4(*head, q.packed.shape[0], q.scales.shape[0], hidden,
+                                           q.cols, *offs, ACT_CODE[activation], 0, *tail)
         _ev_end(ev, name)
-    check(rc, "moe_grouped_gemv_int4")
+    check(rc, name)
     _count(2)
     return out
 
@@ -365,7 +369,8 @@ def grouped_gemv_down_int4(
     """grouped_gemm_down on 4-bit weights for a few rows an expert:
     out[rows_e] = intermediate[rows_e, :w_e] @ W2_e, zero elsewhere.  w2 is
     quantised with the experts' row offsets; expert_weight_offsets are those
-    offsets on the device."""
+    offsets on the device (an expert with others gets zeros and sets the device
+    status word)."""
     return _gemv("grouped_gemv_down_int4", intermediate, w2, expert_token_offsets,
                  expert_weight_offsets, expert_widths, tokens_per_expert, int(hidden_size),
                  intermediate.shape[1] if intermediate.dim() == 2 else 0, "none", True)
