@@ -386,6 +386,9 @@ class TritonMoEMLP(nn.Module):
         stay fp32, so the result differs from `forward` by that rounding.  Call it
         under torch.no_grad()."""
         w1, w2 = (self.w1, self.w2) if experts is None else experts
+        rows = getattr(w2, "row_offsets", None)
+        if rows is not None and rows != tuple(self.expert_offsets):
+            raise ValueError("decode: the 4-bit w2 has other row offsets than this layer's experts")
         out = moe_few_tokens(x.reshape(-1, x.shape[-1]), self.router.weight, w1, w2,
                              self.expert_weight_offsets_t, self.max_expert_width,
                              self.num_active_experts, self.norm_topk_prob)
