@@ -16,7 +16,7 @@ def host(*off):
 
 
 def few(**kw):
-    a = dict(x=P, T=2, ldx=64, H=64, router=P, E=4, w1=P, s1=P, w2=P, s2=P, group=64,
+    a = dict(x=P, T=2, ldx=64, H=64, router=P, rdt=0, E=4, w1=P, s1=P, w2=P, s2=P, group=64,
              rows=host(0, 32, 64, 96, 128), total=128, off=P, mw=32, k=2, norm=1, act=1, out=P,
              ldo=64, ws=P, wsb=1 << 30, dtype=0, status=None, stream=None)
     a.update(kw)
@@ -35,7 +35,8 @@ def test_few_tokens_int4_refuses(kw):
 
 
 def test_few_tokens_int4_unsupported_types_and_no_tokens():
-    assert few(dtype=2) == -2
+    assert few(dtype=2, rdt=2) == -2
+    assert few(rdt=1) == -2 and few(dtype=1, rdt=0) == -2 and few(dtype=2) == -2
     assert few(T=0) == 0
     assert few(T=0, act=2, rows=host(0, 0, 32, 48, 64)) == 0
     assert few(T=0, E=1, k=1, rows=None) == 0

@@ -1,0 +1,51 @@
+"""decode as a server runs it: layers of other types."""
+
+import pytest
+import torch
+
+from tests import few_reference as ref
+from tests.test_few_tokens_gpu import make_module
+from tests.test_int4_gpu import spread, values
+
+pytestmark = pytest.mark.gpu
+
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.mark.parametrize("T", [1, 7, 30])
+@pytest.mark.parametrize("sdtype", [None, BF, HF])
+def test_decode_of_an_fp32_layer_on_int4_experts(sdtype, T, device):
+    m = make_module([(4, 64), (3, 48)], 128, 2, F32)
+    with torch.no_grad():
+        q = m.quantize_experts(group_size=32, dtype=sdtype)
+        dt = sdtype or BF
+        assert q[0].dtype == q[1].dtype == dt
+        x = torch.randn(T, 128, generator=torch.Generator().manual_seed(2)).to(device, dt)
+        out = m.decode(x, experts=q)
+        assert out.dtype == dt
+        seg = [64] * 4 + [48] * 3
+        c1, s1 = ref.quantize(m.w1, 32, [128], dt)
+        c2, s2 = ref.quantize(m.w2, 32, seg, dt)
+        assert ref.clear_choice(x, m.router.weight, 2)
+        r, b = ref.layer(x, m.router.weight, values(c1, s1, 32, [128]), values(c2, s2, 32, seg),
+                         m.expert_offsets, 2, True, "relu_squared",
+                         ref.int4_terms(spread(s1, 32, [128]), dt),
+                         ref.int4_terms(spread(s2, 32, seg), dt))
+        ref.assert_within(out, r, b, "decode")
+        with pytest.raises(TypeError, match="dtype"):
+            m.decode(x.float(), experts=q)
+
+
+@pytest.mark.parametrize("T", [1, 12])
+def test_fp32_router_is_not_rounded(T, device):
+    """Two router weights that 16 bits would make equal: the larger one wins."""
+    m = make_module([(4, 32)], 64, 1, F32)
+    with torch.no_grad():
+        q = m.quantize_experts(group_size=32, dtype=HF)
+        m.router.weight.zero_()
+        m.router.weight[:, 0] = torch.tensor([0.25, 1.0, 1.0 + 2.0**-13, 0.5], device=device)
+        x = torch.randn(T, 64, generator=torch.Generator().manual_seed(3)).to(device, HF)
+        x[:, 0] = 1.0
+        out = m.decode(x, experts=q)
+        m.router.weight[[0, 1, 3]] = -4.0 * m.router.weight[2]  # expert 2 without a doubt
+        assert torch.equal(out, m.decode(x, experts=q))

@@ -61,8 +61,8 @@ int grouped_int4(const void* x, long long rows, long long ldx, const void* w, co
                  long long max_width, int act, int down, void* out, long long ldo, void* ws,
                  long long ws_bytes, int dtype, int* status, cudaStream_t st);
 int few_tokens_int4(const void* x, long long T, long long ldx, long long H, const void* router,
-                    int E, const void* w1, const void* s1, const void* w2, const void* s2,
-                    int group, const int32_t* rows2, long long total, const int* off,
+                    int router_dtype, int E, const void* w1, const void* s1, const void* w2,
+                    const void* s2, int group, const int32_t* rows2, long long total, const int* off,
                     long long max_width, int k, int norm, int act, void* out, long long ldo,
                     void* ws, long long ws_bytes, int dtype, int* status, cudaStream_t st);
 int grouped_down_int4(const void* x, long long rows, long long ldx, const void* w, const void* s,
@@ -285,15 +285,15 @@ int moe_few_tokens(const void* x, int64_t num_tokens, int64_t ld_x, int64_t hidd
 }
 
 int moe_few_tokens_int4(const void* x, int64_t num_tokens, int64_t ld_x, int64_t hidden,
-                        const void* router, int num_experts, const void* w1,
+                        const void* router, int router_dtype, int num_experts, const void* w1,
                         const void* w1_scales, const void* w2, const void* w2_scales, int group,
                         const int32_t* w2_row_offsets, int64_t total_width,
                         const int32_t* expert_weight_offsets, int64_t max_expert_width,
                         int top_k, int normalize, int activation, void* out, int64_t ld_out,
                         void* workspace, int64_t workspace_bytes, int dtype, int* status,
                         void* stream) {
-  return moe::few_tokens_int4(x, num_tokens, ld_x, hidden, router, num_experts, w1, w1_scales, w2,
-                              w2_scales, group, w2_row_offsets, total_width,
+  return moe::few_tokens_int4(x, num_tokens, ld_x, hidden, router, router_dtype, num_experts, w1,
+                              w1_scales, w2, w2_scales, group, w2_row_offsets, total_width,
                               expert_weight_offsets, max_expert_width, top_k, normalize,
                               activation, out, ld_out, workspace, workspace_bytes, dtype, status,
                               S(stream));

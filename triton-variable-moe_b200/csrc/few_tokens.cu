@@ -106,6 +106,7 @@ struct LayerParams {
   const void* x;
   long long ldx;
   const void* router;
+  int router_fp32;  // the router is fp32 beside 16-bit x (4-bit experts only)
   const void* w1;
   const void* s1;  // 4-bit weights: group scales
   const void* w2;
@@ -512,10 +513,23 @@ __device__ __forceinline__ void partial_logits(const LayerParams& p, const T* x,
   }
 }
 
-template <>
-__device__ __forceinline__ void partial_logits<float>(const LayerParams& p, const float* x,
-                                                      int count, int k_lo, int k_hi, float*,
-                                                      float* log, int lde) {
+// Four neighbouring values as floats.
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p) {
+  if constexpr (sizeof(T) == 4) {
+    return *reinterpret_cast<const float4*>(p);
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    const float2 a = unpack2<T>(v.x), b = unpack2<T>(v.y);
+    return make_float4(a.x, a.y, b.x, b.y);
+  }
+}
+
+// The same with an fp32 router (the layer's own type, or that of a layer whose experts
+// alone were quantised): plain FMAs, as the tensor pipe would round the weight.
+template <typename T>
+__device__ __forceinline__ void partial_logits_fp32(const LayerParams& p, const T* x, int count,
+                                                    int k_lo, int k_hi, float* log, int lde) {
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const float* wr = static_cast<const float*>(p.router);
   const int hi = min(k_hi, p.H);
@@ -530,8 +544,7 @@ __device__ __forceinline__ void partial_logits<float>(const LayerParams& p, cons
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           if (t0 + j < count) {
-            const float4 v =
-                *reinterpret_cast<const float4*>(x + static_cast<long long>(t0 + j) * p.ldx + k);
+            const float4 v = load4<T>(x + static_cast<long long>(t0 + j) * p.ldx + k);
             acc[j] = fmaf(v.x, w.x, acc[j]);
             acc[j] = fmaf(v.y, w.y, acc[j]);
             acc[j] = fmaf(v.z, w.z, acc[j]);
@@ -547,6 +560,12 @@ __device__ __forceinline__ void partial_logits<float>(const LayerParams& p, cons
       }
     }
   }
+}
+template <>
+__device__ __forceinline__ void partial_logits<float>(const LayerParams& p, const float* x,
+                                                      int count, int k_lo, int k_hi, float*,
+                                                      float* log, int lde) {
+  partial_logits_fp32<float>(p, x, count, k_lo, k_hi, log, lde);
 }
 
 // Unsigned order of floats; NaN above all (torch.topk's order).  Never 0.
@@ -631,7 +650,7 @@ __device__ __forceinline__ void choose(const LayerParams& p, cg::cluster_group& 
     choose<8>(p, cluster, log, lde, t, sel, wgt);
 }
 
-// ---- router kernel (more than 8 tokens) ----------------------------------------
+// ---- router kernel (more than 8 tokens, or an fp32 router beside 16-bit x) ---------
 // Every cluster of the up kernel would route all tokens (33 tokens, 64 experts: 7 us);
 // here a cluster of 8 CTAs has 8 of them, each CTA an eighth of the hidden size and
 // then one token to choose for.  The up kernel then needs no clusters and runs on all
@@ -648,8 +667,12 @@ __global__ void __launch_bounds__(kThreads, 1) few_router_kernel(const __grid_co
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int per = ceil_div(ceil_div(p.H, 32), kMaxCluster) * 32;
-  partial_logits<T>(p, static_cast<const T*>(p.x) + t0 * p.ldx, count, min(rank * per, p.H),
-                    min((rank + 1) * per, p.H), part, log, lde);
+  const T* x = static_cast<const T*>(p.x) + t0 * p.ldx;
+  const int k_lo = min(rank * per, p.H), k_hi = min((rank + 1) * per, p.H);
+  if (sizeof(T) == 2 && p.router_fp32)
+    partial_logits_fp32<T>(p, x, count, k_lo, k_hi, log, lde);
+  else
+    partial_logits<T>(p, x, count, k_lo, k_hi, part, log, lde);
   cluster.sync();
   if (rank < count && threadIdx.x < 32) {
     int sel;
@@ -1635,7 +1658,9 @@ int launch_layer(LayerParams& p, const RowsOf<L>& rows2, cudaStream_t st) {
   const size_t down_smem = work + sizeof(Common) + 12 * A;
   if (up_smem > kSmemMax || down_smem > kSmemMax) return kStatusUnsupported;
   using T = typename L::Elem;
-  const bool router = p.T > kAddTokens;
+  // (an fp32 router beside 16-bit x has its own kernel for any number of tokens: in the up
+  // kernel the second form of the logits cost 33 tokens of 2048 84.6 -> 86.0 us unused)
+  const bool router = p.T > kAddTokens || p.router_fp32;
   if (!router) p.sel = nullptr;
   p.cluster = router ? 1 : cluster_size(static_cast<long long>(p.E) * p.H * sizeof(T));
   const int n = resident_ctas(up, &resident[dev][p.cluster], p.cluster), sms = num_sms();
@@ -1758,15 +1783,16 @@ long long few_tokens_workspace(long long T, long long H, int E, int k, long long
 
 namespace {
 
-int run_layer(const void* x, long long T, long long ldx, long long H, const void* router, int E,
-              const void* w1, const void* s1, const void* w2, const void* s2, int group,
-              long long blocks2, long long groups2, const PackedRows& rows2, long long total,
-              const int* off, long long max_width, int k, int norm, int act, void* out,
-              long long ldo, void* ws, long long ws_bytes, int dtype, int* status,
-              cudaStream_t st) {
+int run_layer(const void* x, long long T, long long ldx, long long H, const void* router,
+              int router_dtype, int E, const void* w1, const void* s1, const void* w2,
+              const void* s2, int group, long long blocks2, long long groups2,
+              const PackedRows& rows2, long long total, const int* off, long long max_width, int k,
+              int norm, int act, void* out, long long ldo, void* ws, long long ws_bytes, int dtype,
+              int* status, cudaStream_t st) {
   if (!layer_sizes_ok(T, H, E, k, max_width, act)) return kStatusBadArg;
   if (T == 0) return kStatusOk;
   const int shift = group_shift(group);
+  if (router_dtype != dtype && (shift == 0 || router_dtype != 2)) return kStatusUnsupported;
   const int per16 = dtype == 2 ? 4 : 8;  // elements of a 16-byte vector
   if (!x || !router || !w1 || !w2 || !off || !out || !ws || total < 16 || total % 16 != 0 ||
       total > (1ll << 30) || ldx < H || ldx % per16 != 0 || ldo < H || !aligned16(x) ||
@@ -1779,7 +1805,7 @@ int run_layer(const void* x, long long T, long long ldx, long long H, const void
   if (ws_bytes < plan.bytes || !aligned16(ws)) return kStatusBadArg;
   unsigned char* b = static_cast<unsigned char*>(ws);
   LayerParams p{};
-  p.x = x; p.ldx = ldx; p.router = router;
+  p.x = x; p.ldx = ldx; p.router = router; p.router_fp32 = router_dtype == 2 && dtype != 2;
   p.w1 = w1; p.s1 = s1; p.w2 = w2; p.s2 = s2; p.off = off;
   p.T = static_cast<int>(T); p.H = static_cast<int>(H); p.E = E; p.k = k; p.norm = norm; p.act = act;
   p.total = static_cast<int>(total); p.max_width = static_cast<int>(max_width);
@@ -1828,13 +1854,13 @@ int few_tokens(const void* x, long long T, long long ldx, long long H, const voi
                long long ws_bytes, int dtype, int* status, cudaStream_t st) {
   PackedRows unknown;
   unknown.n = 0;
-  return run_layer(x, T, ldx, H, router, E, w1, s1, w2, s2, group, blocks2, groups2, unknown, total,
-                   off, max_width, k, norm, act, out, ldo, ws, ws_bytes, dtype, status, st);
+  return run_layer(x, T, ldx, H, router, dtype, E, w1, s1, w2, s2, group, blocks2, groups2, unknown,
+                   total, off, max_width, k, norm, act, out, ldo, ws, ws_bytes, dtype, status, st);
 }
 
 int few_tokens_int4(const void* x, long long T, long long ldx, long long H, const void* router,
-                    int E, const void* w1, const void* s1, const void* w2, const void* s2,
-                    int group, const int32_t* rows2, long long total, const int* off,
+                    int router_dtype, int E, const void* w1, const void* s1, const void* w2,
+                    const void* s2, int group, const int32_t* rows2, long long total, const int* off,
                     long long max_width, int k, int norm, int act, void* out, long long ldo,
                     void* ws, long long ws_bytes, int dtype, int* status, cudaStream_t st) {
   PackedRows rows;
@@ -1843,8 +1869,8 @@ int few_tokens_int4(const void* x, long long T, long long ldx, long long H, cons
   const int rc = packed_rows(rows2, E, act == ACT_SWIGLU ? total / 2 : total, group, &rows, &blocks,
                              &groups);
   if (rc != kStatusOk) return rc;
-  return run_layer(x, T, ldx, H, router, E, w1, s1, w2, s2, group, blocks, groups, rows, total, off,
-                   max_width, k, norm, act, out, ldo, ws, ws_bytes, dtype, status, st);
+  return run_layer(x, T, ldx, H, router, router_dtype, E, w1, s1, w2, s2, group, blocks, groups, rows,
+                   total, off, max_width, k, norm, act, out, ldo, ws, ws_bytes, dtype, status, st);
 }
 
 long long grouped_int4_workspace(long long rows, long long H, long long max_width, int act,

@@ -96,8 +96,8 @@ _SIGS = {
     "moe_few_tokens_workspace_bytes": [_L, _L, _I, _I, _L, _I],
     "moe_few_tokens": [_P, _L, _L, _L, _P, _I, _P, _P, _P, _P, _I, _L, _L, _L, _P, _L, _I, _I, _I,
                        _P, _L, _P, _L, _I, _P, _P],
-    "moe_few_tokens_int4": [_P, _L, _L, _L, _P, _I, _P, _P, _P, _P, _I, _P, _L, _P, _L, _I, _I, _I,
-                            _P, _L, _P, _L, _I, _P, _P],
+    "moe_few_tokens_int4": [_P, _L, _L, _L, _P, _I, _I, _P, _P, _P, _P, _I, _P, _L, _P, _L, _I, _I,
+                            _I, _P, _L, _P, _L, _I, _P, _P],
     "moe_int4_rows": [_L, _I, _P, _I, _P, _P],
     "moe_int4_quantize": [_P, _L, _L, _L, _I, _I, _P, _I, _P, _P, _I, _P],
     "moe_int4_pack": [_P, _L, _L, _L, _I, _P, _I, _P, _P],

@@ -96,13 +96,14 @@ def moe_few_tokens(
     router_weight [E, H]; w1 [H, total width] and w2 [total width, H] with the
     experts side by side at expert_weight_offsets (device, [E + 1]), in bf16, fp16
     or fp32 (fp32 products are fp32, not tf32), or both Int4Weight (x in the
-    scales' bf16 or fp16; w2 quantised with the experts' row offsets).  activation "relu_squared", "none" or "swiglu" (then w1
-    holds each expert's gate columns and up columns, the offsets step by 2 w_e and
-    w2 has half as many rows as w1 columns).  Hidden size and widths are multiples
-    of 16; an expert whose offsets do not fit (with 4-bit weights: are not those that
-    w2 was quantised with) adds nothing and sets the device status word.  In fp16 an intermediate above 65504 is infinite, as in the
-    training forward; 4-bit products make a NaN of an infinite x or intermediate.
-    Inference only."""
+    scales' bf16 or fp16, the router in that or fp32; w2 quantised with the experts'
+    row offsets).  activation "relu_squared", "none" or "swiglu" (then w1 holds each
+    expert's gate columns and up columns, the offsets step by 2 w_e and w2 has half as
+    many rows as w1 columns).  Hidden size and widths are multiples of 16; an expert
+    whose offsets do not fit (with 4-bit weights: are not those that w2 was quantised
+    with) adds nothing and sets the device status word.  In fp16 an intermediate above
+    65504 is infinite, as in the training forward; 4-bit products make a NaN of an
+    infinite x or intermediate.  Inference only."""
     dt, dev = x.dtype, x.device
     packed = w1.__class__ is Int4Weight and w2.__class__ is Int4Weight
     if packed:
@@ -126,9 +127,11 @@ def moe_few_tokens(
     T, H, E, group, total, ws_bytes, act, dt_code = sig
     if not x.is_cuda:
         raise ValueError("moe_b200 kernels need CUDA tensors (no CPU fallback)")
-    if router_weight.dtype is not dt or w1.dtype is not dt or w2.dtype is not dt:
+    rdt = router_weight.dtype
+    if w1.dtype is not dt or w2.dtype is not dt or (
+            rdt is not dt and not (packed and rdt is torch.float32)):
         raise TypeError(f"moe_few_tokens: x, router_weight, w1 and w2 must share a dtype, got {dt}, "
-                        f"{router_weight.dtype}, {w1.dtype} and {w2.dtype}")
+                        f"{rdt}, {w1.dtype} and {w2.dtype}")
     idx = x.get_device()
     if (router_weight.get_device() != idx or t1.get_device() != idx or t2.get_device() != idx
             or expert_weight_offsets.get_device() != idx):
@@ -154,12 +157,12 @@ def moe_few_tokens(
         ldx = x.stride(0) if T > 1 else H
         if packed:
             rc = lib.moe_few_tokens_int4(
-                x.data_ptr(), T, ldx, H, pr, E, p1, w1.scales.data_ptr(), p2, w2.scales.data_ptr(),
-                group, w2._host_offsets, *tail)
+                x.data_ptr(), T, ldx, H, pr, DTYPE_CODE[rdt], E, p1, w1.scales.data_ptr(), p2,
+                w2.scales.data_ptr(), group, w2._host_offsets, *tail)
         else:
             rc = lib.moe_few_tokens(x.data_ptr(), T, ldx, H, pr, E, p1, None, p2, None, 0, 0, 0, *tail)
         _ops._ev_end(ev, "few_tokens")
     if rc:
         check(rc, "moe_few_tokens")
-    _ops._count(2 if T <= 8 else 4)
+    _ops._count((2 if T <= 8 else 4) + (T <= 8 and rdt is not dt))
     return out

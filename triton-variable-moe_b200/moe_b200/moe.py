@@ -399,7 +399,7 @@ class TritonMoEMLP(nn.Module):
         """w1 and w2 in 4 bits with group scales, for `decode` (and the kernels'
         grouped_gemv_*_int4); a snapshot: quantise again after the weights change.
         dtype: of the scales and of decode's x (default: the weights'; bf16 for
-        fp32 weights)."""
+        fp32 weights, whose router stays fp32)."""
         return (quantize_int4(self.w1, group_size, dtype=dtype),
                 quantize_int4(self.w2, group_size, row_offsets=self.expert_offsets, dtype=dtype))
 
