@@ -72,9 +72,10 @@ extern "C" {
 MOE_API const char* moe_version(void);
 MOE_API const char* moe_status_string(int status);
 
-/* Time limit, in nanoseconds, of every device-side wait of the grouped-GEMM
- * kernels launched after this call (an mbarrier wait, or a fused up+down
- * launch's wait for its row block of the intermediate); 0 restores the
+/* Time limit, in nanoseconds, of every device-side wait of the grouped-GEMM,
+ * few-token and 4-bit product kernels launched after this call (an mbarrier
+ * wait, or a fused up+down launch's wait for its row block of the
+ * intermediate; a captured launch keeps the limit of its capture); 0 restores the
  * default of 2 s.  A wait that runs out sets MOE_ERR_TIMEOUT in the launch's
  * `status` word, the kernel lets its own copies and MMAs in flight finish,
  * releases its tensor memory and returns; its outputs are then undefined.

@@ -134,6 +134,7 @@ struct LayerParams {
   float* y;                  // [slices][T * k][H]
   int max_slices;
   int* status;
+  unsigned long long wait_ns;  // limit of a wait for copies
 };
 
 // The rows of a packed w2's segments, an expert each: segment e is rows row[e] ..
@@ -243,14 +244,18 @@ __device__ __forceinline__ void down_strip(Strip& s, const Active& a, int e, int
   s.groups = group_count(a.width[e], shift);
 }
 
-// Bounded wait for a phase of a copy barrier.  false: it ran out, here or in
-// another warp (abort).
-__device__ __forceinline__ bool ring_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
-  if (mbar_try_wait(bar, parity)) return true;
+// Bounded wait of a warp for a phase of a copy barrier.  false, for all lanes: it ran
+// out, here or in another warp (abort).
+__device__ __forceinline__ bool ring_wait(uint32_t bar, uint32_t parity, volatile int* abort,
+                                          uint64_t limit) {
+  // A poll may suspend the warp, for longer than a copy takes: not with a limit below that.
+  const bool brief = limit < 1000000;
+  if (__all_sync(0xffffffffu, brief ? mbar_test_wait(bar, parity) : mbar_try_wait(bar, parity)))
+    return true;
   const uint64_t t0 = global_timer_ns();
-  while (!mbar_try_wait(bar, parity)) {
-    if (*abort) return false;
-    if (global_timer_ns() - t0 > MOE_WAIT_NS) {
+  while (!__all_sync(0xffffffffu,
+                     brief ? mbar_test_wait(bar, parity) : mbar_try_wait(bar, parity))) {
+    if (__any_sync(0xffffffffu, *abort || global_timer_ns() - t0 > limit)) {
       *abort = 1;
       return false;
     }
@@ -269,7 +274,7 @@ using Int = std::integral_constant<int, N>;
 template <typename L, int NG, typename MakeUnit, typename MakeSource, typename Finish>
 __device__ __forceinline__ void run_units(int total, const Matrix& m,
                                           unsigned char* work, float* red, Common& c,
-                                          MakeUnit unit, MakeSource source, Finish finish) {
+                                          uint64_t limit, MakeUnit unit, MakeSource source, Finish finish) {
   constexpr int kRows = kTeam * L::kStep, TOK = L::template kTokens<NG>;
   constexpr int D = L::template kDepth<NG>;
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
@@ -292,7 +297,7 @@ __device__ __forceinline__ void run_units(int total, const Matrix& m,
   auto top_up = [&]() {
     while (more && copied - used < D) {
       if (ck >= cend) {
-        more = ++cn < total && !*static_cast<volatile int*>(&c.abort);
+        more = ++cn < total;
         if (more) {
           const Unit cu = nth(cn);
           ck = cu.begin + wr * L::kStep;
@@ -332,8 +337,8 @@ __device__ __forceinline__ void run_units(int total, const Matrix& m,
       for (; left > 0; left -= kRows) {  // the vectors of each half load during the half before
         const uint32_t stage = ring + use_slot * L::kStage;
         v.template load<G, P>(1, src, left, lane);
-        if (used < copied && !ring_wait(bars + 8 * use_slot, phase, &c.abort))
-          more = false;  // (its place may still be written: no further copies)
+        if (used < copied && !ring_wait(bars + 8 * use_slot, phase, &c.abort, limit))
+          more = false;  // (its place may still be written: no further copies of this warp)
         L::template half<G, P, NG, Src>(0, acc, at, m, u.strip, left, stage, lane, v);
         v.template advance<G>(kRows);
         v.template load<G, P>(0, src, left - kRows, lane);
@@ -364,11 +369,14 @@ __device__ __forceinline__ void run_units(int total, const Matrix& m,
     finish(u);
     team_sync(team);
   }
-  // after an abort: copies still in flight land before the block ends
-  for (; used < copied; ++used) {
-    const uint64_t t0 = global_timer_ns();
-    while (!mbar_try_wait(bars + 8 * (used % D), (used / D) & 1) &&
-           global_timer_ns() - t0 <= MOE_WAIT_NS) {
+  // After a wait that ran out: the warp's last copies (the ones before them were waited
+  // for) land before the block ends and its shared memory is another's.
+  if (*static_cast<volatile int*>(&c.abort)) {
+    for (int j = max(0, copied - D); j < copied; ++j) {
+      const uint64_t t0 = global_timer_ns();
+      while (!mbar_try_wait(bars + 8 * (j % D), (j / D) & 1) &&
+             global_timer_ns() - t0 <= MOE_WAIT_NS) {
+      }
     }
   }
 }
@@ -1024,7 +1032,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   const int vecs = 1 << (outputs_log2<L>(p.act) - 2);
   const Matrix m{&p.map1, p.w1, p.s1, p.total, p.shift, p.act == ACT_SWIGLU};
-  run_units<L, NG>(total, m, work, red, s.c, unit, source, [&](const Unit& u) {
+  run_units<L, NG>(total, m, work, red, s.c, p.wait_ns, unit, source, [&](const Unit& u) {
     if (u.local < 0) {
       for (int j = tt; j < u.count * vecs; j += kTeamThreads)
         emit(u, j / vecs, 4 * (j % vecs),
@@ -1144,7 +1152,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     : kTeamThreads / (kVecs * (p.T == 1 ? 1 : p.T == 2 ? 2 : 4));
   const Matrix m{&p.map2, p.w2, p.s2, p.H, p.shift, 0};
   run_units<L, NG>(
-      items * tiles > me ? ceil_div(items * tiles - me, teams) : 0, m, work, red, s, unit, source,
+      items * tiles > me ? ceil_div(items * tiles - me, teams) : 0, m, work, red, s, p.wait_ns, unit,
+      source,
       [&](const Unit& u) {
         const int cols = p.H - u.tile * L::kTile;
         float* y = p.y + u.tile * L::kTile;
@@ -1295,6 +1304,7 @@ struct GroupParams {
   void* out;
   long long ldo;
   int* status;
+  unsigned long long wait_ns;
 };
 
 struct alignas(16) GroupSmem {
@@ -1437,7 +1447,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   float* red = reinterpret_cast<float*>(work + kRingBytes<L, NG>) + team * kRedFloats<L, NG>;
   const Matrix m{nullptr, p.w, p.s, p.down ? p.H : p.total, p.shift, p.act == ACT_SWIGLU};
-  run_units<L, NG>(units > me ? ceil_div(units - me, teams) : 0, m, work, red, s.c, unit, source,
+  run_units<L, NG>(units > me ? ceil_div(units - me, teams) : 0, m, work, red, s.c, p.wait_ns, unit,
+                   source,
                    [&](const Unit& u) {
                      float* dst = p.part +
                                   (static_cast<long long>(u.slice) * p.rows + u.row) * p.ldp +
@@ -1825,6 +1836,7 @@ int run_layer(const void* x, long long T, long long ldx, long long H, const void
   p.y = reinterpret_cast<float*>(b + plan.y);
   p.max_slices = plan.slices;
   p.status = status;
+  p.wait_ns = wait_ns();
   if (shift) {
     const bool wide = wide_tiles(E, T * k, act == ACT_SWIGLU ? 2 * max_width : max_width);
     if (dtype == 0)
@@ -1911,7 +1923,7 @@ int run_group(const void* x, long long rows, long long ldx, const void* w, const
   p.part = reinterpret_cast<float*>(static_cast<unsigned char*>(ws) + kGroupHeader);
   p.ldp = padded_columns(down ? H : max_width, act);
   p.max_slices = slice_limit(rows * p.ldp);
-  p.out = out; p.ldo = ldo; p.status = status;
+  p.out = out; p.ldo = ldo; p.status = status; p.wait_ns = wait_ns();
   const bool wide = wide_tiles(E, rows, down ? H : act == ACT_SWIGLU ? 2 * max_width : max_width);
   if (dtype == 0)
     return wide ? launch_group<Int4<__nv_bfloat16, 128>, 1>(p, rows_w, st)

@@ -1133,6 +1133,7 @@ static std::atomic<unsigned long long> g_wait_ns{MOE_WAIT_NS};
 unsigned long long set_wait_ns(unsigned long long ns) {
   return g_wait_ns.exchange(ns == 0 ? MOE_WAIT_NS : ns);
 }
+unsigned long long wait_ns() { return g_wait_ns.load(); }
 
 int num_sms() {
   static std::atomic<int> cached{0};

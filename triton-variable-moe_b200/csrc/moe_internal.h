@@ -45,8 +45,9 @@ int num_sms();
 int int4_rows(long long K, int group, const int32_t* off, int n, long long* blocks,
               long long* groups);
 
-// Limit (ns) of the grouped GEMM's device-side waits for launches that follow;
-// 0 restores the default.  Returns the previous limit.
+// Limit (ns) of the device-side waits of launches that follow; set: 0 restores the
+// default, and the previous limit is returned.
 unsigned long long set_wait_ns(unsigned long long ns);
+unsigned long long wait_ns();
 
 }  // namespace moe
