@@ -17,6 +17,7 @@ differently.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from .._lib import ACT_CODE, DTYPE_CODE, check, lib
 from . import _ops
@@ -138,8 +139,11 @@ def moe_few_tokens(
         raise ValueError("moe_few_tokens: all tensors must be on one device")
     if not (t1.is_contiguous() and t2.is_contiguous() and router_weight.is_contiguous()):
         raise ValueError("moe_few_tokens: router_weight, w1 and w2 must be contiguous")
-    if torch.is_grad_enabled():
-        refuse_grad("moe_few_tokens", x, router_weight, t1, t2)
+    if torch.is_grad_enabled() or forward_ad._current_level >= 0:
+        if packed:
+            refuse_grad("moe_few_tokens", x, router_weight, w1.scales, w2.scales)
+        else:
+            refuse_grad("moe_few_tokens", x, router_weight, t1, t2)
     out = torch.empty((T, H), dtype=dt, device=dev)
     if T == 0:
         return out

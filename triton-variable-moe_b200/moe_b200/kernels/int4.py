@@ -23,6 +23,7 @@ from contextlib import nullcontext
 from dataclasses import dataclass, field
 
 import torch
+from torch.autograd import forward_ad
 
 from .._lib import ACT_CODE, DTYPE_CODE, check, lib, ptr
 from ._ops import _count, _ev_begin, _ev_end, _meta, status_buffer
@@ -45,7 +46,17 @@ def eager_only(fn):
     return call
 
 
+def refuse_tangent(name: str, *tensors: torch.Tensor) -> None:
+    """Forward-mode derivatives, which torch.no_grad() leaves on."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{name} has no forward-mode derivative, and an argument has a "
+                                   "tangent: pass its primal value")
+
+
 def refuse_grad(name: str, *tensors: torch.Tensor) -> None:
+    refuse_tangent(name, *tensors)
     if torch.is_grad_enabled():
         for t in tensors:
             if t.requires_grad:
@@ -199,6 +210,7 @@ def quantize_int4(w: torch.Tensor, group_size: int = 64, row_offsets: Sequence[i
     K, N = w.shape
     offsets = _offsets_tuple(row_offsets)
     blocks, groups, host = _layout(K, N, group_size, offsets)
+    refuse_tangent("quantize_int4", w)
     w = row_view(w.detach())
     dev = w.device
     packed = torch.empty(blocks, N // 16, 512, dtype=torch.uint8, device=dev)
@@ -229,6 +241,7 @@ def pack_int4(codes: torch.Tensor, scales: torch.Tensor, group_size: int,
     if scales.shape != (groups, N) or scales.device != codes.device:
         raise ValueError(f"scales must be {(groups, N)} on {codes.device}, got "
                          f"{tuple(scales.shape)} on {scales.device}")
+    refuse_tangent("pack_int4", scales)
     codes = row_view(codes)
     scales = scales.detach()
     if not scales.is_contiguous() or scales.data_ptr() % 16:
@@ -252,6 +265,7 @@ def dequantize_int4(q: Int4Weight) -> torch.Tensor:
     if not q.packed.is_cuda:
         raise ValueError("moe_b200 kernels need CUDA tensors (no CPU fallback)")
     out = torch.empty(q.rows, q.cols, dtype=q.dtype, device=q.device)
+    refuse_grad("dequantize_int4", q.scales)
     host, n = q._segments()
     with on_device(q.device):
         ev = _ev_begin()
@@ -303,7 +317,7 @@ def _gemv(name, x, q, tok_off, w_off, expert_widths, tok_cnt, hidden, max_width,
     rows = x.shape[0]
     if rows > MAX_GEMV_ROWS:
         raise ValueError(f"{name}: at most {MAX_GEMV_ROWS} rows, got {rows}")
-    refuse_grad(name, x)
+    refuse_grad(name, x, q.scales)
     dev = x.device
     out_cols = hidden if down else max_width
     out = torch.empty(rows, out_cols, dtype=x.dtype, device=dev)
