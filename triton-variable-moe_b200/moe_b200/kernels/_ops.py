@@ -80,7 +80,9 @@ def status_buffer(device: torch.device) -> torch.Tensor:
     idx = device.index if device.index is not None else torch.cuda.current_device()
     buf = _status_bufs.get(idx)
     if buf is None:
-        buf = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+        # (not an inference tensor: the check that clears it runs anywhere)
+        with torch.inference_mode(False):
+            buf = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
         _status_bufs[idx] = buf
     return buf
 
@@ -444,7 +446,8 @@ def up_down_dep_buffer(device: torch.device, rows: int, num_experts: int) -> tor
                 "it in a CUDA graph (its counter buffer is allocated on first use)")
         if buf is not None:
             _dep_buffers_retired.append(buf)
-        buf = torch.zeros(max(words, 1), dtype=torch.int32, device=device)
+        with torch.inference_mode(False):  # (as the status word)
+            buf = torch.zeros(max(words, 1), dtype=torch.int32, device=device)
         _dep_buffers[device] = buf
     return buf
 
