@@ -84,6 +84,11 @@ MOE_API const char* moe_status_string(int status);
  * returns the previous limit. */
 MOE_API uint64_t moe_set_wait_timeout_ns(uint64_t ns);
 
+/* A zeroed word of the current device for `status` arguments, kept until the
+ * process ends.  Also while a stream is being captured: nothing of it is
+ * recorded (a fill in the graph would clear the word at every replay). */
+MOE_API int moe_status_word_create(int** word);
+
 /* Bytes of device workspace moe_route needs for `num_assignments` top-k
  * assignments over `num_experts` experts. */
 MOE_API int64_t moe_route_workspace_bytes(int64_t num_assignments, int num_experts);

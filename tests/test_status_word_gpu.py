@@ -44,3 +44,26 @@ def test_first_call_in_inference_mode(first_call, device):
         with pytest.raises(MoEKernelError):
             check_device_status(device)
         check_device_status(device)
+
+
+def test_first_call_in_a_capture(first_call, device):
+    """The word is zero before the graph runs, and a replay does not clear what another
+    call has set."""
+    from moe_b200._lib import MoEKernelError
+    from moe_b200.kernels import check_device_status, moe_few_tokens
+
+    p = make(3, 64, [(4, 32)], BF)
+    good = torch.tensor(p["off"], dtype=torch.int32, device=device)
+    bad = torch.tensor([0, 32, 60, 96, 128], dtype=torch.int32, device=device)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = moe_few_tokens(p["x"], p["router"], p["w1"], p["w2"], good, 32, 2)
+    check_device_status(device)
+    moe_few_tokens(p["x"], p["router"], p["w1"], p["w2"], bad, 32, 2)
+    graph.replay()
+    torch.cuda.synchronize()
+    with pytest.raises(MoEKernelError):
+        check_device_status(device)
+    check_device_status(device)
+    assert torch.equal(out, moe_few_tokens(p["x"], p["router"], p["w1"], p["w2"], good, 32, 2))

@@ -127,6 +127,24 @@ uint64_t moe_set_wait_timeout_ns(uint64_t ns) {
   return static_cast<uint64_t>(moe::set_wait_ns(static_cast<unsigned long long>(ns)));
 }
 
+int moe_status_word_create(int** word) {
+  if (!word) return MOE_ERR_BAD_ARG;
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return MOE_ERR_CUDA;
+  int* p = nullptr;
+  cudaStream_t s = nullptr;
+  const bool ok = cudaMalloc(&p, sizeof(int)) == cudaSuccess &&
+                  cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking) == cudaSuccess &&
+                  cudaMemsetAsync(p, 0, sizeof(int), s) == cudaSuccess &&
+                  cudaStreamSynchronize(s) == cudaSuccess;
+  if (s) cudaStreamDestroy(s);
+  if (!ok && p) cudaFree(p);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (!ok) return MOE_ERR_CUDA;
+  *word = p;
+  return MOE_OK;
+}
+
 const char* moe_version(void) { return "moe_b200 0.1 (sm_100a tcgen05)"; }
 
 const char* moe_status_string(int s) {

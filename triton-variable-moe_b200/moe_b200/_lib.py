@@ -46,6 +46,7 @@ _L = c_int64
 _SIGS = {
     "moe_version": [],
     "moe_set_wait_timeout_ns": [ctypes.c_uint64],
+    "moe_status_word_create": [_P],
     "moe_status_string": [_I],
     "moe_route_workspace_bytes": [_L, _I],
     "moe_route": [_P, _I, _L, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _L, _P, _P, _L, _P, _P],

@@ -133,14 +133,6 @@ class EPComm:
             self.handle = None
 
 
-class _CudaArray:
-    """__cuda_array_interface__ of raw device memory (for a torch view)."""
-
-    def __init__(self, ptr: int, shape: tuple, typestr: str):
-        self.__cuda_array_interface__ = {"shape": shape, "typestr": typestr,
-                                         "data": (ptr, False), "version": 3, "strides": None}
-
-
 class SharedBuffer:
     """A device buffer of this rank that every rank of the group maps (CUDA IPC
     over NVLink): `peers` is the device array of the world's base pointers the
@@ -175,7 +167,7 @@ class SharedBuffer:
         es = torch.tensor([], dtype=dtype).element_size()
         if rows * cols * es > self.nbytes:
             raise ValueError("view larger than the shared buffer")
-        raw = torch.as_tensor(_CudaArray(self.ptr, (rows * cols * es // 2,), "<i2"),
+        raw = torch.as_tensor(_ops.CudaArray(self.ptr, (rows * cols * es // 2,), "<i2"),
                               device=self.device)
         return raw.view(dtype).view(rows, cols)
 

@@ -9,6 +9,7 @@ device-side counts).
 
 from __future__ import annotations
 
+import ctypes
 from contextlib import contextmanager
 from dataclasses import dataclass
 
@@ -74,15 +75,30 @@ def _ev_end(start, name: str) -> None:
         _kernel_events.append((name, start, e))
 
 
+class CudaArray:
+    """__cuda_array_interface__ of raw device memory (for a torch view)."""
+
+    def __init__(self, ptr: int, shape: tuple, typestr: str):
+        self.__cuda_array_interface__ = {"shape": shape, "typestr": typestr,
+                                         "data": (ptr, False), "version": 3, "strides": None}
+
+
 def status_buffer(device: torch.device) -> torch.Tensor:
     """Per-device int32 word that kernels set when they detect a device-side
     error (bad expert id, row-capacity overflow, a bounded wait giving up)."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
     buf = _status_bufs.get(idx)
     if buf is None:
+        dev = torch.device("cuda", idx)
         # (not an inference tensor: the check that clears it runs anywhere)
-        with torch.inference_mode(False):
-            buf = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+        with torch.inference_mode(False), torch.cuda.device(dev):
+            if torch.cuda.is_current_stream_capturing():
+                # a zero fill recorded into the graph would clear the word at every replay
+                word = ctypes.c_void_p()
+                check(lib.moe_status_word_create(ctypes.addressof(word)), "moe_status_word_create")
+                buf = torch.as_tensor(CudaArray(word.value, (1,), "<i4"), device=dev)
+            else:
+                buf = torch.zeros(1, dtype=torch.int32, device=dev)
         _status_bufs[idx] = buf
     return buf
 
