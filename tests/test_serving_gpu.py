@@ -1,4 +1,4 @@
-"""decode as a server runs it: layers of other types."""
+"""decode as a server runs it: layers of other types and widths."""
 
 import pytest
 import torch
@@ -49,3 +49,18 @@ def test_fp32_router_is_not_rounded(T, device):
         out = m.decode(x, experts=q)
         m.router.weight[[0, 1, 3]] = -4.0 * m.router.weight[2]  # expert 2 without a doubt
         assert torch.equal(out, m.decode(x, experts=q))
+
+
+@pytest.mark.parametrize("sizes", [[(3, 64), (2, 24)], [(2, 8), (2, 16)]])
+def test_decode_refuses_widths_that_it_cannot_compute(sizes, device):
+    m = make_module(sizes, 64, 2, BF, block=8)
+    x = torch.randn(2, 64, device=device, dtype=BF)
+    with torch.no_grad(), pytest.raises(ValueError, match="multiples of 16"):
+        m.decode(x)
+
+
+def test_decode_of_blocks_of_8_that_make_widths_of_16(device):
+    m, n = (make_module([(2, 16), (3, 48)], 64, 2, BF, block=b) for b in (8, 16))
+    x = torch.randn(5, 64, device=device, dtype=BF)
+    with torch.no_grad():
+        assert torch.equal(m.decode(x), n.decode(x))

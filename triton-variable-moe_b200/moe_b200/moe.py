@@ -381,11 +381,15 @@ class TritonMoEMLP(nn.Module):
         """The layer's output for a few tokens, for serving: x [..., n_embd] with at
         most kernels.FEW_TOKENS_MAX (64) tokens in all -> output of x's shape, in two to
         four launches (`forward` takes any number of tokens, and gradients and the
-        auxiliary losses, which this does not).  experts: `quantize_experts()`, to
-        run on 4-bit expert weights.  Logits, routing weights and the intermediate
+        auxiliary losses, which this does not).  x is in the weights' type (4-bit: the
+        scales'), n_embd and the expert widths are multiples of 16.  experts:
+        `quantize_experts()`, to run on 4-bit expert weights.  Logits, routing weights and the intermediate
         stay fp32, so the result differs from `forward` by that rounding.  Call it
         under torch.no_grad()."""
         w1, w2 = (self.w1, self.w2) if experts is None else experts
+        # (widths are multiples of the block size; the kernels leave out an expert of another)
+        if self.block_size % 16 and any(w % 16 for w in self.expert_widths):
+            raise ValueError("decode: expert widths must be multiples of 16")
         rows = getattr(w2, "row_offsets", None)
         if rows is not None and rows != tuple(self.expert_offsets):
             raise ValueError("decode: the 4-bit w2 has other row offsets than this layer's experts")
