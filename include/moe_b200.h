@@ -499,8 +499,9 @@ MOE_API int moe_ep_combine(void* const* peers, int64_t ld_peer, const int32_t* o
  * tokens, in two launches (four above 8): router logits (fp32), sigmoid, the top_k largest
  * logits (equal ones: lower index; NaN above all, as torch.topk), weights
  * p / (sum p + 1e-20) or p, up product, activation, down product, weighted sum.
- * Sums are fp32 and nothing is rounded before the output, so near-equal logits
- * that the storage type would merge are told apart.
+ * Sums, logits and routing weights are fp32, so near-equal logits that the storage
+ * type would merge are told apart.  The intermediate is exact to 2^-16 relative in
+ * bf16, to 2^-22 relative or 2^-25, whichever is more, in fp16, and fp32 in fp32.
  *   x [num_tokens, hidden], router [num_experts, hidden], w1 [hidden,
  *   total_width], w2 [total_width, hidden] (SwiGLU: [total_width / 2, hidden]),
  *   out [num_tokens, hidden]: one dtype, 16-byte aligned, contiguous but for ld_x

@@ -197,12 +197,15 @@ struct RowSource {
 };
 
 // The layer's intermediate, already activated.  For 16-bit weights each fp32
-// value is held as two 16-bit operands (value and remainder: 2^-16 relative in
-// bf16, 2^-22 in fp16), multiplied one after the other: the intermediate is not
-// rounded to the storage type, and the second multiply is free beside the weight
-// loads.  In fp16 a value above 65504 is infinite, as it is in the layer's
-// forward, which stores it (and times 4-bit weights a NaN: see Int4).  A row:
-// [values | remainders].
+// value is held as two 16-bit operands (value and remainder), multiplied one after
+// the other: the intermediate is not rounded to the storage type's digits, and the
+// second multiply is free beside the weight loads.  bf16 keeps 2^-16 of a value.
+// fp16 keeps 2^-22 of it or 2^-25, whichever is more, as its smallest step is 2^-24:
+// values below 2^-3 have fewer digits and those below 2^-25 are zero (the forward, one
+// fp16 number, keeps 2^-11 or 2^-25; a scale a row would keep more, but its maximum is
+// known only when the whole grid is done: a launch more).  In fp16 a value above 65504
+// is infinite, as it is in the layer's forward, which stores it (and times 4-bit
+// weights a NaN: see Int4).  A row: [values | remainders].
 //
 // A unit of up to 4 vectors holds their remainders in the instruction's other four
 // columns (one multiply for both; `split`), and the sums of columns j and j + 4 are

@@ -8,10 +8,11 @@ FEW_TOKENS_MAX tokens (csrc/few_tokens.cu): routing, up product, activation, dow
 product and weighted sum.  It never synchronises the host and can be captured in
 a CUDA graph.
 
-What differs from the training forward is only rounding: logits, routing weights
-and the intermediate stay fp32 (the forward rounds each to the storage type), so
-two experts whose logits differ by less than that rounding may be ranked
-differently.
+What differs from the training forward is only rounding: logits and routing weights
+stay fp32 (the forward rounds each to the storage type), so two experts whose logits
+differ by less than that rounding may be ranked differently, and the intermediate keeps
+twice the digits of the storage type (2^-16 relative in bf16; in fp16 2^-22 relative or
+2^-25, whichever is more).
 """
 
 from __future__ import annotations
