@@ -522,8 +522,10 @@ MOE_API int moe_ep_combine(void* const* peers, int64_t ld_peer, const int32_t* o
  * w2_groups: an expert whose offsets are not its rows of w2 adds nothing and sets
  * the status, and the others are right.  The router is in router_dtype: dtype or
  * fp32, as in an fp32 layer whose experts alone were quantised.
- *   In fp16 an intermediate above 65504 is infinite; 4-bit products make a NaN of an
- *   infinite x or intermediate.
+ *   In fp16 an intermediate above 65504 is infinite.  4-bit products make a NaN of an
+ *   infinite x or intermediate, and in bf16 can of one from 2^115 on; they are summed
+ *   in fp32 with an error of a few 2^-22 of 55 (fp16: 279) scales times the sum of
+ *   |x|, whatever the codes.
  *   workspace: moe_few_tokens_workspace_bytes(...) bytes, 16-byte aligned, any
  *   contents; one per call that may run at the same time.
  * num_tokens = 0 launches nothing.  moe_few_tokens_workspace_bytes returns -1
@@ -560,7 +562,8 @@ MOE_API int moe_few_tokens_int4(const void* x, int64_t num_tokens, int64_t ld_x,
  * B * (cols / 16) * 512 bytes, scales [S, cols] in scale_dtype.
  *   quantize: scale = amax / 7 rounded to scale_dtype, q = rint(w / scale) + 8
  *   (ties to even) within 0..15; scale_dtype is the weight's, bf16 or fp16 for
- *   fp32 weights.  A group holding a NaN or infinity reads back as NaN.
+ *   fp32 weights.  A group holding a NaN or infinity, or whose scale is above
+ *   scale_dtype's range, reads back as NaN.
  *   pack: the same layout from codes [rows, cols] of one byte (low 4 bits).
  *   dequantize: (q - 8) * scale in dtype (the scales').
  */
@@ -585,7 +588,8 @@ MOE_API int moe_int4_dequantize(const void* packed, const void* scales, int64_t 
  * hidden] = x[:, :w_e] @ w2_e over x [rows, max_expert_width], total_width rows,
  * activation NONE.  Every element of out is written; rows of no expert (or beyond
  * tokens_per_expert, when given) and columns >= w_e are zero.  rows <= 65536,
- * dtype bf16 or fp16 (the scales').  For SwiGLU expert_weight_offsets step by
+ * dtype bf16 or fp16 (the scales'); rounding and infinities as moe_few_tokens'
+ * 4-bit products.  For SwiGLU expert_weight_offsets step by
  * 2 w_e.  blocks and groups: moe_int4_rows' of the weight.  An expert whose offsets,
  * rows or count do not fit gets zeros and sets the status; so does, with down = 1,
  * every expert after one whose weight offsets do not.

@@ -393,14 +393,20 @@ struct Dense16 {
 // product with a constant operand gives it, and the sums start from its negative.
 // (Subtracting in the operands instead is exact to the bit but costs another
 // instruction for two codes, where the 1.7 codes a cycle and lane that HBM delivers
-// leave 4 or 5.)  The fp32 sums carry terms of up to 31 + 24 (fp16: 143 + 136) steps
-// for a weight of up to 8: 2^-19 of the sum of magnitudes at worst, and an infinite
-// vector element makes a NaN of every column it meets.  The sums of each
+// leave 4 or 5.)  The fp32 sums carry terms of up to 31 + 24 = 55 (fp16: 143 + 136 =
+// 279) scales times |x| whatever the code, so their error is a few 2^-22 of
+// 55 (279) scale sum |x| and does not shrink with the weights: a column of codes 8 comes
+// out at that error, not at zero (unless its scale is zero, as a quantised column of
+// zeros has it).  An infinite vector element makes a NaN of every column it meets, and
+// so can bf16 ones from 2^115 on: 192 of them times 32 rows reach fp32's end.  The
+// sums of each
 // group are scaled as they are added up, so the scales are never rounded into the
 // weights.  One step is 64 rows of 128 columns: the work beside the codes themselves
 // (copies, vectors, the constant product) is that of 64 columns, and was half of all;
-// 64 columns where there are few units (see wide_tiles in few_tokens.cu).  Bound by
-// instructions, not bytes: 33 tokens on 64 experts of 2048 x 1024 take 84 us, 1.7 TB/s.
+// 64 columns where there are few units (see wide_tiles in few_tokens.cu).  33 tokens on
+// 64 experts of 2048 x 1024 take 84 us, 1.7 TB/s: not the bytes, and no pipe is full
+// either (ALU 50 to 58 %, issue slots 37 to 45 %); a warp's chain of load, rotate, mask,
+// multiply and scale, with four warps a scheduler, and 10 us before the first product.
 template <typename T, int TILE>
 struct Int4 {
   using Elem = T;

@@ -105,7 +105,7 @@ def moe_few_tokens(
     whose offsets do not fit (with 4-bit weights: are not those that w2 was quantised
     with) adds nothing and sets the device status word.  In fp16 an intermediate above
     65504 is infinite, as in the training forward; 4-bit products make a NaN of an
-    infinite x or intermediate.  Inference only."""
+    infinite x or intermediate, and in bf16 can of one from 2^115 on.  Inference only."""
     dt, dev = x.dtype, x.device
     packed = w1.__class__ is Int4Weight and w2.__class__ is Int4Weight
     if packed:
