@@ -500,7 +500,9 @@ MOE_API int moe_ep_combine(void* const* peers, int64_t ld_peer, const int32_t* o
  * logits (equal ones: lower index; NaN above all, as torch.topk), weights
  * p / (sum p + 1e-20) or p, up product, activation, down product, weighted sum.
  * Sums, logits and routing weights are fp32, so near-equal logits that the storage
- * type would merge are told apart.  The intermediate is exact to 2^-16 relative in
+ * type would merge are told apart, and so are logits whose fp32 sigmoids are equal
+ * (above about 17, below -88), of which the layer's own head takes the lower index.
+ * The intermediate is exact to 2^-16 relative in
  * bf16, to 2^-22 relative or 2^-25, whichever is more, in fp16, and fp32 in fp32.
  *   x [num_tokens, hidden], router [num_experts, hidden], w1 [hidden,
  *   total_width], w2 [total_width, hidden] (SwiGLU: [total_width / 2, hidden]),

@@ -64,3 +64,33 @@ def test_decode_of_blocks_of_8_that_make_widths_of_16(device):
     x = torch.randn(5, 64, device=device, dtype=BF)
     with torch.no_grad():
         assert torch.equal(m.decode(x), n.decode(x))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("logits,k,by_logit,by_sigmoid", [
+    ([30.0, 20.0, 40.0, 0.0], 1, [2], [0]),  # sigmoids 1, 1, 1
+    ([1.0, 25.0, 18.0, 32.0], 2, [3, 1], [1, 2]),
+    ([-200.0, -100.0, -300.0, -90.0], 2, [3, 1], [0, 1]),  # all 0
+    ([3.0, 5.0, 4.0, 1.0], 2, [1, 2], [1, 2]),  # the same choice between them
+])
+def test_ranking_where_sigmoids_saturate(logits, k, by_logit, by_sigmoid, dtype, device):
+    """decode takes the larger logits; forward, among equal sigmoids, the lower index."""
+    m = make_module([(4, 32)], 64, k, dtype)
+    with torch.no_grad():
+        m.router.weight.zero_()
+        m.router.weight[:, 0] = torch.tensor(logits, device=device)
+        x = torch.randn(3, 64, generator=torch.Generator().manual_seed(4)).to(device, dtype)
+        x[:, 0] = 1.0
+        inter = m.forward_with_intermediates(x[None])
+        assert inter["selected_experts"].sort(1).values.tolist() == [sorted(by_sigmoid)] * 3
+        sel, _ = ref.choose(x, m.router.weight, k)
+        assert sel.tolist() == [by_logit] * 3
+        out = m.decode(x)
+        r, b = ref.layer(x, m.router.weight, m.w1, m.w2, m.expert_offsets, k, True, "relu_squared")
+        # Below -88.7 expf(-logit) is infinite in fp32 and the sigmoid 0: it is off by all of
+        # its value, at most exp(-88.7) < 2^-127, and its weight by 2^-127 / 1e-20 (the sum of
+        # the chosen sigmoids is at least 0), times the expert's output.
+        y = torch.stack([(x.double() @ m.w1[:, a:c].double()).clamp(min=0).square() @ m.w2[a:c].double()
+                         for a, c in zip(m.expert_offsets, m.expert_offsets[1:])])
+        b = b + k * (2.0**-127 / 1e-20) * y.abs().amax(0)
+        ref.assert_within(out, r, b, "decode")

@@ -10,9 +10,11 @@ a CUDA graph.
 
 What differs from the training forward is only rounding: logits and routing weights
 stay fp32 (the forward rounds each to the storage type), so two experts whose logits
-differ by less than that rounding may be ranked differently, and the intermediate keeps
-twice the digits of the storage type (2^-16 relative in bf16; in fp16 2^-22 relative or
-2^-25, whichever is more).
+differ by less than that rounding may be ranked differently.  Experts are ranked by logit
+where the forward ranks fp32 sigmoids: those of logits above about 17 are all 1 and of
+logits below -88 all 0, and the forward then takes the lower index however far apart the
+logits are (the weights are the same).  The intermediate keeps twice the digits of the
+storage type (2^-16 relative in bf16; in fp16 2^-22 relative or 2^-25, whichever is more).
 """
 
 from __future__ import annotations

@@ -383,10 +383,12 @@ class TritonMoEMLP(nn.Module):
         four launches (`forward` takes any number of tokens, and gradients and the
         auxiliary losses, which this does not).  x is in the weights' type (4-bit: the
         scales'), n_embd and the expert widths are multiples of 16.  experts:
-        `quantize_experts()`, to run on 4-bit expert weights.  Logits and routing weights stay
-        fp32 and the intermediate keeps twice the digits of the weights' type (in fp16
-        to 2^-25 at best), so the result differs from `forward` by their rounding.
-        Call it under torch.no_grad()."""
+        `quantize_experts()`, to run on 4-bit expert weights.  Logits and routing weights
+        stay fp32 and the intermediate keeps twice the digits of the weights' type (in
+        fp16 to 2^-25 at best), so the result differs from `forward` by their rounding.
+        Experts are ranked by logit: where the fp32 sigmoids that `forward` ranks are
+        equal (logits above about 17 or below -88), `forward` takes the lower index and
+        decode the larger logit.  Call it under torch.no_grad()."""
         w1, w2 = (self.w1, self.w2) if experts is None else experts
         # (widths are multiples of the block size; the kernels leave out an expert of another)
         if self.block_size % 16 and any(w % 16 for w in self.expert_widths):
