@@ -23,25 +23,35 @@ def evict(device):
 
 
 def runs_out(run, evict, device):
+    """Three launches whose waits run out, of at most 20: not every launch has a warp that
+    looks for weights before they are there (4 bits: 9 in 10; it loads its tokens first)."""
     from moe_b200._lib import MoEKernelError, lib
     from moe_b200.kernels import check_device_status
 
     want = run()
     check_device_status(device)
-    for _ in range(3):
+    out_of_time = 0
+    for _ in range(20):
         evict()
         torch.cuda.synchronize()
         lib.moe_set_wait_timeout_ns(1)
         try:
-            run()
+            got = run()
             torch.cuda.synchronize()  # the launch returned on its own
         finally:
             lib.moe_set_wait_timeout_ns(0)
-        with pytest.raises(MoEKernelError, match="timed out"):
+        try:
             check_device_status(device)
+            assert torch.equal(got, want)
+        except MoEKernelError as e:
+            assert "timed out" in str(e)
+            out_of_time += 1
         evict()
         assert torch.equal(run(), want)
         check_device_status(device)
+        if out_of_time == 3:
+            return
+    raise AssertionError(f"{out_of_time} of 20 launches ran out of time")
 
 
 @pytest.mark.parametrize("T,dtype,packed", [(4, BF, False), (20, BF, False), (3, F32, False),

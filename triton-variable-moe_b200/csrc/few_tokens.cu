@@ -253,13 +253,14 @@ __device__ __forceinline__ bool ring_wait(uint32_t bar, uint32_t parity, volatil
   if (__all_sync(0xffffffffu, brief ? mbar_test_wait(bar, parity) : mbar_try_wait(bar, parity)))
     return true;
   const uint64_t t0 = global_timer_ns();
-  while (!__all_sync(0xffffffffu,
-                     brief ? mbar_test_wait(bar, parity) : mbar_try_wait(bar, parity))) {
-    if (__any_sync(0xffffffffu, *abort || global_timer_ns() - t0 > limit)) {
+  do {
+    // (+ 1: the timer may stand still for longer than a small limit)
+    if (__any_sync(0xffffffffu, *abort || global_timer_ns() - t0 + 1 >= limit)) {
       *abort = 1;
       return false;
     }
-  }
+  } while (!__all_sync(0xffffffffu,
+                       brief ? mbar_test_wait(bar, parity) : mbar_try_wait(bar, parity)));
   return true;
 }
 
