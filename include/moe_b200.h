@@ -529,7 +529,10 @@ MOE_API int moe_ep_combine(void* const* peers, int64_t ld_peer, const int32_t* o
  *   in fp32 with an error of a few 2^-22 of 55 (fp16: 279) scales times the sum of
  *   |x|, whatever the codes.
  *   workspace: moe_few_tokens_workspace_bytes(...) bytes, 16-byte aligned, any
- *   contents; one per call that may run at the same time.
+ *   contents; one per call that may run at the same time.  For each of
+ *   num_tokens * top_k rows about 4 max_expert_width bytes, and 4 (hidden +
+ *   max_expert_width) more up to 16 times, as long as the larger part of these stays
+ *   within 64 MB: 100 MB at 64 tokens of 4096, top 8, experts of up to 2048.
  * num_tokens = 0 launches nothing.  moe_few_tokens_workspace_bytes returns -1
  * for sizes out of range.
  */
@@ -598,9 +601,9 @@ MOE_API int moe_int4_dequantize(const void* packed, const void* scales, int64_t 
  * moe_grouped_gemv_down_int4 is down = 1 with the weight's row_offsets (HOST,
  * num_experts + 1; NULL for a single expert) in place of blocks and groups: each
  * expert's weight offsets have to be its rows, and no expert depends on another's.
- * workspace:
- * moe_grouped_gemv_int4_workspace_bytes(...) bytes, as moe_few_tokens' (-1 for
- * sizes out of range).
+ * workspace: moe_grouped_gemv_int4_workspace_bytes(...) bytes, as moe_few_tokens' (-1
+ * for sizes out of range): 4 bytes an output element (SwiGLU 8; columns in whole
+ * tiles of 128), up to 16 times that to 64 MB in all; 512 MB at 32768 rows of 4096.
  */
 MOE_API int64_t moe_grouped_gemv_int4_workspace_bytes(int64_t rows, int64_t hidden,
                                                       int64_t max_expert_width, int activation,

@@ -917,7 +917,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int c = 0; c < p.cluster; ++c) {
           cluster.map_shared_rank(sel_s, c)[t * p.k + lane] = static_cast<uint8_t>(sel);
           cluster.map_shared_rank(wgt_s, c)[t * p.k + lane] = wgt;
-          // (32-bit words: 64-bit atomics of several CTAs on one shared word lose bits)
+          // (32-bit words: in clusters of 2 to 8 CTAs 64-bit ORs through these addresses
+          // lost bits in every word of 512,000, 32-bit ones in none; why is not known)
           atomicOr(cluster.map_shared_rank(mask32, c) + 2 * sel + (t >> 5), 1u << (t & 31));
         }
       }
@@ -1285,8 +1286,8 @@ __global__ void __launch_bounds__(kSumThreads) few_sum_kernel(const __grid_const
 // ---- 4-bit products of rows grouped by expert --------------------------------
 // The up or down product by itself: its units are (expert, 8 rows, tile, slice), the
 // slices meet in the sum kernel, which also applies the activation and writes the zeros.
-// Bound by the instructions a code, as the layer's 4-bit products: 192 rows on 64 experts
-// of 1024 x 2048 take 37 us (1.8 TB/s); 6 rows on 16 small experts 10.5, two launches.
+// Bound by the work a code, as the layer's 4-bit products: 192 rows on 64 experts of
+// 1024 x 2048 take 37.5 us (1.8 TB/s); 6 rows on 16 small experts 10.7, two launches.
 struct GroupParams {
   const void* x;
   long long ldx;

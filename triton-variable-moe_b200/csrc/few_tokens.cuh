@@ -262,6 +262,26 @@ struct Matrix {
   int gated;
 };
 
+// Where the copies of a dense strip are: the step at row k, then every `rows` further.
+template <int STAGE>
+struct BoxCursor {
+  int col, jump, row;
+  __device__ __forceinline__ void set(const Matrix&, const Strip& s, int k) {
+    col = s.col;
+    jump = s.jump;
+    row = s.row + k;
+  }
+  template <int ROWS>
+  __device__ __forceinline__ void next(const Matrix&) {
+    row += ROWS;
+  }
+  __device__ __forceinline__ void issue(const Matrix& m, uint32_t stage, uint32_t bar) const {
+    expect_bytes(bar, STAGE);
+    box_load(stage, m.map, col, row, bar);
+    if (m.gated) box_load(stage + STAGE / 2, m.map, col + jump, row, bar);
+  }
+};
+
 // 16-bit weights, row-major.  One step is a box of 32 rows x 64 columns, 128-byte
 // swizzled (gated: two of 32 columns, 64-byte swizzled).  Lane t = lane % 4 has
 // reduction rows 16 s + 4 t .. + 3 as its k slots of multiply s: for t < 2 the
@@ -299,24 +319,7 @@ struct Dense16 {
       }
     }
   };
-  // Where the copies of a strip are: the step at row k, then every `rows` further.
-  struct Cursor {
-    int col, jump, row;
-    __device__ __forceinline__ void set(const Matrix&, const Strip& s, int k) {
-      col = s.col;
-      jump = s.jump;
-      row = s.row + k;
-    }
-    template <int ROWS>
-    __device__ __forceinline__ void next(const Matrix&) {
-      row += ROWS;
-    }
-    __device__ __forceinline__ void issue(const Matrix& m, uint32_t stage, uint32_t bar) const {
-      expect_bytes(bar, kStage);
-      box_load(stage, m.map, col, row, bar);
-      if (m.gated) box_load(stage + 2048, m.map, col + jump, row, bar);
-    }
-  };
+  using Cursor = BoxCursor<kStage>;
   // The vectors' elements of half h (16 rows) of a step.
   template <int NG, typename Src>
   struct Vectors {
@@ -614,24 +617,7 @@ struct Dense32 {
       off = gated ? (c >> 3) * 2048 + p * 1024 + (c & 7) * 16 : p * 2048 + c * 16;
     }
   };
-  // Where the copies of a strip are: the step at row k, then every `rows` further.
-  struct Cursor {
-    int col, jump, row;
-    __device__ __forceinline__ void set(const Matrix&, const Strip& s, int k) {
-      col = s.col;
-      jump = s.jump;
-      row = s.row + k;
-    }
-    template <int ROWS>
-    __device__ __forceinline__ void next(const Matrix&) {
-      row += ROWS;
-    }
-    __device__ __forceinline__ void issue(const Matrix& m, uint32_t stage, uint32_t bar) const {
-      expect_bytes(bar, kStage);
-      box_load(stage, m.map, col, row, bar);
-      if (m.gated) box_load(stage + 2048, m.map, col + jump, row, bar);
-    }
-  };
+  using Cursor = BoxCursor<kStage>;
   template <int NG, typename Src>
   struct Vectors {
     const float* r[4 * NG];  // at this half-warp's first row
