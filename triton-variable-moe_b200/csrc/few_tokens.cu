@@ -1320,9 +1320,11 @@ struct alignas(16) GroupSmem {
 };
 static_assert(sizeof(GroupSmem) % 16 == 0, "16-byte vectors follow");
 
-template <typename L, int NG>
+// ROWS: PackedRows for the down product, NoRows for up (a kilobyte of arguments is 0.7 us a
+// launch on the host).
+template <typename L, int NG, typename ROWS>
 __global__ void __launch_bounds__(kThreads, 1)
-    few_group_kernel(const __grid_constant__ GroupParams p, const __grid_constant__ PackedRows rows) {
+    few_group_kernel(const __grid_constant__ GroupParams p, const __grid_constant__ ROWS rows) {
   using T = typename L::Elem;
   constexpr int TOK = L::template kTokens<NG>, kRound = kTeam * L::kStep;
   extern __shared__ __align__(1024) unsigned char raw[];
@@ -1344,7 +1346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   const int outputs = 1 << outputs_log2<L>(p.act), teams = gridDim.x * kTeams;
   if (wid == 0) {  // as find_active
-    if (p.down) {
+    if constexpr (std::is_same_v<ROWS, PackedRows>) {
       find_packed(rows, s.off, p.E, p.total, p.act, p.shift, p.blocks, p.groups, s.kb, s.sg, s.fits);
       __syncwarp();
     }
@@ -1731,12 +1733,12 @@ int layer_for_tokens(LayerParams& p, cudaStream_t st) {
                                           : launch_layer<L, 2>(p, {}, st);
 }
 
-template <typename L, int NG>
-int launch_group(const GroupParams& p, const PackedRows& rows, cudaStream_t st) {
+template <typename L, int NG, typename ROWS>
+int launch_group(const GroupParams& p, const ROWS& rows, cudaStream_t st) {
   static std::atomic<unsigned long long> ok{0};
   const int dev = current_device();
   if (dev < 0) return kStatusCuda;
-  auto* kernel = few_group_kernel<L, NG>;
+  auto* kernel = few_group_kernel<L, NG, ROWS>;
   auto* sum = few_group_sum_kernel<L>;
   if (!allow_smem(kernel, ok, dev)) return kStatusCuda;
   cudaLaunchAttribute attr[1];
@@ -1898,6 +1900,17 @@ long long grouped_int4_workspace(long long rows, long long H, long long max_widt
 
 namespace {
 
+template <typename ROWS>
+int group_for_type(const GroupParams& p, const ROWS& rows, bool wide, int dtype, cudaStream_t st) {
+  if (dtype == 0)
+    return wide ? launch_group<Int4<__nv_bfloat16, 128>, 1>(p, rows, st)
+                : launch_group<Int4<__nv_bfloat16, 64>, 1>(p, rows, st);
+  if (dtype == 1)
+    return wide ? launch_group<Int4<__half, 128>, 1>(p, rows, st)
+                : launch_group<Int4<__half, 64>, 1>(p, rows, st);
+  return kStatusUnsupported;
+}
+
 int run_group(const void* x, long long rows, long long ldx, const void* w, const void* s,
               int group, long long blocks, long long groups, const PackedRows& rows_w, long long H,
               long long total, const int* tok_off, const int* off, const int* tok_cnt, int E,
@@ -1927,13 +1940,8 @@ int run_group(const void* x, long long rows, long long ldx, const void* w, const
   p.max_slices = slice_limit(rows * p.ldp);
   p.out = out; p.ldo = ldo; p.status = status; p.wait_ns = wait_ns();
   const bool wide = wide_tiles(E, rows, down ? H : act == ACT_SWIGLU ? 2 * max_width : max_width);
-  if (dtype == 0)
-    return wide ? launch_group<Int4<__nv_bfloat16, 128>, 1>(p, rows_w, st)
-                : launch_group<Int4<__nv_bfloat16, 64>, 1>(p, rows_w, st);
-  if (dtype == 1)
-    return wide ? launch_group<Int4<__half, 128>, 1>(p, rows_w, st)
-                : launch_group<Int4<__half, 64>, 1>(p, rows_w, st);
-  return kStatusUnsupported;
+  return down ? group_for_type(p, rows_w, wide, dtype, st)
+              : group_for_type(p, NoRows{}, wide, dtype, st);
 }
 
 }  // namespace

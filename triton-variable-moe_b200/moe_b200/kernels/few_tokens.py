@@ -158,16 +158,19 @@ def moe_few_tokens(
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     with on_device(dev):
         ev = _ops._ev_begin()
-        tail = (total, off.data_ptr(), max_expert_width, top_k, 1 if norm_topk_prob else 0, act,
-                out.data_ptr(), H, ws.data_ptr(), ws_bytes, dt_code, status_buffer(dev).data_ptr(),
-                stream_of(dev))
-        ldx = x.stride(0) if T > 1 else H
         if packed:
             rc = lib.moe_few_tokens_int4(
-                x.data_ptr(), T, ldx, H, pr, DTYPE_CODE[rdt], E, p1, w1.scales.data_ptr(), p2,
-                w2.scales.data_ptr(), group, w2._host_offsets, *tail)
+                x.data_ptr(), T, x.stride(0) if T > 1 else H, H, pr, DTYPE_CODE[rdt], E, p1,
+                w1.scales.data_ptr(), p2, w2.scales.data_ptr(), group, w2._host_offsets, total,
+                off.data_ptr(), max_expert_width, top_k, 1 if norm_topk_prob else 0, act,
+                out.data_ptr(), H, ws.data_ptr(), ws_bytes, dt_code, status_buffer(dev).data_ptr(),
+                stream_of(dev))
         else:
-            rc = lib.moe_few_tokens(x.data_ptr(), T, ldx, H, pr, E, p1, None, p2, None, 0, 0, 0, *tail)
+            rc = lib.moe_few_tokens(
+                x.data_ptr(), T, x.stride(0) if T > 1 else H, H, pr, E, p1, None, p2, None, 0, 0, 0,
+                total, off.data_ptr(), max_expert_width, top_k, 1 if norm_topk_prob else 0, act,
+                out.data_ptr(), H, ws.data_ptr(), ws_bytes, dt_code, status_buffer(dev).data_ptr(),
+                stream_of(dev))
         _ops._ev_end(ev, "few_tokens")
     if rc:
         check(rc, "moe_few_tokens")

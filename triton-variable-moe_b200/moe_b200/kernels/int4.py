@@ -51,15 +51,17 @@ def eager_only(fn):
 
 def refuse_tangent(name: str, *tensors: torch.Tensor) -> None:
     """Forward-mode derivatives, which torch.no_grad() leaves on."""
-    if forward_ad._current_level >= 0:
-        for t in tensors:
-            if forward_ad.unpack_dual(t).tangent is not None:
-                raise RuntimeError(f"{name} has no forward-mode derivative, and an argument has a "
-                                   "tangent: pass its primal value")
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has no forward-mode derivative, and an argument has a "
+                               "tangent: pass its primal value")
 
 
 def refuse_grad(name: str, *tensors: torch.Tensor) -> None:
-    refuse_tangent(name, *tensors)
+    if forward_ad._current_level >= 0:
+        refuse_tangent(name, *tensors)
     if torch.is_grad_enabled():
         for t in tensors:
             if t.requires_grad:
@@ -333,16 +335,19 @@ def _gemv(name, x, q, tok_off, w_off, expert_widths, tok_cnt, hidden, max_width,
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     with on_device(dev):
         ev = _ev_begin()
-        head = (ptr(x), rows, x.stride(0) if rows > 1 else x.shape[1], ptr(q.packed), ptr(q.scales),
-                q.group_size)
-        offs = (ptr(tok_off), ptr(w_off), ptr(tok_cnt), E, max_width)
-        tail = (ptr(out), out_cols, ptr(ws), ws_bytes, DTYPE_CODE[x.dtype],
-                ptr(status_buffer(dev)), stream_of(dev))
+        ldx = x.stride(0) if rows > 1 else x.shape[1]
         if down:
-            rc = lib.moe_grouped_gemv_down_int4(*head, q._host_offsets, hidden, q.rows, *offs, *tail)
+            rc = lib.moe_grouped_gemv_down_int4(
+                ptr(x), rows, ldx, ptr(q.packed), ptr(q.scales), q.group_size, q._host_offsets,
+                hidden, q.rows, ptr(tok_off), ptr(w_off), ptr(tok_cnt), E, max_width, ptr(out),
+                out_cols, ptr(ws), ws_bytes, DTYPE_CODE[x.dtype], ptr(status_buffer(dev)),
+                stream_of(dev))
         else:
-            rc = lib.moe_grouped_gemv_int4(*head, q.packed.shape[0], q.scales.shape[0], hidden,
-                                           q.cols, *offs, ACT_CODE[activation], 0, *tail)
+            rc = lib.moe_grouped_gemv_int4(
+                ptr(x), rows, ldx, ptr(q.packed), ptr(q.scales), q.group_size, q.packed.shape[0],
+                q.scales.shape[0], hidden, q.cols, ptr(tok_off), ptr(w_off), ptr(tok_cnt), E,
+                max_width, ACT_CODE[activation], 0, ptr(out), out_cols, ptr(ws), ws_bytes,
+                DTYPE_CODE[x.dtype], ptr(status_buffer(dev)), stream_of(dev))
         _ev_end(ev, name)
     check(rc, name)
     _count(2)
