@@ -245,13 +245,13 @@ __device__ __forceinline__ void down_strip(Strip& s, const Active& a, int e, int
 }
 
 // Bounded wait of a warp for a phase of a copy barrier.  false, for all lanes: it ran
-// out, here or in another warp (abort).
-__device__ __forceinline__ bool ring_wait(uint32_t bar, uint32_t parity, volatile int* abort,
+// out, here or in another warp (abort).  A poll may suspend the warp, for longer than a
+// copy takes: not with a limit below a millisecond.  (The part after the first poll is
+// hardly ever run, and kept out of the loops.)
+__device__ __noinline__ bool ring_wait_on(uint32_t bar, uint32_t parity, volatile int* abort,
                                           uint64_t limit) {
-  // A poll may suspend the warp, for longer than a copy takes: not with a limit below that.
   const bool brief = limit < 1000000;
-  if (__all_sync(0xffffffffu, brief ? mbar_test_wait(bar, parity) : mbar_try_wait(bar, parity)))
-    return true;
+  if (brief && __all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
   const uint64_t t0 = global_timer_ns();
   do {
     // (+ 1: the timer may stand still for longer than a small limit)
@@ -262,6 +262,11 @@ __device__ __forceinline__ bool ring_wait(uint32_t bar, uint32_t parity, volatil
   } while (!__all_sync(0xffffffffu,
                        brief ? mbar_test_wait(bar, parity) : mbar_try_wait(bar, parity)));
   return true;
+}
+__device__ __forceinline__ bool ring_wait(uint32_t bar, uint32_t parity, volatile int* abort,
+                                          uint64_t limit) {
+  return (limit >= 1000000 && __all_sync(0xffffffffu, mbar_try_wait(bar, parity))) ||
+         ring_wait_on(bar, parity, abort, limit);
 }
 
 // Runs the `total` units of a team.  Every warp copies its steps (begin + (wr + 4 j)
@@ -664,7 +669,9 @@ __device__ __forceinline__ void choose(const LayerParams& p, cg::cluster_group& 
 // here a cluster of 8 CTAs has 8 of them, each CTA an eighth of the hidden size and
 // then one token to choose for.  The up kernel then needs no clusters and runs on all
 // SMs.
-template <typename T>
+// R: type of the router, T's or fp32 (an instance of its own: as a branch it cost 17 tokens
+// of 1104 0.2 us).
+template <typename T, typename R>
 __global__ void __launch_bounds__(kThreads, 1) few_router_kernel(const __grid_constant__ LayerParams p) {
   extern __shared__ __align__(1024) unsigned char raw[];
   cg::cluster_group cluster = cg::this_cluster();
@@ -678,7 +685,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_router_kernel(const __grid_co
   const int per = ceil_div(ceil_div(p.H, 32), kMaxCluster) * 32;
   const T* x = static_cast<const T*>(p.x) + t0 * p.ldx;
   const int k_lo = min(rank * per, p.H), k_hi = min((rank + 1) * per, p.H);
-  if (sizeof(T) == 2 && p.router_fp32)
+  if constexpr (!std::is_same_v<R, T>)
     partial_logits_fp32<T>(p, x, count, k_lo, k_hi, log, lde);
   else
     partial_logits<T>(p, x, count, k_lo, k_hi, part, log, lde);
@@ -706,6 +713,7 @@ struct alignas(16) UpSmem {
   int kb[kMaxExperts];    // packed w2 (otherwise 0): first block row, first group,
   int sg[kMaxExperts];
   int fits[kMaxExperts];  // and whether the expert lies in it
+  int row[kMaxExperts + 1];  // its row offsets, where they are known
 };
 static_assert(sizeof(UpSmem) % 16 == 0, "16-byte vectors follow");
 
@@ -724,12 +732,13 @@ __device__ __forceinline__ bool expert_width(int a, int b, int total, int max_wi
 }
 
 // One warp: where each expert's rows of a packed w2 start, and whether they are the
-// call's.  Known rows: the expert's offsets have to be its segment's.  Otherwise the
+// call's.  Known rows (in shared memory: read from the arguments here, a lane each, they
+// cost the down product of 192 rows 0.6 us): the expert's offsets have to be its segment's.  Otherwise the
 // segments are those of the offsets, as far as these are columns of w1: nothing says
 // where the experts after others start, and they are refused.
-__device__ __forceinline__ void find_packed(const PackedRows& rows, const int* off, int E, int total,
-                                            int act, int shift, int blocks2, int groups2, int* kb_s,
-                                            int* sg_s, int* fits) {
+__device__ __forceinline__ void find_packed(bool known, const int* row, const int* off, int E,
+                                            int total, int act, int shift, int blocks2, int groups2,
+                                            int* kb_s, int* sg_s, int* fits) {
   const int lane = threadIdx.x & 31, gated = act == ACT_SWIGLU ? 1 : 0;
   int kb = 0, sg = 0;
   bool lost = false;
@@ -743,8 +752,8 @@ __device__ __forceinline__ void find_packed(const PackedRows& rows, const int* o
     }
     bool ok;
     int w;
-    if (rows.n > 0) {
-      const int lo = e < E ? rows.row[e] : 0, hi = e < E ? rows.row[e + 1] : 0;
+    if (known) {
+      const int lo = e < E ? row[e] : 0, hi = e < E ? row[e + 1] : 0;
       ok = a == lo << gated && b == hi << gated;
       w = hi - lo;
     } else {
@@ -875,7 +884,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (!p.sel) asm volatile("griddepcontrol.wait;" ::: "memory");
   // every block of this grid runs by the time the last one gets here
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  for (int e = tid; e <= p.E; e += kThreads) s.off[e] = p.off[e];
+  for (int e = tid; e <= p.E; e += kThreads) {
+    s.off[e] = p.off[e];
+    if constexpr (L::kPacked) s.row[e] = rows2.row[e];
+  }
   for (int e = tid; e < p.E; e += kThreads) {
     s.mask[e] = 0;
     s.kb[e] = s.sg[e] = 0;
@@ -888,8 +900,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto packed = [&]() {  // (one warp, while others route)
     if constexpr (L::kPacked)
       if (wid == kWarps - 1)
-        find_packed(rows2, s.off, p.E, p.total, p.act, p.shift, p.blocks2, p.groups2, s.kb, s.sg,
-                    s.fits);
+        find_packed(rows2.n > 0, s.row, s.off, p.E, p.total, p.act, p.shift, p.blocks2, p.groups2,
+                    s.kb, s.sg, s.fits);
   };
   if (p.sel) {
     __syncthreads();
@@ -1317,6 +1329,7 @@ struct alignas(16) GroupSmem {
   int kb[kMaxExperts];  // as UpSmem's
   int sg[kMaxExperts];
   int fits[kMaxExperts];
+  int row[kMaxExperts + 1];
 };
 static_assert(sizeof(GroupSmem) % 16 == 0, "16-byte vectors follow");
 
@@ -1336,6 +1349,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   for (int e = tid; e <= p.E; e += kThreads) {
     s.off[e] = p.off[e];
     s.tok[e] = p.tok_off[e];
+    if constexpr (std::is_same_v<ROWS, PackedRows>) s.row[e] = rows.row[e];
     if (e < p.E) {
       s.cnt[e] = p.tok_cnt ? p.tok_cnt[e] : 0x7fffffff;
       s.kb[e] = s.sg[e] = 0;
@@ -1347,7 +1361,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int outputs = 1 << outputs_log2<L>(p.act), teams = gridDim.x * kTeams;
   if (wid == 0) {  // as find_active
     if constexpr (std::is_same_v<ROWS, PackedRows>) {
-      find_packed(rows, s.off, p.E, p.total, p.act, p.shift, p.blocks, p.groups, s.kb, s.sg, s.fits);
+      find_packed(rows.n > 0, s.row, s.off, p.E, p.total, p.act, p.shift, p.blocks, p.groups, s.kb,
+                  s.sg, s.fits);
       __syncwarp();
     }
     int active = 0;
@@ -1693,9 +1708,9 @@ int launch_layer(LayerParams& p, const RowsOf<L>& rows2, cudaStream_t st) {
   cfg.stream = st;
   cfg.attrs = attr;
   if (router) {
-    static std::atomic<unsigned long long> router_ok{0};
-    auto* kernel = few_router_kernel<T>;
-    if (!allow_smem(kernel, router_ok, dev)) return kStatusCuda;
+    static std::atomic<unsigned long long> router_ok[2];
+    auto* kernel = p.router_fp32 ? few_router_kernel<T, float> : few_router_kernel<T, T>;
+    if (!allow_smem(kernel, router_ok[p.router_fp32], dev)) return kStatusCuda;
     attr[1].val.clusterDim.x = kMaxCluster;
     cfg.gridDim = dim3(static_cast<unsigned>(ceil_div(p.T, kMaxCluster) * kMaxCluster));
     cfg.blockDim = dim3(kThreads);
@@ -1868,8 +1883,7 @@ int few_tokens(const void* x, long long T, long long ldx, long long H, const voi
                long long blocks2, long long groups2, long long total, const int* off,
                long long max_width, int k, int norm, int act, void* out, long long ldo, void* ws,
                long long ws_bytes, int dtype, int* status, cudaStream_t st) {
-  PackedRows unknown;
-  unknown.n = 0;
+  const PackedRows unknown{};
   return run_layer(x, T, ldx, H, router, dtype, E, w1, s1, w2, s2, group, blocks2, groups2, unknown,
                    total, off, max_width, k, norm, act, out, ldo, ws, ws_bytes, dtype, status, st);
 }
@@ -1879,7 +1893,7 @@ int few_tokens_int4(const void* x, long long T, long long ldx, long long H, cons
                     const void* s2, int group, const int32_t* rows2, long long total, const int* off,
                     long long max_width, int k, int norm, int act, void* out, long long ldo,
                     void* ws, long long ws_bytes, int dtype, int* status, cudaStream_t st) {
-  PackedRows rows;
+  PackedRows rows{};
   long long blocks = 0, groups = 0;
   if (act < 0 || act > 2 || total % (act == ACT_SWIGLU ? 32 : 16) != 0) return kStatusBadArg;
   const int rc = packed_rows(rows2, E, act == ACT_SWIGLU ? total / 2 : total, group, &rows, &blocks,
@@ -1951,8 +1965,7 @@ int grouped_int4(const void* x, long long rows, long long ldx, const void* w, co
                  const int* tok_off, const int* off, const int* tok_cnt, int E,
                  long long max_width, int act, int down, void* out, long long ldo, void* ws,
                  long long ws_bytes, int dtype, int* status, cudaStream_t st) {
-  PackedRows unknown;
-  unknown.n = 0;
+  const PackedRows unknown{};
   return run_group(x, rows, ldx, w, s, group, blocks, groups, unknown, H, total, tok_off, off,
                    tok_cnt, E, max_width, act, down, out, ldo, ws, ws_bytes, dtype, status, st);
 }
@@ -1962,7 +1975,7 @@ int grouped_down_int4(const void* x, long long rows, long long ldx, const void* 
                       const int* tok_off, const int* off, const int* tok_cnt, int E,
                       long long max_width, void* out, long long ldo, void* ws, long long ws_bytes,
                       int dtype, int* status, cudaStream_t st) {
-  PackedRows r;
+  PackedRows r{};
   long long blocks = 0, groups = 0;
   const int rc = packed_rows(rows_w, E, total, group, &r, &blocks, &groups);
   if (rc != kStatusOk) return rc;
