@@ -28,9 +28,9 @@
 //                partial sums in a fixed order, weights them and writes the
 //                output: results do not depend on timing.  (More than 8 tokens: a
 //                sum kernel after it.)
-// Measured: one token of 768 on 16 experts 18.3 us, all latency; 5 tokens on 64 experts of
-// 2048 x 1024 69 us (3.8 TB/s over the call, 5.2 while it streams); 64 tokens of 4096 on
-// 128 experts 424 us, 5.6 TB/s where a copy reaches 6.6.  (Prefetching the down weights to
+// Measured: one token of 768 on 16 experts 18.5 us, all latency; 5 tokens on 64 experts of
+// 2048 x 1024 69.5 us (3.8 TB/s over the call, 5.2 while it streams); 64 tokens of 4096 on
+// 128 experts 423 us, 5.6 TB/s where a copy reaches 6.6.  (Prefetching the down weights to
 // L2 as the up kernel ends: 69.3 to 69.9 us at 16 MB, 73 at 64 MB, as other teams still
 // stream theirs.)
 // No block waits for another but at hardware barriers and the grid dependency
