@@ -523,7 +523,8 @@ MOE_API int moe_ep_combine(void* const* peers, int64_t ld_peer, const int32_t* o
  * (HOST, num_experts + 1; NULL for a single expert) in place of w2_blocks and
  * w2_groups: an expert whose offsets are not its rows of w2 adds nothing and sets
  * the status, and the others are right.  The router is in router_dtype: dtype or
- * fp32, as in an fp32 layer whose experts alone were quantised.
+ * fp32, as in an fp32 layer whose experts alone were quantised (then a launch more up
+ * to 8 tokens).
  *   In fp16 an intermediate above 65504 is infinite.  4-bit products make a NaN of an
  *   infinite x or intermediate, and in bf16 can of one from 2^115 on; they are summed
  *   in fp32 with an error of a few 2^-22 of 55 (fp16: 279) scales times the sum of
@@ -551,7 +552,8 @@ MOE_API int moe_few_tokens(const void* x, int64_t num_tokens, int64_t ld_x, int6
 MOE_API int moe_few_tokens_int4(const void* x, int64_t num_tokens, int64_t ld_x, int64_t hidden,
                                 const void* router, int router_dtype, int num_experts,
                                 const void* w1, const void* w1_scales, const void* w2,
-                                const void* w2_scales, int group, const int32_t* w2_row_offsets, int64_t total_width,
+                                const void* w2_scales, int group,
+                                const int32_t* w2_row_offsets, int64_t total_width,
                                 const int32_t* expert_weight_offsets, int64_t max_expert_width,
                                 int top_k, int normalize, int activation, void* out,
                                 int64_t ld_out, void* workspace, int64_t workspace_bytes,

@@ -1,4 +1,5 @@
-// The MoE layer for a few tokens (decode), in two kernels (four above 8 tokens), and
+// The MoE layer for a few tokens (decode), in two kernels (four above 8 tokens; the router
+// kernel also runs for an fp32 router beside 16-bit x), and
 // the products of 4-bit expert weights with rows grouped by expert, in two.
 //
 // Mathematics, for token t and its k experts S(t):
@@ -280,7 +281,8 @@ using Int = std::integral_constant<int, N>;
 template <typename L, int NG, typename MakeUnit, typename MakeSource, typename Finish>
 __device__ __forceinline__ void run_units(int total, const Matrix& m,
                                           unsigned char* work, float* red, Common& c,
-                                          uint64_t limit, MakeUnit unit, MakeSource source, Finish finish) {
+                                          uint64_t limit, MakeUnit unit, MakeSource source,
+                                          Finish finish) {
   constexpr int kRows = kTeam * L::kStep, TOK = L::template kTokens<NG>;
   constexpr int D = L::template kDepth<NG>;
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
@@ -733,9 +735,9 @@ __device__ __forceinline__ bool expert_width(int a, int b, int total, int max_wi
 
 // One warp: where each expert's rows of a packed w2 start, and whether they are the
 // call's.  Known rows (in shared memory: read from the arguments here, a lane each, they
-// cost the down product of 192 rows 0.6 us): the expert's offsets have to be its segment's.  Otherwise the
-// segments are those of the offsets, as far as these are columns of w1: nothing says
-// where the experts after others start, and they are refused.
+// cost the down product of 192 rows 0.6 us): the expert's offsets have to be its
+// segment's.  Otherwise the segments are those of the offsets, as far as these are columns
+// of w1: nothing says where the experts after others start, and they are refused.
 __device__ __forceinline__ void find_packed(bool known, const int* row, const int* off, int E,
                                             int total, int act, int shift, int blocks2, int groups2,
                                             int* kb_s, int* sg_s, int* fits) {
@@ -1299,7 +1301,7 @@ __global__ void __launch_bounds__(kSumThreads) few_sum_kernel(const __grid_const
 // The up or down product by itself: its units are (expert, 8 rows, tile, slice), the
 // slices meet in the sum kernel, which also applies the activation and writes the zeros.
 // Bound by the work a code, as the layer's 4-bit products: 192 rows on 64 experts of
-// 1024 x 2048 take 37.5 us (1.8 TB/s); 6 rows on 16 small experts 10.7, two launches.
+// 1024 x 2048 take 37.2 us (1.8 TB/s); 6 rows on 16 small experts 10.3, two launches.
 struct GroupParams {
   const void* x;
   long long ldx;

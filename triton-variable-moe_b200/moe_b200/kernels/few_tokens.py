@@ -1,5 +1,5 @@
 """The whole MoE layer for a few tokens (decode), in two launches (four above 8
-tokens).
+tokens; three up to 8 with an fp32 router beside 4-bit experts).
 
 No counterpart in the reference: its layer (triton_moe/moe.py:148-249) sorts the
 tokens and pads every expert's rows to a tile, which at a few tokens is mostly
